@@ -304,6 +304,51 @@ typedef struct LcbsaRowJob {
 int lcbsa_norm_rope_jobs(const LcbsaRowJob* jobs, int n_jobs, float eps, void* stream);
 
 /*
+ * Dense attention with shaped scores, beside the block-sparse one: the layers without block sparsity, the attention to packed prompts, the
+ * text encoder and an autoregressive model next to the DiT.  q [B, Hq, Sq, D], k and v [B, Hk, Sk, D] with Hq a multiple of
+ * Hk (query head h reads key head h / (Hq / Hk)), bf16 or fp16, head_dim 64 or 128, any strides under the 16-byte rules, any lengths.
+ *
+ *   s_ij = scale q_i . k_j    c_ij = cap tanh(s_ij / cap) (cap 0: s_ij)    x_ij = c_ij - slopes[h] |pos_i - j| (slopes null: c_ij)
+ *   out_i = sum_j softmax_j(x_ij) v_j over the keys that query i sees; a query that sees none: out 0, lse -inf.
+ *
+ * What a query sees.  Without cu_q the queries and the keys of a batch entry are one document, of k_len[b] keys where k_len is given
+ * (a padded cache), else of Sk.  With cu_q, cu_k (int32, ascending, docs + 1 each, the batch entries cu_stride apart, 0: the same for all)
+ * document d has the queries cu_q[d] .. cu_q[d + 1] - 1 and the keys cu_k[d] .. cu_k[d + 1] - 1, and a query sees keys of its own
+ * document alone; queries before the first document and behind the last see none.  pos_i, the query's place among the keys, puts the last
+ * query of a document at its last key.  causal: keys behind pos_i are hidden, but for the first prefix[d] of the document (int32, the batch
+ * entries prefix_stride apart; null: none).  Bounds outside the tensors are clamped, never followed.
+ * Keys and values that no query of a call sees, and those hidden from a query, may hold anything, infinities and NaN included.
+ *
+ * lse: fp32 dense [B, Hq, Sq], natural log, nullable in the forward.  A row with a NaN or +inf score is NaN, its lse too.
+ * The workspace (lcbsa_dense_attn_workspace_bytes, 256-byte aligned) belongs to one call until its kernels have run.
+ * The backward takes the forward's out and lse and writes every row of dq, dk and dv; no atomics, so two calls give the same
+ * bits; the slopes are constants.
+ */
+typedef struct LcbsaScores {
+    float scale, cap;
+    const float* slopes;     /* [Hq] or null */
+    const int32_t *cu_q, *cu_k, *k_len, *prefix;
+    int64_t cu_stride, prefix_stride;
+    int32_t docs, causal;
+} LcbsaScores;
+size_t lcbsa_dense_attn_workspace_bytes(const LcbsaTensor* q, const LcbsaTensor* k, int backward);
+int lcbsa_dense_attn_fwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaScores* scores, const LcbsaTensor* out,
+                         float* lse, void* workspace, size_t workspace_bytes, void* stream);
+int lcbsa_dense_attn_bwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaTensor* out, const LcbsaTensor* dout,
+                         const LcbsaScores* scores, const float* lse, const LcbsaTensor* dq, const LcbsaTensor* dk, const LcbsaTensor* dv,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions along one axis (the 3-D form over a latent grid is lcbsa_norm_rope) for one or two tensors [B, H_i, S, D] that share
+ * dtype, batch, S and D: q and k of a layer.  The first 2 * pairs dimensions turn, the others are copied; pairs are (2p, 2p + 1) with
+ * interleaved, else (p, p + pairs).  Pair p turns by position * turns[p] / 2^64 turns and is multiplied by factor; inverse turns the other way
+ * (the gradient).  positions: int32 or int64 (pos_bits) with the given strides, or null: offset + index of the token; any value.
+ * bf16 or fp16, head_dim a multiple of 8, pairs a multiple of 8 up to 128.  Outputs overlap neither the inputs nor each other.
+ */
+int lcbsa_rotary(const LcbsaTensor* x, const LcbsaTensor* out, int n, const uint64_t* turns, int pairs, int interleaved, int inverse,
+                 float factor, const void* positions, int pos_bits, int64_t pos_batch_stride, int64_t pos_stride, int64_t offset, void* stream);
+
+/*
  * Enqueue `count` device-to-device copies of `nbytes` each on `stream`: dst[i] <- src[i], one cudaMemcpyAsync per
  * slab, so the copy engines move them; a destination may be another GPU's memory mapped into this process
  * (symmetric memory, CUDA IPC).  The pointer arrays are host memory and are read before the call returns.

@@ -5,6 +5,7 @@
 #include <cstring>
 
 #include "common.cuh"
+#include "dense_common.cuh"
 
 namespace {
 
@@ -61,6 +62,25 @@ int check_tensor(const char* name, const LcbsaTensor* t, const LcbsaGrid* g) {
         if ((t->stride[i] * (long long)es) % 16 != 0 || t->stride[i] < 0)
             return fail(LCBSA_EINVAL, "%s: stride[%d] must be a non-negative multiple of 16 bytes", name, i);
     if ((t->size[3] * (long long)es) % 16 != 0) return fail(LCBSA_EINVAL, "%s: head_dim row must be a multiple of 16 bytes", name);
+    return LCBSA_OK;
+}
+
+// The same for a [B,H,S,D] operand without a grid; an empty tensor has no data.
+int check_rows(const char* name, const LcbsaTensor* t) {
+    if (!t) return fail(LCBSA_EINVAL, "%s: null tensor", name);
+    if (t->dtype != LCBSA_BF16 && t->dtype != LCBSA_FP16) return fail(t->dtype == LCBSA_FP32 ? LCBSA_EUNSUPPORTED : LCBSA_EINVAL, "%s: takes bf16 or fp16", name);
+    long long n = 1;
+    for (int i = 0; i < 4; ++i) {
+        if (t->size[i] < 0 || t->size[i] > 0x7fffffff) return fail(LCBSA_EINVAL, "%s: size[%d] is negative or above 2^31", name, i);
+        n = t->size[i] == 0 ? 0 : n;
+    }
+    if (n == 0) return LCBSA_OK;
+    if (!t->data) return fail(LCBSA_EINVAL, "%s: null tensor", name);
+    if (t->stride[3] != 1) return fail(LCBSA_EINVAL, "%s: the head_dim axis must be contiguous", name);
+    if (reinterpret_cast<uintptr_t>(t->data) % 16 != 0) return fail(LCBSA_EINVAL, "%s: data pointer not 16-byte aligned", name);
+    for (int i = 0; i < 3; ++i)
+        if ((t->stride[i] * 2) % 16 != 0 || t->stride[i] < 0) return fail(LCBSA_EINVAL, "%s: stride[%d] must be a non-negative multiple of 16 bytes", name, i);
+    if (t->size[3] % 8 != 0) return fail(LCBSA_EINVAL, "%s: head_dim row must be a multiple of 16 bytes", name);
     return LCBSA_OK;
 }
 
@@ -538,6 +558,130 @@ int lcbsa_norm_rope(const LcbsaTensor* x, const void* weight, const LcbsaGrid* g
                     const LcbsaTensor* out, void* stream) {
     if (!weight || !rope_tab) return fail(LCBSA_EINVAL, "norm_rope: null weight or rope table");
     return lcbsa_norm_rope_ex(x, weight, g, rope_tab, g ? g->T : 0, 0, eps, out, stream);
+}
+
+static int dense_args(const char* what, const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaScores* sc, lcbsa::DenseArgs* a) {
+    if (int rc = check_rows("q", q)) return rc;
+    if (int rc = check_rows("k", k)) return rc;
+    if (int rc = check_rows("v", v)) return rc;
+    if (!sc) return fail(LCBSA_EINVAL, "%s: null scores", what);
+    if (q->dtype != k->dtype || q->dtype != v->dtype) return fail(LCBSA_EINVAL, "%s: dtypes differ", what);
+    if (q->size[0] != k->size[0] || q->size[3] != k->size[3]) return fail(LCBSA_EINVAL, "%s: q and k disagree on batch or head_dim", what);
+    for (int i = 0; i < 4; ++i)
+        if (k->size[i] != v->size[i]) return fail(LCBSA_EINVAL, "%s: k and v have different shapes", what);
+    if (k->size[1] < 1 || q->size[1] % k->size[1] != 0)
+        return fail(LCBSA_EINVAL, "%s: %lld query heads do not share %lld key heads evenly", what, (long long)q->size[1], (long long)k->size[1]);
+    if (!std::isfinite(sc->scale) || !std::isfinite(sc->cap) || sc->cap < 0.f) return fail(LCBSA_EINVAL, "%s: scale must be finite, cap finite and not negative", what);
+    if ((sc->cu_q == nullptr) != (sc->cu_k == nullptr)) return fail(LCBSA_EINVAL, "%s: the documents of the queries and of the keys go together", what);
+    if (sc->cu_q && sc->k_len) return fail(LCBSA_EINVAL, "%s: documents and key lengths exclude each other", what);
+    if (sc->cu_q && (sc->docs < 1 || sc->cu_stride < 0)) return fail(LCBSA_EINVAL, "%s: documents need a number of at least 1 and a stride of at least 0", what);
+    if (sc->prefix && (!sc->causal || sc->prefix_stride < 0)) return fail(LCBSA_EINVAL, "%s: a prefix needs a causal order and a stride of at least 0", what);
+    a->dtype = q->dtype;
+    a->B = (int)q->size[0]; a->Hq = (int)q->size[1]; a->Hk = (int)k->size[1]; a->group = a->Hq / a->Hk; a->D = (int)q->size[3];
+    a->Sq = (int)q->size[2]; a->Sk = (int)k->size[2];
+    a->q = view_of(q); a->k = view_of(k); a->v = view_of(v);
+    a->mask = lcbsa::DenseMask{sc->cu_q, sc->cu_k, sc->k_len, sc->prefix, sc->docs, sc->causal != 0, sc->cu_stride, sc->prefix_stride};
+    a->scale = sc->scale; a->cap = sc->cap; a->slopes = sc->slopes;
+    const char* why = "";
+    if (!lcbsa::dense_supported(*a, &why)) return fail(LCBSA_EUNSUPPORTED, "%s: %s", what, why);
+    return LCBSA_OK;
+}
+
+// the sizes alone decide how much workspace a call needs
+static lcbsa::DenseArgs dense_sizes(const LcbsaTensor* q, const LcbsaTensor* k) {
+    lcbsa::DenseArgs a{};
+    a.dtype = q->dtype;
+    a.B = (int)q->size[0]; a.Hq = (int)q->size[1]; a.Hk = (int)k->size[1]; a.group = a.Hk > 0 ? a.Hq / a.Hk : 0; a.D = (int)q->size[3];
+    a.Sq = (int)q->size[2]; a.Sk = (int)k->size[2];
+    return a;
+}
+
+static int dense_workspace(const char* what, const void* ws, size_t have, size_t need) {
+    if (need == 0) return LCBSA_OK;
+    if (!ws || have < need) return fail(LCBSA_EWORKSPACE, "%s: workspace of %zu bytes, need %zu", what, have, need);
+    if (reinterpret_cast<uintptr_t>(ws) % 256 != 0) return fail(LCBSA_EINVAL, "%s: workspace not 256-byte aligned", what);
+    return LCBSA_OK;
+}
+
+static int same_shape(const char* what, const char* name, const LcbsaTensor* t, const LcbsaTensor* like) {
+    if (int rc = check_rows(name, t)) return rc;
+    if (t->dtype != like->dtype) return fail(LCBSA_EINVAL, "%s: dtypes differ", what);
+    for (int i = 0; i < 4; ++i)
+        if (t->size[i] != like->size[i]) return fail(LCBSA_EINVAL, "%s: %s has another shape than its input", what, name);
+    return LCBSA_OK;
+}
+
+size_t lcbsa_dense_attn_workspace_bytes(const LcbsaTensor* q, const LcbsaTensor* k, int backward) {
+    if (!q || !k) return 0;
+    const lcbsa::DenseArgs a = dense_sizes(q, k);
+    return backward ? lcbsa::dense_bwd_workspace_bytes(a) : lcbsa::dense_fwd_workspace_bytes(a);
+}
+
+int lcbsa_dense_attn_fwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaScores* scores, const LcbsaTensor* out,
+                         float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    lcbsa::DenseArgs a{};
+    if (int rc = dense_args("dense_attn", q, k, v, scores, &a)) return rc;
+    if (int rc = same_shape("dense_attn", "out", out, q)) return rc;
+    if (int rc = dense_workspace("dense_attn", workspace, workspace_bytes, lcbsa::dense_fwd_workspace_bytes(a))) return rc;
+    a.o = view_of(out);
+    a.lse = lse;
+    a.status = device_status_ptr();
+    if (!a.status) return fail(LCBSA_ECUDA, "dense_attn: cannot resolve the device status words");
+    const char* why = "";
+    cudaError_t e = lcbsa::launch_dense_fwd(a, workspace, static_cast<cudaStream_t>(stream), &why);
+    if (e != cudaSuccess) return cuda_fail(e, "dense_attn", why);
+    return LCBSA_OK;
+}
+
+int lcbsa_dense_attn_bwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaTensor* out, const LcbsaTensor* dout,
+                         const LcbsaScores* scores, const float* lse, const LcbsaTensor* dq, const LcbsaTensor* dk, const LcbsaTensor* dv,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+    lcbsa::DenseArgs a{};
+    if (int rc = dense_args("dense_attn_bwd", q, k, v, scores, &a)) return rc;
+    if (int rc = same_shape("dense_attn_bwd", "out", out, q)) return rc;
+    if (int rc = same_shape("dense_attn_bwd", "dout", dout, q)) return rc;
+    if (int rc = same_shape("dense_attn_bwd", "dq", dq, q)) return rc;
+    if (int rc = same_shape("dense_attn_bwd", "dk", dk, k)) return rc;
+    if (int rc = same_shape("dense_attn_bwd", "dv", dv, k)) return rc;
+    if (!lse && a.B * a.Hq * a.Sq > 0) return fail(LCBSA_EINVAL, "dense_attn_bwd: null lse");
+    if (int rc = dense_workspace("dense_attn_bwd", workspace, workspace_bytes, lcbsa::dense_bwd_workspace_bytes(a))) return rc;
+    a.o = view_of(out); a.dout = view_of(dout); a.dq = view_of(dq); a.dk = view_of(dk); a.dv = view_of(dv);
+    a.lse = const_cast<float*>(lse);
+    a.status = device_status_ptr();
+    if (!a.status) return fail(LCBSA_ECUDA, "dense_attn_bwd: cannot resolve the device status words");
+    const char* why = "";
+    cudaError_t e = lcbsa::launch_dense_bwd(a, workspace, static_cast<cudaStream_t>(stream), &why);
+    if (e != cudaSuccess) return cuda_fail(e, "dense_attn_bwd", why);
+    return LCBSA_OK;
+}
+
+int lcbsa_rotary(const LcbsaTensor* x, const LcbsaTensor* out, int n, const uint64_t* turns, int pairs, int interleaved, int inverse,
+                 float factor, const void* positions, int pos_bits, int64_t pos_batch_stride, int64_t pos_stride, int64_t offset, void* stream) {
+    if (!x || !out || n < 1 || n > lcbsa::kMaxRotaryJobs) return fail(LCBSA_EINVAL, "rotary: 1..%d tensors", lcbsa::kMaxRotaryJobs);
+    if (!turns || pairs < 8 || pairs > lcbsa::kMaxRotaryPairs || pairs % 8 != 0)
+        return fail(LCBSA_EINVAL, "rotary: pairs must be a multiple of 8 in 8..%d", lcbsa::kMaxRotaryPairs);
+    if (!std::isfinite(factor)) return fail(LCBSA_EINVAL, "rotary: factor is not finite");
+    if (positions && pos_bits != 32 && pos_bits != 64) return fail(LCBSA_EINVAL, "rotary: positions have 32 or 64 bits");
+    lcbsa::RotaryArgs P{};
+    P.n = n;
+    for (int i = 0; i < n; ++i) {
+        if (int rc = check_rows("rotary input", &x[i])) return rc;
+        if (int rc = same_shape("rotary", "rotary output", &out[i], &x[i])) return rc;
+        if (x[i].dtype != x[0].dtype || x[i].size[0] != x[0].size[0] || x[i].size[2] != x[0].size[2] || x[i].size[3] != x[0].size[3])
+            return fail(LCBSA_EINVAL, "rotary: the tensors of a call share dtype, batch, length and head_dim");
+        if (2 * pairs > x[i].size[3]) return fail(LCBSA_EINVAL, "rotary: %d turning dimensions of a head of %lld", 2 * pairs, (long long)x[i].size[3]);
+        P.job[i].x = view_of(&x[i]);
+        P.job[i].out = view_of(&out[i]);
+        P.job[i].H = (int)x[i].size[1];
+    }
+    memcpy(P.turns, turns, pairs * sizeof(uint64_t));
+    P.S = (int)x[0].size[2];
+    P.pairs = pairs; P.interleaved = interleaved != 0; P.inverse = inverse != 0; P.factor = factor;
+    P.pos = positions; P.pos64 = pos_bits == 64; P.pos_sb = pos_batch_stride; P.pos_ss = pos_stride; P.offset = offset;
+    const char* why = "";
+    cudaError_t e = lcbsa::launch_rotary(x[0].dtype, P, (int)x[0].size[0], (int)x[0].size[3], static_cast<cudaStream_t>(stream), &why);
+    if (e != cudaSuccess) return cuda_fail(e, "rotary", why);
+    return LCBSA_OK;
 }
 
 int lcbsa_copy_slabs(void* const* dst, const void* const* src, size_t nbytes, int count, void* stream) {

@@ -160,170 +160,6 @@ __global__ void __launch_bounds__(256) bwd_emit_kernel(const uint32_t* bitmap, i
 // the A-operand layout of the next (as P is for P V in the forward).  64 x 64 tiles, four warps of 16 rows, the
 // streamed tiles double-buffered with cp.async, two CTAs per SM.
 
-// 16 rows x 64 columns (fp32 accumulators, 8 n-tiles) = A[16 x D] * B[64 x D]^T with A already in registers
-template <typename T, int D>
-__device__ __forceinline__ void mma_abt(float (&acc)[8][4], const uint32_t (&af)[D / 16][4], uint32_t b_tile, int lane) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-#pragma unroll
-        for (int np = 0; np < 4; ++np) {
-            const int mid = lane >> 3;
-            const int row = np * 16 + (lane & 7) + (mid >> 1) * 8;
-            const int c = 2 * ks + (mid & 1);
-            uint32_t bf[4];
-            mm::ldsm_x4(bf, b_tile + row * (D * 2) + ((c ^ (row & 7)) << 4));
-            mm::mma16816<T>(acc[2 * np], af[ks], bf[0], bf[1]);
-            mm::mma16816<T>(acc[2 * np + 1], af[ks], bf[2], bf[3]);
-        }
-    }
-}
-
-// Two such products at once (S and dP of the same tile pair): two independent accumulation chains in one instruction
-// stream, which is what hides the ldmatrix -> mma latency with only two warps per scheduler.
-template <typename T, int D>
-__device__ __forceinline__ void mma_abt2(float (&acc0)[8][4], float (&acc1)[8][4], const uint32_t (&a0)[D / 16][4],
-                                         const uint32_t (&a1)[D / 16][4], uint32_t b0_tile, uint32_t b1_tile, int lane) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        acc0[i][0] = acc0[i][1] = acc0[i][2] = acc0[i][3] = 0.f;
-        acc1[i][0] = acc1[i][1] = acc1[i][2] = acc1[i][3] = 0.f;
-    }
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-#pragma unroll
-        for (int np = 0; np < 4; ++np) {
-            const int mid = lane >> 3;
-            const int row = np * 16 + (lane & 7) + (mid >> 1) * 8;
-            const int c = 2 * ks + (mid & 1);
-            const uint32_t off = row * (D * 2) + ((c ^ (row & 7)) << 4);
-            uint32_t bf0[4], bf1[4];
-            mm::ldsm_x4(bf0, b0_tile + off);
-            mm::ldsm_x4(bf1, b1_tile + off);
-            mm::mma16816<T>(acc0[2 * np], a0[ks], bf0[0], bf0[1]);
-            mm::mma16816<T>(acc1[2 * np], a1[ks], bf1[0], bf1[1]);
-            mm::mma16816<T>(acc0[2 * np + 1], a0[ks], bf0[2], bf0[3]);
-            mm::mma16816<T>(acc1[2 * np + 1], a1[ks], bf1[2], bf1[3]);
-        }
-    }
-}
-
-// The same with the A operands read from shared tiles step by step (this warp's 16 rows of a0_tile and a1_tile)
-template <typename T, int D>
-__device__ __forceinline__ void mma_abt2_sa(float (&acc0)[8][4], float (&acc1)[8][4], uint32_t a0_tile, uint32_t a1_tile, uint32_t b0_tile,
-                                            uint32_t b1_tile, int warp, int lane) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        acc0[i][0] = acc0[i][1] = acc0[i][2] = acc0[i][3] = 0.f;
-        acc1[i][0] = acc1[i][1] = acc1[i][2] = acc1[i][3] = 0.f;
-    }
-    const int arow = warp * 16 + (lane & 15);
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t a0[4], a1[4];
-        {
-            const int c = 2 * ks + (lane >> 4);
-            const uint32_t off = arow * (D * 2) + ((c ^ (arow & 7)) << 4);
-            mm::ldsm_x4(a0, a0_tile + off);
-            mm::ldsm_x4(a1, a1_tile + off);
-        }
-#pragma unroll
-        for (int np = 0; np < 4; ++np) {
-            const int mid = lane >> 3;
-            const int row = np * 16 + (lane & 7) + (mid >> 1) * 8;
-            const int c = 2 * ks + (mid & 1);
-            const uint32_t off = row * (D * 2) + ((c ^ (row & 7)) << 4);
-            uint32_t bf0[4], bf1[4];
-            mm::ldsm_x4(bf0, b0_tile + off);
-            mm::ldsm_x4(bf1, b1_tile + off);
-            mm::mma16816<T>(acc0[2 * np], a0, bf0[0], bf0[1]);
-            mm::mma16816<T>(acc1[2 * np], a1, bf1[0], bf1[1]);
-            mm::mma16816<T>(acc0[2 * np + 1], a0, bf0[2], bf0[3]);
-            mm::mma16816<T>(acc1[2 * np + 1], a1, bf1[2], bf1[3]);
-        }
-    }
-}
-
-// A fragments (16 rows of this warp, all of D) of a swizzled [64][D] tile
-template <int D>
-__device__ __forceinline__ void load_a_frags(uint32_t (&af)[D / 16][4], uint32_t tile, int warp, int lane) {
-    const int row = warp * 16 + (lane & 15);
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-        const int c = 2 * ks + (lane >> 4);
-        mm::ldsm_x4(af[ks], tile + row * (D * 2) + ((c ^ (row & 7)) << 4));
-    }
-}
-
-// out[16 x D] += X[16 x 64] * B[64 x D], X given as fp32 accumulators of the layout mma_abt produces (rounded to T here)
-template <typename T, int D>
-__device__ __forceinline__ void mma_xb(float (&out)[D / 8][4], const float (&x)[8][4], uint32_t b_tile, int lane) {
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-        uint32_t pa[4];
-        pa[0] = mm::pack2(T(), x[2 * kk][0], x[2 * kk][1]);
-        pa[1] = mm::pack2(T(), x[2 * kk][2], x[2 * kk][3]);
-        pa[2] = mm::pack2(T(), x[2 * kk + 1][0], x[2 * kk + 1][1]);
-        pa[3] = mm::pack2(T(), x[2 * kk + 1][2], x[2 * kk + 1][3]);
-#pragma unroll
-        for (int dp = 0; dp < D / 16; ++dp) {
-            const int mid = lane >> 3;
-            const int row = kk * 16 + (lane & 7) + (mid & 1) * 8;
-            const int c = 2 * dp + (mid >> 1);
-            uint32_t bf[4];
-            mm::ldsm_x4_t(bf, b_tile + row * (D * 2) + ((c ^ (row & 7)) << 4));
-            mm::mma16816<T>(out[2 * dp], pa, bf[0], bf[1]);
-            mm::mma16816<T>(out[2 * dp + 1], pa, bf[2], bf[3]);
-        }
-    }
-}
-
-// Two of those at once: out0 += X0 * B0 and out1 += X1 * B1 (dV and dK of one tile pair)
-template <typename T, int D>
-__device__ __forceinline__ void mma_xb2(float (&out0)[D / 8][4], const float (&x0)[8][4], uint32_t b0_tile, float (&out1)[D / 8][4],
-                                        const float (&x1)[8][4], uint32_t b1_tile, int lane) {
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-        uint32_t pa0[4], pa1[4];
-        pa0[0] = mm::pack2(T(), x0[2 * kk][0], x0[2 * kk][1]);
-        pa0[1] = mm::pack2(T(), x0[2 * kk][2], x0[2 * kk][3]);
-        pa0[2] = mm::pack2(T(), x0[2 * kk + 1][0], x0[2 * kk + 1][1]);
-        pa0[3] = mm::pack2(T(), x0[2 * kk + 1][2], x0[2 * kk + 1][3]);
-        pa1[0] = mm::pack2(T(), x1[2 * kk][0], x1[2 * kk][1]);
-        pa1[1] = mm::pack2(T(), x1[2 * kk][2], x1[2 * kk][3]);
-        pa1[2] = mm::pack2(T(), x1[2 * kk + 1][0], x1[2 * kk + 1][1]);
-        pa1[3] = mm::pack2(T(), x1[2 * kk + 1][2], x1[2 * kk + 1][3]);
-#pragma unroll
-        for (int dp = 0; dp < D / 16; ++dp) {
-            const int mid = lane >> 3;
-            const int row = kk * 16 + (lane & 7) + (mid & 1) * 8;
-            const int c = 2 * dp + (mid >> 1);
-            const uint32_t off = row * (D * 2) + ((c ^ (row & 7)) << 4);
-            uint32_t bf0[4], bf1[4];
-            mm::ldsm_x4_t(bf0, b0_tile + off);
-            mm::ldsm_x4_t(bf1, b1_tile + off);
-            mm::mma16816<T>(out0[2 * dp], pa0, bf0[0], bf0[1]);
-            mm::mma16816<T>(out1[2 * dp], pa1, bf1[0], bf1[1]);
-            mm::mma16816<T>(out0[2 * dp + 1], pa0, bf0[2], bf0[3]);
-            mm::mma16816<T>(out1[2 * dp + 1], pa1, bf1[2], bf1[3]);
-        }
-    }
-}
-
-// fp32 accumulators of this warp's 16 rows (all of D) -> a swizzled [64][D] tile in T
-template <typename T, int D>
-__device__ __forceinline__ void stage_rows(unsigned char* tile, const float (&o)[D / 8][4], int warp, int lane) {
-    const int r0 = warp * 16 + (lane >> 2), r1 = r0 + 8;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-        const int col = i * 8 + 2 * (lane & 3);
-        const int c = col >> 3, within = (col & 7) * 2;
-        *reinterpret_cast<uint32_t*>(tile + r0 * (D * 2) + ((c ^ (r0 & 7)) << 4) + within) = mm::pack2(T(), o[i][0], o[i][1]);
-        *reinterpret_cast<uint32_t*>(tile + r1 * (D * 2) + ((c ^ (r1 & 7)) << 4) + within) = mm::pack2(T(), o[i][2], o[i][3]);
-    }
-}
-
 // rows of a swizzled [64][D] tile -> the rows of the block that exist
 template <typename T, int D>
 __device__ __forceinline__ void write_rows(const unsigned char* tile, T* head, long long ss, const Geom& g, const mm::SlotEntry* tab, int blk,
@@ -420,8 +256,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) bwd_dq_mma_kernel(const __grid
     __syncthreads();
 
     uint32_t qf[D / 16][4], dof[D / 16][4];
-    load_a_frags<D>(qf, mm::smem_u32(q_s), warp, lane);
-    load_a_frags<D>(dof, mm::smem_u32(do_s), warp, lane);
+    mm::load_a_frags<D>(qf, mm::smem_u32(q_s), warp, lane);
+    mm::load_a_frags<D>(dof, mm::smem_u32(do_s), warp, lane);
 
     // per-row constants of this thread's two rows
     float lse2[2], dl[2];
@@ -460,7 +296,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) bwd_dq_mma_kernel(const __grid
         const unsigned char* kok = k_ok + buf * kTile;
 
         float s[8][4], dp[8][4];
-        mma_abt2<T, D>(s, dp, qf, dof, kt, vt, lane);
+        mm::mma_abt2<T, D>(s, dp, qf, dof, kt, vt, lane);
         // dS in place of dP: ds = p * (dp - delta) * scale, p = 2^(s * scale2 - lse2); absent keys and rows give 0
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
@@ -472,12 +308,12 @@ __global__ void __launch_bounds__(kBwdThreads, 2) bwd_dq_mma_kernel(const __grid
                 dp[nt][e] = p * (dp[nt][e] - dl[r]) * a.sm_scale;
             }
         }
-        mma_xb<T, D>(dq, dp, kt, lane);  // dQ += dS K
+        mm::mma_xb<T, D>(dq, dp, kt, lane);  // dQ += dS K
         __syncthreads();
     }
     mm::cp_async_wait<0>();
     __syncthreads();
-    stage_rows<T, D>(q_s, dq, warp, lane);
+    mm::stage_rows<T, D>(q_s, dq, warp, lane);
     __syncthreads();
     write_rows<T, D>(q_s, dqh, a.dq.ss, a.gq, qtab, qb, qsub * kTile, tid);
 }
@@ -569,7 +405,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) bwd_dkdv_mma_kernel(const __gr
 
         // S^T = K Q^T and dP^T = V dO^T for this warp's 16 keys: rows are keys, columns are the 64 query rows of the tile
         float st[8][4], dpt[8][4];
-        mma_abt2_sa<T, D>(st, dpt, mm::smem_u32(k_s), mm::smem_u32(v_s), qt, dot, warp, lane);
+        mm::mma_abt2_sa<T, D>(st, dpt, mm::smem_u32(k_s), mm::smem_u32(v_s), qt, dot, warp, lane);
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
 #pragma unroll
@@ -580,13 +416,13 @@ __global__ void __launch_bounds__(kBwdThreads, 2) bwd_dkdv_mma_kernel(const __gr
                 dpt[nt][e] = p * (dpt[nt][e] - dl[col]) * a.sm_scale;                                       // dS^T
             }
         }
-        mma_xb2<T, D>(dv, st, dot, dk, dpt, qt, lane);  // dV += P^T dO,  dK += dS^T Q
+        mm::mma_xb2<T, D>(dv, st, dot, dk, dpt, qt, lane);  // dV += P^T dO,  dK += dS^T Q
         __syncthreads();
     }
     mm::cp_async_wait<0>();
     __syncthreads();
-    stage_rows<T, D>(k_s, dk, warp, lane);
-    stage_rows<T, D>(v_s, dv, warp, lane);
+    mm::stage_rows<T, D>(k_s, dk, warp, lane);
+    mm::stage_rows<T, D>(v_s, dv, warp, lane);
     __syncthreads();
     write_rows<T, D>(k_s, dkh, a.dk.ss, a.gk, ktab, kb, ksub * kTile, tid);
     write_rows<T, D>(v_s, dvh, a.dv.ss, a.gk, ktab, kb, ksub * kTile, tid);

@@ -205,4 +205,22 @@ struct RowJobs {
 };
 cudaError_t launch_norm_rope(int dtype, RowJobs& jobs, int B, int D, cudaStream_t st, const char** why);
 
+// Rotary positions along one axis (rotary.cu): `pairs` pairs of every head turn by position * turns[pair] / 2^64 turns.
+constexpr int kMaxRotaryJobs = 2, kMaxRotaryPairs = 128;
+struct RotaryJob {
+    View x, out;
+    int H, groups;  // groups of heads (filled in by the launch)
+};
+struct RotaryArgs {
+    RotaryJob job[kMaxRotaryJobs];
+    unsigned long long turns[kMaxRotaryPairs];
+    int n, S, pairs, interleaved, inverse, pos64;
+    float factor;
+    const void* pos;  // null: offset + index of the token
+    long long pos_sb, pos_ss, offset;
+    int hpc, slots;   // heads of a thread, vectors of a head that a thread each takes (filled in by the launch)
+    long long items;
+};
+cudaError_t launch_rotary(int dtype, RotaryArgs& args, int B, int D, cudaStream_t st, const char** why);
+
 }  // namespace lcbsa

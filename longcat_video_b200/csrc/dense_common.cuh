@@ -1,0 +1,141 @@
+// Dense attention whose scores may be capped, biased by distance and masked: what its kernels share.
+//
+//   s_ij = scale q_i . k_j      c_ij = cap tanh(s_ij / cap)  (s_ij without a cap)      x_ij = c_ij - slope_h |pos_i - j|
+//   o_i = sum_j exp(x_ij - lse_i) v_j      lse_i = log sum_j exp(x_ij)      over the keys j of one run [lo_i, hi_i)
+//
+// Every mask there is (documents, a causal order, a prefix that all queries of a document see, keys behind a length) lets a
+// query see ONE run of keys, so a mask is three numbers per query, and a tile of scores is whole, mixed or empty by four
+// numbers per 64 queries.  Kernels work in units of log2: scores carry a factor log2(e), exp is ex2.
+#pragma once
+#include "common.cuh"
+
+namespace lcbsa {
+
+constexpr int kDenseUnit = 64;  // rows of a query unit, keys of a key unit
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// What a query sees: keys [lo, hi); pos is its position among the keys.
+struct Seen {
+    int lo, hi, pos;
+};
+
+// The mask as the caller describes it.  cu_q, cu_k (both or neither): first query / key of every document of a batch entry, and the end of
+// the last, docs + 1 numbers `cu_stride` apart per entry; without them the sequence is one document, with k_len[b] keys where that is given.
+struct DenseMask {
+    const int32_t *cu_q, *cu_k, *k_len, *prefix;
+    int docs, causal;
+    long long cu_stride, prefix_stride;  // per batch entry, 0: the same for all
+};
+
+struct DenseArgs {
+    int dtype, B, Hq, Hk, group, D, Sq, Sk;
+    View q, k, v, o, dout, dq, dk, dv;
+    DenseMask mask;
+    float scale, cap;
+    const float* slopes;   // [Hq] or null
+    float* lse;            // [B*Hq, Sq], natural log; nullable in the forward
+    unsigned int* status;
+    // carved out of the workspace (see dense_plan_kernel)
+    int4* rows;            // [B, units * 64]: lo, hi, pos, 0 of every query; rows behind the last query see nothing
+    int4* units;           // [B, units]: min lo, max hi over the rows of a unit that see a key, max lo, min hi over all of them
+    int2* hulls;           // [B, key units]: first and one past the last query that can see a key of the unit
+    float* delta;          // [B*Hq, Sq]
+};
+
+__host__ __device__ __forceinline__ int dense_units(int n) { return (n + kDenseUnit - 1) / kDenseUnit; }
+
+// Number of entries of cu[0 .. docs] that are <= x (the entries ascend).
+__device__ __forceinline__ int dense_count_le(const int32_t* cu, int docs, int x) {
+    int lo = 0, hi = docs + 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(cu + mid) <= x) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Whatever the bounds hold, the run lies inside [0, Sk).
+__device__ __forceinline__ Seen dense_seen(const DenseMask& m, int b, int i, int Sq, int Sk) {
+    int k0 = 0, k1 = Sk, q1 = Sq, d = 0;
+    if (m.cu_q != nullptr) {
+        const int32_t *cq = m.cu_q + b * m.cu_stride, *ck = m.cu_k + b * m.cu_stride;
+        d = dense_count_le(cq, m.docs, i) - 1;
+        if (d < 0 || d >= m.docs) return Seen{0, 0, 0};  // before the first document or behind the last
+        k0 = min(max(__ldg(ck + d), 0), Sk);
+        k1 = min(max(__ldg(ck + d + 1), k0), Sk);
+        q1 = __ldg(cq + d + 1);
+    } else if (m.k_len != nullptr) {
+        k1 = min(max(__ldg(m.k_len + b), 0), Sk);
+    }
+    const int pos = k1 - (q1 - i);  // the last query of a document stands at its last key
+    int hi = k1;
+    if (m.causal) {
+        const int pre = m.prefix != nullptr ? min(max(__ldg(m.prefix + b * m.prefix_stride + d), 0), Sk) : 0;
+        hi = min(max(max(pos + 1, k0 + pre), k0), k1);
+    }
+    return Seen{k0, hi, pos};
+}
+
+// Score of one pair in units of log2, as the exponent of its probability.  mul: scale * log2(e), with a cap 2 * scale / cap * log2(e).
+//   cap tanh(y) = cap - 2 cap / (1 + exp(2 y)): two special functions, exact at both ends (exp = inf: cap; exp = 0: -cap), off by a few
+//   2^-24 of the cap in between; the machine's own tanh is off by 2^-11, which a cap of 50 would make 2 % of a probability.
+struct ScoreShape {
+    float mul, cap2, slope2;  // cap2: cap * log2(e), slope2: slope of the head * log2(e)
+};
+inline ScoreShape score_shape(float scale, float cap) {
+    ScoreShape s;
+    s.mul = cap > 0.f ? (float)(2.0 * (double)scale / (double)cap * 1.4426950408889634) : scale * kLog2e;
+    s.cap2 = cap * kLog2e;
+    s.slope2 = 0.f;
+    return s;
+}
+__device__ __forceinline__ float dense_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float dense_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// far: |pos - key| (kBias).  tanh2: 2 / (1 + exp(2 y)), from which the backward has 1 - tanh^2 = tanh2 (2 - tanh2).
+template <bool kCap, bool kBias>
+__device__ __forceinline__ float shaped_score(const ScoreShape& f, float s, float far, float& tanh2) {
+    float x;
+    if (kCap) {
+        tanh2 = 2.f * dense_rcp(1.f + dense_ex2(s * f.mul));
+        x = fmaf(-f.cap2, tanh2, f.cap2);
+    } else {
+        x = s * f.mul;
+    }
+    if (kBias) x = fmaf(-f.slope2, far, x);
+    return x;
+}
+
+// Whether one of the eight 16-bit values of a 16-byte chunk is an infinity or a NaN (all exponent bits set).
+template <typename T>
+__device__ __forceinline__ bool chunk_nonfinite(const uint4& v) {
+    constexpr uint32_t kExp = DType<T>::code == LCBSA_BF16 ? 0x7f807f80u : 0x7c007c00u;
+    constexpr uint32_t kLow = DType<T>::code == LCBSA_BF16 ? 0x00800080u : 0x04000400u;
+    // adding one to the exponent field of (v & kExp) carries out of it exactly when all its bits are set
+    auto hot = [](uint32_t u) { return (((u & kExp) >> 1) + (kLow >> 1)) & 0x40004000u; };
+    return (hot(v.x) | hot(v.y) | hot(v.z) | hot(v.w)) != 0;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t zero_nonfinite(uint32_t u) {
+    constexpr uint32_t kExp = DType<T>::code == LCBSA_BF16 ? 0x7f80u : 0x7c00u;
+    if ((u & kExp) == kExp) u &= 0xffff0000u;
+    if (((u >> 16) & kExp) == kExp) u &= 0x0000ffffu;
+    return u;
+}
+
+// dense_few.cu: any number of queries, made for few of them; dense_bwd.cu: the plan and the backward
+bool dense_supported(const DenseArgs& a, const char** why);
+size_t dense_fwd_workspace_bytes(const DenseArgs& a);
+cudaError_t launch_dense_fwd(const DenseArgs& a, void* workspace, cudaStream_t st, const char** why);
+size_t dense_bwd_workspace_bytes(const DenseArgs& a);
+cudaError_t launch_dense_bwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why);
+
+}  // namespace lcbsa

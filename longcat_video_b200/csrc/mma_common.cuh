@@ -85,5 +85,152 @@ __device__ __forceinline__ void load_tile(unsigned char* tile, const T* head_bas
     }
 }
 
+// ------------------------------------------------------------------------------------------ products of 64-row tiles (the backward passes)
+
+// 16 rows x 64 columns (fp32 accumulators, 8 n-tiles) = A[16 x D] * B[64 x D]^T with A already in registers, twice at once (S and dP of
+// the same tile pair): two independent accumulation chains in one instruction
+// stream, which is what hides the ldmatrix -> mma latency with only two warps per scheduler.
+template <typename T, int D>
+__device__ __forceinline__ void mma_abt2(float (&acc0)[8][4], float (&acc1)[8][4], const uint32_t (&a0)[D / 16][4],
+                                         const uint32_t (&a1)[D / 16][4], uint32_t b0_tile, uint32_t b1_tile, int lane) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        acc0[i][0] = acc0[i][1] = acc0[i][2] = acc0[i][3] = 0.f;
+        acc1[i][0] = acc1[i][1] = acc1[i][2] = acc1[i][3] = 0.f;
+    }
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+#pragma unroll
+        for (int np = 0; np < 4; ++np) {
+            const int mid = lane >> 3;
+            const int row = np * 16 + (lane & 7) + (mid >> 1) * 8;
+            const int c = 2 * ks + (mid & 1);
+            const uint32_t off = row * (D * 2) + ((c ^ (row & 7)) << 4);
+            uint32_t bf0[4], bf1[4];
+            ldsm_x4(bf0, b0_tile + off);
+            ldsm_x4(bf1, b1_tile + off);
+            mma16816<T>(acc0[2 * np], a0[ks], bf0[0], bf0[1]);
+            mma16816<T>(acc1[2 * np], a1[ks], bf1[0], bf1[1]);
+            mma16816<T>(acc0[2 * np + 1], a0[ks], bf0[2], bf0[3]);
+            mma16816<T>(acc1[2 * np + 1], a1[ks], bf1[2], bf1[3]);
+        }
+    }
+}
+
+// The same with the A operands read from shared tiles step by step (this warp's 16 rows of a0_tile and a1_tile)
+template <typename T, int D>
+__device__ __forceinline__ void mma_abt2_sa(float (&acc0)[8][4], float (&acc1)[8][4], uint32_t a0_tile, uint32_t a1_tile, uint32_t b0_tile,
+                                            uint32_t b1_tile, int warp, int lane) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        acc0[i][0] = acc0[i][1] = acc0[i][2] = acc0[i][3] = 0.f;
+        acc1[i][0] = acc1[i][1] = acc1[i][2] = acc1[i][3] = 0.f;
+    }
+    const int arow = warp * 16 + (lane & 15);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t a0[4], a1[4];
+        {
+            const int c = 2 * ks + (lane >> 4);
+            const uint32_t off = arow * (D * 2) + ((c ^ (arow & 7)) << 4);
+            ldsm_x4(a0, a0_tile + off);
+            ldsm_x4(a1, a1_tile + off);
+        }
+#pragma unroll
+        for (int np = 0; np < 4; ++np) {
+            const int mid = lane >> 3;
+            const int row = np * 16 + (lane & 7) + (mid >> 1) * 8;
+            const int c = 2 * ks + (mid & 1);
+            const uint32_t off = row * (D * 2) + ((c ^ (row & 7)) << 4);
+            uint32_t bf0[4], bf1[4];
+            ldsm_x4(bf0, b0_tile + off);
+            ldsm_x4(bf1, b1_tile + off);
+            mma16816<T>(acc0[2 * np], a0, bf0[0], bf0[1]);
+            mma16816<T>(acc1[2 * np], a1, bf1[0], bf1[1]);
+            mma16816<T>(acc0[2 * np + 1], a0, bf0[2], bf0[3]);
+            mma16816<T>(acc1[2 * np + 1], a1, bf1[2], bf1[3]);
+        }
+    }
+}
+
+// A fragments (16 rows of this warp, all of D) of a swizzled [64][D] tile
+template <int D>
+__device__ __forceinline__ void load_a_frags(uint32_t (&af)[D / 16][4], uint32_t tile, int warp, int lane) {
+    const int row = warp * 16 + (lane & 15);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        const int c = 2 * ks + (lane >> 4);
+        ldsm_x4(af[ks], tile + row * (D * 2) + ((c ^ (row & 7)) << 4));
+    }
+}
+
+// out[16 x D] += X[16 x 64] * B[64 x D], X given as fp32 accumulators of the layout mma_abt2 produces (rounded to T here)
+template <typename T, int D>
+__device__ __forceinline__ void mma_xb(float (&out)[D / 8][4], const float (&x)[8][4], uint32_t b_tile, int lane) {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+        uint32_t pa[4];
+        pa[0] = pack2(T(), x[2 * kk][0], x[2 * kk][1]);
+        pa[1] = pack2(T(), x[2 * kk][2], x[2 * kk][3]);
+        pa[2] = pack2(T(), x[2 * kk + 1][0], x[2 * kk + 1][1]);
+        pa[3] = pack2(T(), x[2 * kk + 1][2], x[2 * kk + 1][3]);
+#pragma unroll
+        for (int dp = 0; dp < D / 16; ++dp) {
+            const int mid = lane >> 3;
+            const int row = kk * 16 + (lane & 7) + (mid & 1) * 8;
+            const int c = 2 * dp + (mid >> 1);
+            uint32_t bf[4];
+            ldsm_x4_t(bf, b_tile + row * (D * 2) + ((c ^ (row & 7)) << 4));
+            mma16816<T>(out[2 * dp], pa, bf[0], bf[1]);
+            mma16816<T>(out[2 * dp + 1], pa, bf[2], bf[3]);
+        }
+    }
+}
+
+// Two of those at once: out0 += X0 * B0 and out1 += X1 * B1 (dV and dK of one tile pair)
+template <typename T, int D>
+__device__ __forceinline__ void mma_xb2(float (&out0)[D / 8][4], const float (&x0)[8][4], uint32_t b0_tile, float (&out1)[D / 8][4],
+                                        const float (&x1)[8][4], uint32_t b1_tile, int lane) {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+        uint32_t pa0[4], pa1[4];
+        pa0[0] = pack2(T(), x0[2 * kk][0], x0[2 * kk][1]);
+        pa0[1] = pack2(T(), x0[2 * kk][2], x0[2 * kk][3]);
+        pa0[2] = pack2(T(), x0[2 * kk + 1][0], x0[2 * kk + 1][1]);
+        pa0[3] = pack2(T(), x0[2 * kk + 1][2], x0[2 * kk + 1][3]);
+        pa1[0] = pack2(T(), x1[2 * kk][0], x1[2 * kk][1]);
+        pa1[1] = pack2(T(), x1[2 * kk][2], x1[2 * kk][3]);
+        pa1[2] = pack2(T(), x1[2 * kk + 1][0], x1[2 * kk + 1][1]);
+        pa1[3] = pack2(T(), x1[2 * kk + 1][2], x1[2 * kk + 1][3]);
+#pragma unroll
+        for (int dp = 0; dp < D / 16; ++dp) {
+            const int mid = lane >> 3;
+            const int row = kk * 16 + (lane & 7) + (mid & 1) * 8;
+            const int c = 2 * dp + (mid >> 1);
+            const uint32_t off = row * (D * 2) + ((c ^ (row & 7)) << 4);
+            uint32_t bf0[4], bf1[4];
+            ldsm_x4_t(bf0, b0_tile + off);
+            ldsm_x4_t(bf1, b1_tile + off);
+            mma16816<T>(out0[2 * dp], pa0, bf0[0], bf0[1]);
+            mma16816<T>(out1[2 * dp], pa1, bf1[0], bf1[1]);
+            mma16816<T>(out0[2 * dp + 1], pa0, bf0[2], bf0[3]);
+            mma16816<T>(out1[2 * dp + 1], pa1, bf1[2], bf1[3]);
+        }
+    }
+}
+
+// fp32 accumulators of this warp's 16 rows (all of D) -> a swizzled [64][D] tile in T
+template <typename T, int D>
+__device__ __forceinline__ void stage_rows(unsigned char* tile, const float (&o)[D / 8][4], int warp, int lane) {
+    const int r0 = warp * 16 + (lane >> 2), r1 = r0 + 8;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+        const int col = i * 8 + 2 * (lane & 3);
+        const int c = col >> 3, within = (col & 7) * 2;
+        *reinterpret_cast<uint32_t*>(tile + r0 * (D * 2) + ((c ^ (r0 & 7)) << 4) + within) = pack2(T(), o[i][0], o[i][1]);
+        *reinterpret_cast<uint32_t*>(tile + r1 * (D * 2) + ((c ^ (r1 & 7)) << 4) + within) = pack2(T(), o[i][2], o[i][3]);
+    }
+}
+
 }  // namespace mm
 }  // namespace lcbsa
