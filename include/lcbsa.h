@@ -320,6 +320,8 @@ int lcbsa_norm_rope_jobs(const LcbsaRowJob* jobs, int n_jobs, float eps, void* s
  * Keys and values that no query of a call sees, and those hidden from a query, may hold anything, infinities and NaN included.
  *
  * lse: fp32 dense [B, Hq, Sq], natural log, nullable in the forward.  A row with a NaN or +inf score is NaN, its lse too.
+ * rest: nullable, dense [B, Hq, Sq, D] in the type of q: what rounding out to its type left.  A backward that is given it takes
+ * rowsum(dout * out) from both, which halves what that sum adds to the error of dq and dk.
  * The workspace (lcbsa_dense_attn_workspace_bytes, 256-byte aligned) belongs to one call until its kernels have run.
  * The backward takes the forward's out and lse and writes every row of dq, dk and dv; no atomics, so two calls give the same
  * bits; the slopes are constants.
@@ -333,9 +335,9 @@ typedef struct LcbsaScores {
 } LcbsaScores;
 size_t lcbsa_dense_attn_workspace_bytes(const LcbsaTensor* q, const LcbsaTensor* k, int backward);
 int lcbsa_dense_attn_fwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaScores* scores, const LcbsaTensor* out,
-                         float* lse, void* workspace, size_t workspace_bytes, void* stream);
+                         float* lse, void* rest, void* workspace, size_t workspace_bytes, void* stream);
 int lcbsa_dense_attn_bwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaTensor* out, const LcbsaTensor* dout,
-                         const LcbsaScores* scores, const float* lse, const LcbsaTensor* dq, const LcbsaTensor* dk, const LcbsaTensor* dv,
+                         const LcbsaScores* scores, const float* lse, const void* rest, const LcbsaTensor* dq, const LcbsaTensor* dk, const LcbsaTensor* dv,
                          void* workspace, size_t workspace_bytes, void* stream);
 
 /*

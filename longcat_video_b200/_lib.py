@@ -102,10 +102,10 @@ SIGNATURES = {
     "lcbsa_norm_rope": (ctypes.c_int, [_P(LcbsaTensor), ctypes.c_void_p, _P(LcbsaGrid), ctypes.c_void_p, ctypes.c_float,
                                        _P(LcbsaTensor), ctypes.c_void_p]),
     "lcbsa_dense_attn_workspace_bytes": (ctypes.c_size_t, [_P(LcbsaTensor), _P(LcbsaTensor), ctypes.c_int]),
-    "lcbsa_dense_attn_fwd": (ctypes.c_int, [_P(LcbsaTensor)] * 3 + [_P(LcbsaScores), _P(LcbsaTensor), ctypes.c_void_p, ctypes.c_void_p,
-                                            ctypes.c_size_t, ctypes.c_void_p]),
-    "lcbsa_dense_attn_bwd": (ctypes.c_int, [_P(LcbsaTensor)] * 5 + [_P(LcbsaScores), ctypes.c_void_p] + [_P(LcbsaTensor)] * 3
-                             + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "lcbsa_dense_attn_fwd": (ctypes.c_int, [_P(LcbsaTensor)] * 3 + [_P(LcbsaScores), _P(LcbsaTensor)] + [ctypes.c_void_p] * 3
+                             + [ctypes.c_size_t, ctypes.c_void_p]),
+    "lcbsa_dense_attn_bwd": (ctypes.c_int, [_P(LcbsaTensor)] * 5 + [_P(LcbsaScores), ctypes.c_void_p, ctypes.c_void_p]
+                             + [_P(LcbsaTensor)] * 3 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "lcbsa_rotary": (ctypes.c_int, [_P(LcbsaTensor), _P(LcbsaTensor), ctypes.c_int, _P(ctypes.c_uint64), ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                     ctypes.c_float, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]),
     "lcbsa_copy_slabs": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p]),

@@ -618,13 +618,15 @@ size_t lcbsa_dense_attn_workspace_bytes(const LcbsaTensor* q, const LcbsaTensor*
 }
 
 int lcbsa_dense_attn_fwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaScores* scores, const LcbsaTensor* out,
-                         float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+                         float* lse, void* rest, void* workspace, size_t workspace_bytes, void* stream) {
     lcbsa::DenseArgs a{};
     if (int rc = dense_args("dense_attn", q, k, v, scores, &a)) return rc;
     if (int rc = same_shape("dense_attn", "out", out, q)) return rc;
     if (int rc = dense_workspace("dense_attn", workspace, workspace_bytes, lcbsa::dense_fwd_workspace_bytes(a))) return rc;
+    if (reinterpret_cast<uintptr_t>(rest) % 16 != 0) return fail(LCBSA_EINVAL, "dense_attn: rest not 16-byte aligned");
     a.o = view_of(out);
     a.lse = lse;
+    a.rest = rest;
     a.status = device_status_ptr();
     if (!a.status) return fail(LCBSA_ECUDA, "dense_attn: cannot resolve the device status words");
     const char* why = "";
@@ -634,7 +636,7 @@ int lcbsa_dense_attn_fwd(const LcbsaTensor* q, const LcbsaTensor* k, const Lcbsa
 }
 
 int lcbsa_dense_attn_bwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaTensor* out, const LcbsaTensor* dout,
-                         const LcbsaScores* scores, const float* lse, const LcbsaTensor* dq, const LcbsaTensor* dk, const LcbsaTensor* dv,
+                         const LcbsaScores* scores, const float* lse, const void* rest, const LcbsaTensor* dq, const LcbsaTensor* dk, const LcbsaTensor* dv,
                          void* workspace, size_t workspace_bytes, void* stream) {
     lcbsa::DenseArgs a{};
     if (int rc = dense_args("dense_attn_bwd", q, k, v, scores, &a)) return rc;
@@ -643,10 +645,12 @@ int lcbsa_dense_attn_bwd(const LcbsaTensor* q, const LcbsaTensor* k, const Lcbsa
     if (int rc = same_shape("dense_attn_bwd", "dq", dq, q)) return rc;
     if (int rc = same_shape("dense_attn_bwd", "dk", dk, k)) return rc;
     if (int rc = same_shape("dense_attn_bwd", "dv", dv, k)) return rc;
+    if (reinterpret_cast<uintptr_t>(rest) % 16 != 0) return fail(LCBSA_EINVAL, "dense_attn_bwd: rest not 16-byte aligned");
     if (!lse && a.B * a.Hq * a.Sq > 0) return fail(LCBSA_EINVAL, "dense_attn_bwd: null lse");
     if (int rc = dense_workspace("dense_attn_bwd", workspace, workspace_bytes, lcbsa::dense_bwd_workspace_bytes(a))) return rc;
     a.o = view_of(out); a.dout = view_of(dout); a.dq = view_of(dq); a.dk = view_of(dk); a.dv = view_of(dv);
     a.lse = const_cast<float*>(lse);
+    a.rest = const_cast<void*>(rest);
     a.status = device_status_ptr();
     if (!a.status) return fail(LCBSA_ECUDA, "dense_attn_bwd: cannot resolve the device status words");
     const char* why = "";

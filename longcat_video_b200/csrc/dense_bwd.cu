@@ -22,71 +22,8 @@ namespace {
 constexpr int kTile = kDenseUnit;
 constexpr int kBwdThreads = 128;
 
-// ------------------------------------------------------------------------------------------ the plan
-//
-// What every query sees, in the order of the queries; per unit of 64 queries the union of the runs of its rows (min lo, max hi) and the
-// run that all see (max lo, min hi); per unit of 64 keys the first and the last query that can see one of them, from the
-// documents at its two ends.  A warp takes a query unit, a thread of the CTAs behind them a key unit.
-__global__ void __launch_bounds__(128) dense_plan_kernel(const __grid_constant__ DenseArgs a, int q_ctas) {
-    const int b = blockIdx.y, lane = threadIdx.x & 31, n_u = dense_units(a.Sq), n_k = dense_units(a.Sk);
-    if ((int)blockIdx.x < q_ctas) {
-        const int u = blockIdx.x * 4 + (threadIdx.x >> 5);
-        if (u >= n_u) return;
-        int u_lo = 0x7fffffff, u_hi = 0, all_lo = 0, all_hi = 0x7fffffff;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int i = u * kTile + e * 32 + lane;
-            Seen s{0, 0, 0};
-            if (i < a.Sq) s = dense_seen(a.mask, b, i, a.Sq, a.Sk);
-            a.rows[(long long)b * n_u * kTile + i] = make_int4(s.lo, s.hi, s.pos, 0);
-            if (s.lo < s.hi) {
-                u_lo = min(u_lo, s.lo);
-                u_hi = max(u_hi, s.hi);
-                all_lo = max(all_lo, s.lo);
-                all_hi = min(all_hi, s.hi);
-            } else {
-                all_hi = 0;
-            }
-        }
-        u_lo = __reduce_min_sync(0xffffffffu, u_lo);
-        u_hi = __reduce_max_sync(0xffffffffu, u_hi);
-        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
-        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
-        if (lane == 0) a.units[(long long)b * n_u + u] = make_int4(min(u_lo, u_hi), u_hi, all_lo, all_hi);
-        return;
-    }
-    const int u = (blockIdx.x - q_ctas) * 128 + threadIdx.x;
-    if (u >= n_k) return;
-    const DenseMask& m = a.mask;
-    const int k_first = u * kTile, k_last = min(k_first + kTile, a.Sk) - 1;
-    int d = 0, k0 = 0, k1 = a.Sk, q0 = 0, q1 = a.Sq, q_end = a.Sq;
-    if (m.cu_q != nullptr) {
-        const int32_t *cq = m.cu_q + b * m.cu_stride, *ck = m.cu_k + b * m.cu_stride;
-        d = max(dense_count_le(ck, m.docs, k_first) - 1, 0);
-        const int d1 = min(dense_count_le(ck, m.docs, k_last) - 1, m.docs - 1);
-        if (d > d1) {
-            a.hulls[(long long)b * n_k + u] = make_int2(0, 0);
-            return;
-        }
-        k0 = min(max(__ldg(ck + d), 0), a.Sk);
-        k1 = min(max(__ldg(ck + d + 1), k0), a.Sk);
-        q0 = __ldg(cq + d);
-        q1 = __ldg(cq + d + 1);
-        q_end = __ldg(cq + d1 + 1);
-    } else if (m.k_len != nullptr) {
-        k1 = min(max(__ldg(m.k_len + b), 0), a.Sk);
-        if (k_first >= k1) q_end = 0;
-    }
-    if (m.causal) {
-        const int pre = m.prefix != nullptr ? min(max(__ldg(m.prefix + b * m.prefix_stride + d), 0), a.Sk) : 0;
-        const int key = max(k_first, k0);
-        if (key >= k0 + pre) q0 = max(q0, q1 - (k1 - key));
-    }
-    q0 = min(max(q0, 0), a.Sq);
-    a.hulls[(long long)b * n_k + u] = make_int2(q0, min(max(q_end, q0), a.Sq));
-}
-
-// One warp per query row: rowsum(dout * out) in fp32.
+// One warp per query row: rowsum(dout * out) in fp32, out with what its rounding left (a half step of out moves dS by as much as
+// rounding dS does: dq of a causal row of 600 keys, bf16, is off by 1.53 times its own rounding without it, 1.46 with it).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) dense_delta_kernel(const __grid_constant__ DenseArgs a) {
     constexpr int kPer = D / 32;
@@ -96,9 +33,14 @@ __global__ void __launch_bounds__(256) dense_delta_kernel(const __grid_constant_
     const int i = (int)(r % a.Sq), bh = (int)(r / a.Sq), b = bh / a.Hq, h = bh % a.Hq;
     const T* o = static_cast<const T*>(a.o.data) + b * a.o.sb + h * a.o.sh + i * a.o.ss + lane * kPer;
     const T* g = static_cast<const T*>(a.dout.data) + b * a.dout.sb + h * a.dout.sh + i * a.dout.ss + lane * kPer;
+    const T* left = a.rest != nullptr ? static_cast<const T*>(a.rest) + r * D + lane * kPer : nullptr;
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) s = fmaf(DType<T>::to_f32(o[e]), DType<T>::to_f32(g[e]), s);
+    for (int e = 0; e < kPer; ++e) {
+        float v = DType<T>::to_f32(o[e]);
+        if (left != nullptr) v += DType<T>::to_f32(left[e]);
+        s = fmaf(v, DType<T>::to_f32(g[e]), s);
+    }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
     if (lane == 0) a.delta[r] = s;
@@ -370,38 +312,25 @@ cudaError_t passes(const DenseArgs& a, cudaStream_t st) {
 template <typename T, int D>
 cudaError_t backward(const DenseArgs& a, cudaStream_t st) {
     const long long rows = (long long)a.B * a.Hq * a.Sq;
-    if ((rows + 7) / 8 > 0x7fffffffll || a.B > 65535) return cudaErrorInvalidConfiguration;
-    const int q_ctas = (dense_units(a.Sq) + 3) / 4, k_ctas = (dense_units(a.Sk) + 127) / 128;
-    if (q_ctas + k_ctas > 0) dense_plan_kernel<<<dim3(q_ctas + k_ctas, a.B), 128, 0, st>>>(a, q_ctas);
+    if ((rows + 7) / 8 > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    cudaError_t e = launch_dense_plan(a, st);
+    if (e != cudaSuccess) return e;
     if (rows > 0) dense_delta_kernel<T, D><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(a);
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
     if (cap) return bias ? passes<T, D, true, true>(a, st) : passes<T, D, true, false>(a, st);
     return bias ? passes<T, D, false, true>(a, st) : passes<T, D, false, false>(a, st);
 }
 
-size_t align256(size_t n) { return (n + 255) / 256 * 256; }
-
 }  // namespace
 
-size_t dense_bwd_workspace_bytes(const DenseArgs& a) {
-    const size_t n_u = dense_units(a.Sq), n_k = dense_units(a.Sk);
-    return align256(a.B * n_u * kTile * sizeof(int4)) + align256(a.B * n_u * sizeof(int4)) + align256(a.B * n_k * sizeof(int2)) +
-           align256((size_t)a.B * a.Hq * a.Sq * sizeof(float));
-}
+size_t dense_bwd_workspace_bytes(const DenseArgs& a) { return dense_plan_bytes(a, true) + (size_t)a.B * a.Hq * a.Sq * sizeof(float); }
 
 cudaError_t launch_dense_bwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why) {
     if (a.B * a.Hq == 0) return cudaSuccess;
-    const size_t n_u = dense_units(a.Sq), n_k = dense_units(a.Sk);
-    unsigned char* w = static_cast<unsigned char*>(workspace);
-    a.rows = reinterpret_cast<int4*>(w);
-    w += align256(a.B * n_u * kTile * sizeof(int4));
-    a.units = reinterpret_cast<int4*>(w);
-    w += align256(a.B * n_u * sizeof(int4));
-    a.hulls = reinterpret_cast<int2*>(w);
-    w += align256(a.B * n_k * sizeof(int2));
-    a.delta = reinterpret_cast<float*>(w);
+    dense_plan_carve(a, workspace, true);
+    a.delta = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + dense_plan_bytes(a, true));
     const cudaError_t e = a.dtype == LCBSA_BF16 ? (a.D == 128 ? backward<__nv_bfloat16, 128>(a, st) : backward<__nv_bfloat16, 64>(a, st))
                                                 : (a.D == 128 ? backward<__half, 128>(a, st) : backward<__half, 64>(a, st));
     if (e == cudaErrorInvalidConfiguration) *why = "more CTAs than a launch takes";

@@ -11,6 +11,7 @@
 
 namespace lcbsa {
 
+constexpr int kDenseCounters = 2;
 constexpr int kDenseUnit = 64;  // rows of a query unit, keys of a key unit
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -34,12 +35,14 @@ struct DenseArgs {
     float scale, cap;
     const float* slopes;   // [Hq] or null
     float* lse;            // [B*Hq, Sq], natural log; nullable in the forward
+    void* rest;            // nullable, dense [B, Hq, Sq, D] in the input type: what rounding the output left, for delta
     unsigned int* status;
     // carved out of the workspace (see dense_plan_kernel)
     int4* rows;            // [B, units * 64]: lo, hi, pos, 0 of every query; rows behind the last query see nothing
     int4* units;           // [B, units]: min lo, max hi over the rows of a unit that see a key, max lo, min hi over all of them
-    int2* hulls;           // [B, key units]: first and one past the last query that can see a key of the unit
-    float* delta;          // [B*Hq, Sq]
+    int2* hulls;           // [B, key units]: first and one past the last query that can see a key of the unit (backward)
+    float* delta;          // [B*Hq, Sq] (backward)
+    int* next_item;        // items taken by the persistent kernels, zero when they start
 };
 
 __host__ __device__ __forceinline__ int dense_units(int n) { return (n + kDenseUnit - 1) / kDenseUnit; }
@@ -131,10 +134,17 @@ __device__ __forceinline__ uint32_t zero_nonfinite(uint32_t u) {
     return u;
 }
 
+// the plan of a call (dense_plan.cu)
+size_t dense_plan_bytes(const DenseArgs& a, bool backward);
+void dense_plan_carve(DenseArgs& a, void* workspace, bool backward);
+cudaError_t launch_dense_plan(const DenseArgs& a, cudaStream_t st);
+// dense_tc.cu: the forward on tcgen05
+bool dense_tc_supported(const DenseArgs& a);
+cudaError_t launch_dense_tc(const DenseArgs& a, cudaStream_t st, const char** why);
 // dense_few.cu: any number of queries, made for few of them; dense_bwd.cu: the plan and the backward
 bool dense_supported(const DenseArgs& a, const char** why);
 size_t dense_fwd_workspace_bytes(const DenseArgs& a);
-cudaError_t launch_dense_fwd(const DenseArgs& a, void* workspace, cudaStream_t st, const char** why);
+cudaError_t launch_dense_fwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why);
 size_t dense_bwd_workspace_bytes(const DenseArgs& a);
 cudaError_t launch_dense_bwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why);
 

@@ -323,7 +323,12 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
             const float inv = l == 0.f ? 0.f : 1.f / l;
             T* dst = static_cast<T*>(const_cast<void*>(a.o.data)) + (long long)b * a.o.sb + (long long)h * a.o.sh + (long long)i * a.o.ss + lane * kPer;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) dst[e] = DType<T>::from_f32(x[e] * inv);
+            for (int e = 0; e < kPer; ++e) {
+                const float v = x[e] * inv;
+                dst[e] = DType<T>::from_f32(v);
+                if (a.rest != nullptr)
+                    static_cast<T*>(a.rest)[(((long long)b * a.Hq + h) * a.Sq + i) * D + lane * kPer + e] = DType<T>::from_f32(v - DType<T>::to_f32(dst[e]));
+            }
             if (a.lse != nullptr && lane == 0) a.lse[((long long)b * a.Hq + h) * a.Sq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         }
     }
@@ -360,7 +365,12 @@ __global__ void __launch_bounds__(128) dense_combine_kernel(const __grid_constan
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* dst = static_cast<T*>(const_cast<void*>(a.o.data)) + (long long)b * a.o.sb + (long long)h * a.o.sh + (long long)i * a.o.ss + lane * kPer;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) dst[e] = DType<T>::from_f32(acc[e] * inv);
+    for (int e = 0; e < kPer; ++e) {
+        const float v = acc[e] * inv;
+        dst[e] = DType<T>::from_f32(v);
+        if (a.rest != nullptr)
+            static_cast<T*>(a.rest)[(((long long)b * a.Hq + h) * a.Sq + i) * D + lane * kPer + e] = DType<T>::from_f32(v - DType<T>::to_f32(dst[e]));
+    }
     if (a.lse != nullptr && lane == 0) a.lse[((long long)b * a.Hq + h) * a.Sq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -417,15 +427,25 @@ bool dense_supported(const DenseArgs& a, const char** why) {
     return true;
 }
 
+// Which kernel: the tcgen05 kernel computes 128 rows of one head at a time, this one 16 rows of a group of heads.  (To be measured.)
+static bool few_queries(const DenseArgs& a) { return (long long)a.group * a.Sq <= 64; }
+
 size_t dense_fwd_workspace_bytes(const DenseArgs& a) {
     FewParams P;
     few_plan(a, P);
-    if (P.splits == 1) return 0;
-    return (size_t)a.B * a.Hk * P.rows * P.splits * (a.D + 2) * 4;
+    const size_t plan = few_queries(a) ? 0 : dense_plan_bytes(a, false);
+    if (P.splits == 1) return plan;
+    const size_t few = (size_t)a.B * a.Hk * P.rows * P.splits * (a.D + 2) * 4;
+    return few > plan ? few : plan;
 }
 
-cudaError_t launch_dense_fwd(const DenseArgs& a, void* workspace, cudaStream_t st, const char** why) {
+cudaError_t launch_dense_fwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why) {
     if (a.B * a.Hq == 0 || a.Sq == 0) return cudaSuccess;
+    if (!few_queries(a) && dense_tc_supported(a)) {
+        dense_plan_carve(a, workspace, false);
+        const cudaError_t e = launch_dense_plan(a, st);
+        return e == cudaSuccess ? launch_dense_tc(a, st, why) : e;
+    }
     FewParams P;
     P.a = a;
     P.shape = score_shape(a.scale, a.cap);

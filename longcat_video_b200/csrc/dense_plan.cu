@@ -1,0 +1,100 @@
+// The plan of a dense attention call: what its masks come to (see dense_common.cuh).
+//
+// What every query sees, in the order of the queries; per unit of 64 queries the union of the runs of its rows (min lo, max hi) and the
+// run that all see (max lo, min hi); per unit of 64 keys the first and the last query that can see one of them, from the
+// documents at its two ends.  A warp takes a query unit, a thread of the CTAs behind them a key unit.
+#include "dense_common.cuh"
+
+namespace lcbsa {
+
+namespace {
+
+__global__ void __launch_bounds__(128) dense_plan_kernel(const __grid_constant__ DenseArgs a, int q_ctas) {
+    if (a.next_item != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kDenseCounters) a.next_item[threadIdx.x] = 0;
+    const int b = blockIdx.y, lane = threadIdx.x & 31, n_u = dense_units(a.Sq), n_k = dense_units(a.Sk);
+    if ((int)blockIdx.x < q_ctas) {
+        const int u = blockIdx.x * 4 + (threadIdx.x >> 5);
+        if (u >= n_u) return;
+        int u_lo = 0x7fffffff, u_hi = 0, all_lo = 0, all_hi = 0x7fffffff;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = u * kDenseUnit + e * 32 + lane;
+            Seen s{0, 0, 0};
+            if (i < a.Sq) s = dense_seen(a.mask, b, i, a.Sq, a.Sk);
+            a.rows[(long long)b * n_u * kDenseUnit + i] = make_int4(s.lo, s.hi, s.pos, 0);
+            if (s.lo < s.hi) {
+                u_lo = min(u_lo, s.lo);
+                u_hi = max(u_hi, s.hi);
+                all_lo = max(all_lo, s.lo);
+                all_hi = min(all_hi, s.hi);
+            } else {
+                all_hi = 0;
+            }
+        }
+        u_lo = __reduce_min_sync(0xffffffffu, u_lo);
+        u_hi = __reduce_max_sync(0xffffffffu, u_hi);
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+        if (lane == 0) a.units[(long long)b * n_u + u] = make_int4(min(u_lo, u_hi), u_hi, all_lo, all_hi);
+        return;
+    }
+    const int u = (blockIdx.x - q_ctas) * 128 + threadIdx.x;
+    if (u >= n_k) return;
+    const DenseMask& m = a.mask;
+    const int k_first = u * kDenseUnit, k_last = min(k_first + kDenseUnit, a.Sk) - 1;
+    int d = 0, k0 = 0, k1 = a.Sk, q0 = 0, q1 = a.Sq, q_end = a.Sq;
+    if (m.cu_q != nullptr) {
+        const int32_t *cq = m.cu_q + b * m.cu_stride, *ck = m.cu_k + b * m.cu_stride;
+        d = max(dense_count_le(ck, m.docs, k_first) - 1, 0);
+        const int d1 = min(dense_count_le(ck, m.docs, k_last) - 1, m.docs - 1);
+        if (d > d1) {
+            a.hulls[(long long)b * n_k + u] = make_int2(0, 0);
+            return;
+        }
+        k0 = min(max(__ldg(ck + d), 0), a.Sk);
+        k1 = min(max(__ldg(ck + d + 1), k0), a.Sk);
+        q0 = __ldg(cq + d);
+        q1 = __ldg(cq + d + 1);
+        q_end = __ldg(cq + d1 + 1);
+    } else if (m.k_len != nullptr) {
+        k1 = min(max(__ldg(m.k_len + b), 0), a.Sk);
+        if (k_first >= k1) q_end = 0;
+    }
+    if (m.causal) {
+        const int pre = m.prefix != nullptr ? min(max(__ldg(m.prefix + b * m.prefix_stride + d), 0), a.Sk) : 0;
+        const int key = max(k_first, k0);
+        if (key >= k0 + pre) q0 = max(q0, q1 - (k1 - key));
+    }
+    q0 = min(max(q0, 0), a.Sq);
+    a.hulls[(long long)b * n_k + u] = make_int2(q0, min(max(q_end, q0), a.Sq));
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+size_t dense_plan_bytes(const DenseArgs& a, bool backward) {
+    const size_t n_u = dense_units(a.Sq), n_k = dense_units(a.Sk);
+    return 256 + align256(a.B * n_u * kDenseUnit * sizeof(int4)) + align256(a.B * n_u * sizeof(int4)) + (backward ? align256(a.B * n_k * sizeof(int2)) : 0);
+}
+
+void dense_plan_carve(DenseArgs& a, void* workspace, bool backward) {
+    const size_t n_u = dense_units(a.Sq);
+    unsigned char* w = static_cast<unsigned char*>(workspace);
+    a.next_item = reinterpret_cast<int*>(w);
+    w += 256;
+    a.rows = reinterpret_cast<int4*>(w);
+    w += align256(a.B * n_u * kDenseUnit * sizeof(int4));
+    a.units = reinterpret_cast<int4*>(w);
+    w += align256(a.B * n_u * sizeof(int4));
+    a.hulls = backward ? reinterpret_cast<int2*>(w) : nullptr;
+}
+
+cudaError_t launch_dense_plan(const DenseArgs& a, cudaStream_t st) {
+    if (a.B > 65535) return cudaErrorInvalidConfiguration;
+    const int q_ctas = (dense_units(a.Sq) + 3) / 4, k_ctas = a.hulls != nullptr ? (dense_units(a.Sk) + 127) / 128 : 0;
+    if (q_ctas + k_ctas > 0) dense_plan_kernel<<<dim3(q_ctas + k_ctas, a.B), 128, 0, st>>>(a, q_ctas);
+    return cudaGetLastError();
+}
+
+}  // namespace lcbsa

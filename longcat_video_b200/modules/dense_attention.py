@@ -95,27 +95,28 @@ def _shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, sc
     return _Shape(scale, softcap, bool(causal), slopes, cu_q, cu_k, k_lens, prefix_lens)
 
 
-def _forward(q, k, v, shape: _Shape, need_lse: bool):
+def _forward(q, k, v, shape: _Shape, need_lse: bool, need_rest: bool = False):
     q, k, v = _as_abi(q), _as_abi(k), _as_abi(v)
     dev = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if need_lse else None
+    rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_rest else None
     lib, ref = L.lib(), ctypes.byref
     qd, kd, vd, od, sd = L.tensor_desc(q), L.tensor_desc(k), L.tensor_desc(v), L.tensor_desc(out), shape.desc()
     need = lib.lcbsa_dense_attn_workspace_bytes(ref(qd), ref(kd), 0)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     with L.on_device(dev):
         L.check(lib.lcbsa_dense_attn_fwd(ref(qd), ref(kd), ref(vd), ref(sd), ref(od), None if lse is None else lse.data_ptr(),
-                                         None if ws is None else ws.data_ptr(), need, L.current_stream(dev)))
-    return out, lse
+                                         None if rest is None else rest.data_ptr(), None if ws is None else ws.data_ptr(), need, L.current_stream(dev)))
+    return out, lse, rest
 
 
 class _DenseAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, shape):
-        out, lse = _forward(q, k, v, shape, True)
+        out, lse, rest = _forward(q, k, v, shape, True, True)
         numbers = [t for t in shape if isinstance(t, torch.Tensor)]
-        ctx.save_for_backward(q, k, v, out, lse, *numbers)
+        ctx.save_for_backward(q, k, v, out, lse, rest, *numbers)
         ctx.shape = shape._replace(**{n: None for n in shape._fields if isinstance(getattr(shape, n), torch.Tensor)})
         ctx.names = [n for n in shape._fields if isinstance(getattr(shape, n), torch.Tensor)]
         ctx.mark_non_differentiable(lse)
@@ -124,7 +125,7 @@ class _DenseAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
-        q, k, v, out, lse, *numbers = ctx.saved_tensors
+        q, k, v, out, lse, rest, *numbers = ctx.saved_tensors
         shape = ctx.shape._replace(**dict(zip(ctx.names, numbers)))
         q, k, v, out, dout = _as_abi(q), _as_abi(k), _as_abi(v), _as_abi(out), _as_abi(dout)
         dev = q.device
@@ -135,7 +136,7 @@ class _DenseAttention(torch.autograd.Function):
         need = lib.lcbsa_dense_attn_workspace_bytes(ref(qd), ref(kd), 1)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
         with L.on_device(dev):
-            L.check(lib.lcbsa_dense_attn_bwd(ref(qd), ref(kd), ref(vd), ref(od), ref(gd), ref(sd), lse.data_ptr(), ref(dqd), ref(dkd), ref(dvd),
+            L.check(lib.lcbsa_dense_attn_bwd(ref(qd), ref(kd), ref(vd), ref(od), ref(gd), ref(sd), lse.data_ptr(), rest.data_ptr(), ref(dqd), ref(dkd), ref(dvd),
                                              ws.data_ptr(), need, L.current_stream(dev)))
         return dq, dk, dv, None
 
@@ -169,5 +170,5 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _DenseAttention.apply(q, k, v, shape)
     else:
-        out, lse = _forward(q, k, v, shape, return_lse)
+        out, lse, _ = _forward(q, k, v, shape, return_lse)
     return (out, lse) if return_lse else out

@@ -28,7 +28,7 @@ def _scores(**kw):
 
 def _fwd(q, k, v, s, out, ws=None, n=0):
     ref = ctypes.byref
-    return L.lib().lcbsa_dense_attn_fwd(ref(q), ref(k), ref(v), ref(s), ref(out), None, ws, n, None), L.lib().lcbsa_last_error().decode()
+    return L.lib().lcbsa_dense_attn_fwd(ref(q), ref(k), ref(v), ref(s), ref(out), None, None, ws, n, None), L.lib().lcbsa_last_error().decode()
 
 
 def test_no_cpu_path():
@@ -70,9 +70,9 @@ def test_the_library_refuses_before_a_launch():
     f32 = _desc(1, 1, 8, 64, L.LCBSA_FP32)
     assert _fwd(f32, f32, f32, ok, f32)[0] == -2
     ref = ctypes.byref
-    rc = L.lib().lcbsa_dense_attn_bwd(ref(q), ref(k), ref(k), ref(q), ref(q), ref(ok), 4096, ref(q), ref(k), ref(k), None, 0, None)
+    rc = L.lib().lcbsa_dense_attn_bwd(ref(q), ref(k), ref(k), ref(q), ref(q), ref(ok), 4096, None, ref(q), ref(k), ref(k), None, 0, None)
     assert rc == -3
-    rc = L.lib().lcbsa_dense_attn_bwd(ref(q), ref(k), ref(k), ref(q), ref(q), ref(ok), None, ref(q), ref(k), ref(k), 4096, 1 << 30, None)
+    rc = L.lib().lcbsa_dense_attn_bwd(ref(q), ref(k), ref(k), ref(q), ref(q), ref(ok), None, None, ref(q), ref(k), ref(k), 4096, 1 << 30, None)
     assert rc == -1
 
 
