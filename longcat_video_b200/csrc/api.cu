@@ -569,7 +569,7 @@ static int dense_args(const char* what, const LcbsaTensor* q, const LcbsaTensor*
     if (q->size[0] != k->size[0] || q->size[3] != k->size[3]) return fail(LCBSA_EINVAL, "%s: q and k disagree on batch or head_dim", what);
     for (int i = 0; i < 4; ++i)
         if (k->size[i] != v->size[i]) return fail(LCBSA_EINVAL, "%s: k and v have different shapes", what);
-    if (k->size[1] < 1 || q->size[1] % k->size[1] != 0)
+    if (k->size[1] < 1 || q->size[1] < 1 || q->size[1] % k->size[1] != 0)
         return fail(LCBSA_EINVAL, "%s: %lld query heads do not share %lld key heads evenly", what, (long long)q->size[1], (long long)k->size[1]);
     if (!std::isfinite(sc->scale) || !std::isfinite(sc->cap) || sc->cap < 0.f) return fail(LCBSA_EINVAL, "%s: scale must be finite, cap finite and not negative", what);
     if ((sc->cu_q == nullptr) != (sc->cu_k == nullptr)) return fail(LCBSA_EINVAL, "%s: the documents of the queries and of the keys go together", what);
@@ -649,11 +649,12 @@ int lcbsa_dense_attn_bwd(const LcbsaTensor* q, const LcbsaTensor* k, const Lcbsa
     if (!lse && a.B * a.Hq * a.Sq > 0) return fail(LCBSA_EINVAL, "dense_attn_bwd: null lse");
     if (int rc = dense_workspace("dense_attn_bwd", workspace, workspace_bytes, lcbsa::dense_bwd_workspace_bytes(a))) return rc;
     a.o = view_of(out); a.dout = view_of(dout); a.dq = view_of(dq); a.dk = view_of(dk); a.dv = view_of(dv);
+    const char* why = "";
+    if (!lcbsa::dense_bwd_supported(a, &why)) return fail(LCBSA_EUNSUPPORTED, "dense_attn_bwd: %s", why);
     a.lse = const_cast<float*>(lse);
     a.rest = const_cast<void*>(rest);
     a.status = device_status_ptr();
     if (!a.status) return fail(LCBSA_ECUDA, "dense_attn_bwd: cannot resolve the device status words");
-    const char* why = "";
     cudaError_t e = lcbsa::launch_dense_bwd(a, workspace, static_cast<cudaStream_t>(stream), &why);
     if (e != cudaSuccess) return cuda_fail(e, "dense_attn_bwd", why);
     return LCBSA_OK;

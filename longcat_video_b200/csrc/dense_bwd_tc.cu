@@ -1,0 +1,873 @@
+// Dense attention backward (see dense_common.cuh for the forward's formulas): dq, dk, dv from dout, the output and the lse.
+//
+//   delta_i = dout_i . o_i        p_ij = exp(x_ij - lse_i)        dv_j = sum_i p_ij dout_i
+//   ds_ij = p_ij (dout_i . v_j - delta_i) (1 - tanh^2(s_ij / cap)) scale        dq_i = sum_j ds_ij k_j        dk_j = sum_i ds_ij q_i
+//
+// dk_j and dv_j also add up over the query heads that share the key head.  Two passes on TMA + tcgen05 + TMEM, so that every gradient is
+// summed by one CTA in one order and nothing is added with atomics.  A CTA owns a tile pair (A1, A2) of 128 rows and walks pairs
+// (B1, B2) of 64 rows:
+//
+//   dQ pass: A1 = Q  A2 = dO  B1 = K  B2 = V, over the keys that the rows see;   dK/dV pass: A1 = K  A2 = V  B1 = Q  B2 = dO, over
+//   the query units that may see the keys, query head after query head of the group
+//       S = A1 B1^T    dP = A2 B2^T    P, dS in registers, to TMEM in the input type    dQ += dS B1,  or  dV += P^T B2, dK += dS^T B1
+//
+// The roles of the warps, the rings and the TMEM columns are those of the block-sparse backward for 128-token blocks (attn_bwd_tc.cu), where
+// they are explained.  What differs: the walks are runs, so no lists are read; an entry is whole (all of its pairs are seen) or mixed, and
+// only mixed ones are masked pair by pair; a query unit brings what its rows see along with its lse and delta.
+//
+// Hidden values may be anything.  A hidden pair's P and dS are set to zero; in mixed entries the issuer of the gradient MMAs looks through the
+// tiles that are summed over and, once S and dP have read them, sets values that are not finite to zero (0 * inf is not 0).  A pair
+// that is seen has its NaN from S and dP; for dV it is the query's delta that says that dO is not finite.
+//
+// Every mbarrier wait is bounded; when one runs out the CTA flags the status word, drains its copies, frees TMEM, returns.
+#include <type_traits>
+
+#include "dense_common.cuh"
+#include "tc_common.cuh"
+
+namespace lcbsa {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kM = 128;                     // rows of an own tile
+constexpr int kBlk = kDenseUnit;            // rows of a streamed tile
+constexpr int kStatsBytes = 2 * kBlk * 4;   // -lse * log2(e) [64], -delta [64] of a query unit
+constexpr int kSeenBytes = kSeenPitch * 16; // what its rows see
+constexpr int kThreads = 384;
+constexpr int kRegsMath = 200, kRegsOther = 104;  // setmaxnreg: (200 + 200 + 104) * 128 = the 63 K registers of the launch
+constexpr int kItemRing = 4;
+
+template <int D> struct Lay {
+    static constexpr int aTile = kM * D * 2, aHalf = kM * 128;     // own tiles; a half: 64 columns, 128 B a row, 128B-swizzled
+    static constexpr int bTile = kBlk * D * 2, bHalf = kBlk * 128;
+    static constexpr int slots = D == 128 ? 4 : 8;                 // ring of (B1, B2) pairs
+    static constexpr int extra = kStatsBytes + kSeenBytes;
+    static constexpr int offA = 0;
+    static constexpr int offB = offA + 2 * aTile;
+    static constexpr int offExtra = offB + slots * 2 * bTile;
+    static constexpr int offBar = offExtra + slots * extra;
+    // barriers: full[slots], empty[slots], s_full[2], s_free[2], x_full[2], ts_done[2], a_full, a_empty, at_full, at_free, acc_done,
+    //           acc_free, item_full[kItemRing], item_empty[kItemRing]
+    static constexpr int numBars = 2 * slots + 8 + 6 + 2 * kItemRing;
+    static constexpr int offMisc = (offBar + numBars * 8 + 15) / 16 * 16;  // abort flag, TMEM base
+    static constexpr int offItems = offMisc + 64;
+    static constexpr int smem = offItems + kItemRing * 32;
+};
+static_assert(Lay<128>::offExtra % 16 == 0 && Lay<128>::extra % 16 == 0 && Lay<128>::offBar % 8 == 0, "bulk copies and barriers are aligned");
+
+// TMEM columns.  dQ pass: dQ 0, S 128 and 192, dP 256 (one buffer), dS 320 and 352, Q 384, dO 448.  dK/dV pass: dK 0, dV 128, S^T 256,
+// dP^T 320, P^T 384, dS^T 416 (one buffer each), K 448; V stays in shared memory.
+template <int kMode> struct Cols;
+template <> struct Cols<0> {
+    static constexpr uint32_t acc1 = 0, acc2 = 0, own1 = 384, own2 = 448;
+    static constexpr int bufs = 2;
+    __device__ static __forceinline__ uint32_t s(int buf) { return 128u + 64u * buf; }
+    static constexpr uint32_t dp = 256, xp = 0;
+    __device__ static __forceinline__ uint32_t xd(int buf) { return 320u + 32u * buf; }
+};
+template <> struct Cols<1> {
+    static constexpr uint32_t acc1 = 0, acc2 = 128, own1 = 448, own2 = 0;
+    static constexpr int bufs = 1;
+    __device__ static __forceinline__ uint32_t s(int) { return 256u; }
+    static constexpr uint32_t dp = 320, xp = 384;
+    __device__ static __forceinline__ uint32_t xd(int) { return 416u; }
+};
+
+struct BwdParams {
+    CUtensorMap tm_a1, tm_a2, tm_b1, tm_b2;
+    int fold_a1, fold_a2, fold_b1, fold_b2;  // bit 0: one head in the map, bit 1: one batch entry
+    const int4* seen;
+    const int2* hulls;
+    const float* stats;
+    const float* slopes;
+    int* next_item;
+    unsigned int* status;
+    void *out1, *out2;  // dQ pass: dq; dK/dV pass: dk, dv
+    long long o1_sb, o1_sh, o1_ss, o2_sb, o2_sh, o2_ss;
+    int B, Hq, Hk, group, n_u, n_k;  // query units, key units of an entry
+    int heads, n_own, rows;          // heads, own tiles of a head and rows of the own axis
+    int n_items;
+    float scale;
+    ScoreShape shape;
+};
+
+// called by a whole converged warp with warp-uniform operands, like the _elect copies of tc_common.cuh
+__device__ __forceinline__ void bulk_load_elect(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
+        ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+        : "memory");
+}
+
+// rowsum(dout * out) in fp32, out with what its rounding left: a half step of out moves dS by as much as rounding dS does (dq of a
+// causal row of 600 keys, bf16, is off by 1.53 times its own rounding without the rest, 1.46 with it).  D / 8 lanes a row; rows behind the last
+// query of their unit get zeros.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant__ DenseArgs a, long long total) {
+    constexpr int kLanes = D / 8;
+    const int sub = threadIdx.x % kLanes;
+    const long long r = (long long)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;  // (b * Hq + h) * units * 64 + row of the unit
+    const int n_u = dense_units(a.Sq);
+    float s = 0.f;
+    const long long bh = r / ((long long)n_u * kBlk);
+    const int i = (int)(r % ((long long)n_u * kBlk)), b = (int)(bh / a.Hq), h = (int)(bh % a.Hq);
+    const bool there = r < total && i < a.Sq;
+    if (there) {
+        const uint4 o = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o.data) + b * a.o.sb + h * a.o.sh + i * a.o.ss + sub * 8);
+        const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout.data) + b * a.dout.sb + h * a.dout.sh + i * a.dout.ss + sub * 8);
+        uint4 left = make_uint4(0u, 0u, 0u, 0u);
+        if (a.rest != nullptr) left = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.rest) + (bh * a.Sq + i) * D + sub * 8);
+        const T *op = reinterpret_cast<const T*>(&o), *gp = reinterpret_cast<const T*>(&g), *lp = reinterpret_cast<const T*>(&left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(DType<T>::to_f32(op[e]) + DType<T>::to_f32(lp[e]), DType<T>::to_f32(gp[e]), s);
+    }
+#pragma unroll
+    for (int x = kLanes / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    if (r < total && sub == 0) {
+        float* dst = a.stats + (r / kBlk) * (2 * kBlk) + r % kBlk;
+        dst[0] = there ? -(a.lse[bh * a.Sq + i] * kLog2e) : 0.f;
+        dst[kBlk] = there ? -s : 0.f;
+    }
+}
+
+// 64 columns of this thread's accumulator row -> 128 bytes of the row in global memory (input type)
+template <bool kBf16>
+__device__ __forceinline__ void store_row64(unsigned char* row_ptr, int col0, const uint32_t (&r)[64]) {
+#pragma unroll
+    for (int q8 = 0; q8 < 8; ++q8) {
+        uint4 pk;
+        pk.x = pack2(kBf16, __uint_as_float(r[q8 * 8 + 0]), __uint_as_float(r[q8 * 8 + 1]));
+        pk.y = pack2(kBf16, __uint_as_float(r[q8 * 8 + 2]), __uint_as_float(r[q8 * 8 + 3]));
+        pk.z = pack2(kBf16, __uint_as_float(r[q8 * 8 + 4]), __uint_as_float(r[q8 * 8 + 5]));
+        pk.w = pack2(kBf16, __uint_as_float(r[q8 * 8 + 6]), __uint_as_float(r[q8 * 8 + 7]));
+        *reinterpret_cast<uint4*>(row_ptr + (col0 + q8 * 8) * 2) = pk;
+    }
+}
+
+// whether one of the n scores is not small enough for the polynomial of the cap (or not a number)
+template <int n>
+__device__ __forceinline__ bool any_large(const uint32_t (&r)[n], float inv) {
+    uint32_t m[4] = {0u, 0u, 0u, 0u};  // magnitudes order like their bits, NaN above all
+#pragma unroll
+    for (int j = 0; j < n; ++j) m[j & 3] = max(m[j & 3], r[j] & 0x7fffffffu);
+    const float top = __uint_as_float(max(max(m[0], m[1]), max(m[2], m[3])));
+    return __any_sync(0xffffffffu, !(fabsf(inv) * top <= kCapSmall));
+}
+
+// kMode 0: dQ pass, 1: dK/dV pass.  Persistent, one CTA per SM.
+template <bool kBf16, int D, int kMode, bool kCap, bool kBias>
+__global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_constant__ BwdParams P) {
+    using C = Cols<kMode>;
+    using Ly = Lay<D>;
+    using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+    constexpr int kSlots = Ly::slots, kB = 2 * kSlots, kBufs = C::bufs, kHalves = D / 64;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const uint32_t sbase = smem_u32(smem);
+    const uint32_t bar0 = sbase + Ly::offBar;
+    // Entries are numbered over the whole kernel: entry s uses ring slot s % kSlots, S, P and dS of buffer s % kBufs.  Items with entries
+    // are numbered too, for the barriers that turn once an item.
+    auto bar_full = [&](int s) { return bar0 + 8u * s; };
+    auto bar_empty = [&](int s) { return bar0 + 8u * (kSlots + s); };
+    auto bar_s_full = [&](int buf) { return bar0 + 8u * (kB + buf); };
+    auto bar_s_free = [&](int buf) { return bar0 + 8u * (kB + 2 + buf); };
+    auto bar_x_full = [&](int buf) { return bar0 + 8u * (kB + 4 + buf); };
+    auto bar_ts_done = [&](int buf) { return bar0 + 8u * (kB + 6 + buf); };
+    const uint32_t bar_a_full = bar0 + 8u * (kB + 8), bar_a_empty = bar0 + 8u * (kB + 9), bar_at_full = bar0 + 8u * (kB + 10);
+    const uint32_t bar_at_free = bar0 + 8u * (kB + 11), bar_acc_done = bar0 + 8u * (kB + 12), bar_acc_free = bar0 + 8u * (kB + 13);
+    auto bar_item_full = [&](int k) { return bar0 + 8u * (kB + 14 + k); };
+    auto bar_item_empty = [&](int k) { return bar0 + 8u * (kB + 14 + kItemRing + k); };
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Ly::offMisc);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::offMisc + 32);
+    int4* items = reinterpret_cast<int4*>(smem + Ly::offItems);
+    const Ctl ctl{abort_flag, P.status};
+
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // provably warp-uniform
+    if (tid == 0) {
+        ctl_init(ctl);
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(bar_full(s), 2);  // one arrival per producer
+            mbar_init(bar_empty(s), 1);
+        }
+        for (int buf = 0; buf < 2; ++buf) {
+            mbar_init(bar_s_full(buf), 1);
+            mbar_init(bar_s_free(buf), kMode == 1 ? 8 : 4);  // one elected arrival per warp that works on an entry
+            mbar_init(bar_x_full(buf), kMode == 1 ? 8 : 4);
+            mbar_init(bar_ts_done(buf), 1);
+        }
+        mbar_init(bar_a_full, 1);
+        mbar_init(bar_a_empty, kMode == 1 ? 9 : 8);  // the arithmetic warps have moved it; dK/dV pass: and the last dP has read A2
+        mbar_init(bar_at_full, 8);
+        mbar_init(bar_at_free, 1);
+        mbar_init(bar_acc_done, 1);
+        mbar_init(bar_acc_free, 8);
+        for (int k = 0; k < kItemRing; ++k) {
+            mbar_init(bar_item_full(k), 1);
+            mbar_init(bar_item_empty(k), 11);  // every warp but the one that announces
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (sbase & 1023u) {  // the swizzled tiles need the base that the declaration asks for
+            *abort_flag = 1;
+            if (atomicCAS(P.status, 0u, 1u) == 0u) {
+                P.status[1] = blockIdx.x;
+                P.status[2] = sbase;
+                P.status[3] = 0;
+            }
+        }
+    }
+    if (warp == 9) {  // TMEM: all 512 columns, allocated and freed by the issuing warp
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const bool start_ok = *abort_flag == 0;  // else nothing runs, nothing is written
+
+    // An item: own tile `own` of head bh, n entries.  dQ pass: keys from `first` on, all rows see [all_lo, all_hi).  dK/dV pass: `span` query units
+    // from unit `first` on, for every query head of the group.  bh < 0: there is none, or the kernel is giving up.
+    struct Item {
+        int bh, own, first, n, all_lo, all_hi, span;
+    };
+    auto take_item = [&](unsigned k) {  // item number k of this CTA, for every warp but warp 8
+        Item it{-1, 0, 0, 0, 0, 0, 0};
+        if (!mbar_wait_warp(bar_item_full(k % kItemRing), (k / kItemRing) & 1, ctl, 200, k)) return it;
+        const int4 a = items[2 * (k % kItemRing)], c = items[2 * (k % kItemRing) + 1];
+        __syncwarp();
+        mbar_arrive_elect(bar_item_empty(k % kItemRing));
+        return Item{a.x, a.y, a.z, a.w, c.x, c.y, c.z};
+    };
+    // Whether some pair of an entry is hidden.  dQ pass: entry e of the item; dK/dV pass: the unit's summary against the own keys
+    auto mixed_keys = [](const Item& it, int e) {
+        const int k = it.first + kBlk * e;
+        return k < it.all_lo || k + kBlk > it.all_hi;
+    };
+    auto mixed_queries = [](const Item& it, const int4& unit) {
+        const int k = it.own * kM;
+        return k < unit.z || k + kM > unit.w;
+    };
+    auto seen_of_slot = [&](int slot) { return reinterpret_cast<const int4*>(smem + Ly::offExtra + slot * Ly::extra + kStatsBytes); };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+        if (!start_ok) {
+        } else if (warp == 8 || warp == 11) {
+            // ================================================================== TMA producers: warp 8 items, own tiles, B1 and what comes with it, warp 11 B2
+            const bool is_b1 = warp == 8;
+            const CUtensorMap* tm = is_b1 ? &P.tm_b1 : &P.tm_b2;
+            const int fold = is_b1 ? P.fold_b1 : P.fold_b2;
+            bool ok = true;
+            unsigned s = 0, kk = 0;  // entries, items with entries
+            int ahead2 = 0;          // number taken off the counter for the item behind the next
+            Item ahead{-1, 0, 0, 0, 0, 0, 0};
+            auto take = [&]() { return lane == 0 ? (int)gridDim.x + atomicAdd(P.next_item, 1) : 0; };
+            auto look = [&](int id) {
+                Item it{-1, 0, 0, 0, 0, 0, 0};
+                if (id >= P.n_items) return it;
+                const int heads = P.B * P.heads;
+                it.bh = id % heads;
+                const int b = it.bh / P.heads;
+                if (kMode == 0) {  // the last queries first: with a causal order they have most keys
+                    it.own = P.n_own - 1 - id / heads;
+                    const int4* u = P.seen + ((long long)b * P.n_u + 2 * it.own) * kSeenPitch + kBlk;
+                    int4 x = __ldg(u), y = make_int4(0, 0, 0, 0x7fffffff);
+                    if (2 * it.own + 1 < P.n_u) y = __ldg(u + kSeenPitch);
+                    const int lo = min(x.x < x.y ? x.x : 0x7fffffff, y.x < y.y ? y.x : 0x7fffffff), hi = max(x.y, y.y);
+                    it.n = hi > lo ? (hi - lo + kBlk - 1) / kBlk : 0;
+                    it.first = hi > lo ? lo : 0;
+                    it.all_lo = max(x.z, y.z);
+                    it.all_hi = min(x.w, y.w);
+                } else {  // the first keys first
+                    it.own = id / heads;
+                    const int2* hu = P.hulls + (long long)b * P.n_k + 2 * it.own;
+                    int2 x = __ldg(hu);
+                    if (2 * it.own + 1 < P.n_k) {
+                        const int2 y = __ldg(hu + 1);
+                        if (x.x >= x.y) x = y;
+                        else if (y.x < y.y) x = make_int2(min(x.x, y.x), max(x.y, y.y));
+                    }
+                    if (x.x < x.y) {
+                        it.first = x.x / kBlk;
+                        it.span = (x.y - 1) / kBlk - it.first + 1;
+                        it.n = it.span * P.group;
+                    }
+                }
+                return it;
+            };
+            if (is_b1) {
+                ahead = look(blockIdx.x);
+                ahead2 = take();
+            }
+            auto step = [&]() {
+                ahead = look(__shfl_sync(0xffffffffu, ahead2, 0));
+                ahead2 = take();
+            };
+            for (unsigned k = 0;; ++k) {
+                Item it;
+                if (is_b1) {
+                    it = ahead;
+                    ok = mbar_wait_warp(bar_item_empty(k % kItemRing), ((k / kItemRing) & 1) ^ 1, ctl, 201, k);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        items[2 * (k % kItemRing)] = make_int4(it.bh, it.own, it.first, it.n);
+                        items[2 * (k % kItemRing) + 1] = make_int4(it.all_lo, it.all_hi, it.span, 0);
+                        mbar_arrive(bar_item_full(k % kItemRing));
+                    }
+                    __syncwarp();
+                } else {
+                    it = take_item(k);
+                }
+                if (it.bh < 0) break;
+                if (it.n == 0) {
+                    if (is_b1) step();
+                    continue;
+                }
+                const int b = it.bh / P.heads, h = it.bh % P.heads;
+                if (is_b1) {
+                    ok = mbar_wait_warp(bar_a_empty, (kk & 1) ^ 1, ctl, 202, kk);
+                    if (!ok) break;
+                    mbar_arrive_tx_elect(bar_a_full, 2 * Ly::aTile);
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half) {
+                        tma_load_5d_elect(sbase + Ly::offA + half * Ly::aHalf, &P.tm_a1, bar_a_full, 64 * half, it.own * kM,
+                                          (P.fold_a1 & 1) ? 0 : h, (P.fold_a1 & 2) ? 0 : b, 0);
+                        tma_load_5d_elect(sbase + Ly::offA + Ly::aTile + half * Ly::aHalf, &P.tm_a2, bar_a_full, 64 * half, it.own * kM,
+                                          (P.fold_a2 & 1) ? 0 : h, (P.fold_a2 & 2) ? 0 : b, 0);
+                    }
+                }
+                ++kk;
+                int unit = it.first, head = kMode == 0 ? h / P.group : h * P.group;  // of the entry: dK/dV pass a query unit, dQ pass unused
+                for (int e = 0; e < it.n; ++e) {
+                    const int slot = s % kSlots;
+                    ok = mbar_wait_warp(bar_empty(slot), ((s / kSlots) & 1) ^ 1, ctl, 210 + kMode, s);
+                    if (!ok) break;
+                    ++s;
+                    const bool more = kMode == 1 && is_b1;
+                    mbar_arrive_tx_elect(bar_full(slot), Ly::bTile + (more ? Ly::extra : 0));
+                    const uint32_t dst = sbase + Ly::offB + slot * 2 * Ly::bTile + (is_b1 ? 0 : Ly::bTile);
+                    const int row = kMode == 0 ? it.first + kBlk * e : unit * kBlk;
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half)
+                        tma_load_5d_elect(dst + half * Ly::bHalf, tm, bar_full(slot), 64 * half, row, (fold & 1) ? 0 : head, (fold & 2) ? 0 : b, 0);
+                    if (more) {
+                        const uint32_t x = sbase + Ly::offExtra + slot * Ly::extra;
+                        bulk_load_elect(x, P.stats + (((long long)b * P.Hq + head) * P.n_u + unit) * (2 * kBlk), kStatsBytes, bar_full(slot));
+                        bulk_load_elect(x + kStatsBytes, P.seen + ((long long)b * P.n_u + unit) * kSeenPitch, kSeenBytes, bar_full(slot));
+                    }
+                    if (kMode == 1 && ++unit == it.first + it.span) {
+                        unit = it.first;
+                        ++head;
+                    }
+                    if (is_b1 && e == it.n - 1) step();  // behind the item's last copies, none of which waits for the counter
+                }
+                if (!ok) break;
+            }
+            if ((!ok || *abort_flag != 0) && lane == 0) {
+                // drain: give the copies this warp issued a bounded time to land before the CTA exits
+                const long long t0 = clock64();
+                while (is_b1 && kk > 0 && !mbar_try(bar_a_full, (kk - 1) & 1) && clock64() - t0 < 40000000ll) {
+                }
+                for (unsigned r = s > kSlots ? s - kSlots : 0; r < s; ++r)
+                    while (!mbar_try(bar_full(r % kSlots), (r / kSlots) & 1) && clock64() - t0 < 40000000ll) {
+                    }
+            }
+        } else if (warp == 9) {
+            // ================================================================== issuer of S and dP (S^T and dP^T)
+            const uint32_t idesc_ss = instr_desc(kBf16, kM, kBlk, 0);
+            const uint64_t a2d = smem_desc(sbase + Ly::offA + Ly::aTile, 16, 1024);  // dK/dV pass
+            bool ok = true;
+            unsigned s = 0, kk = 0;
+            for (unsigned k = 0; ok; ++k) {
+                const Item it = take_item(k);
+                if (it.bh < 0) break;
+                if (it.n == 0) continue;
+                ok = mbar_wait_warp(bar_at_full, kk & 1, ctl, 220 + kMode, kk);  // the own tiles are in TMEM
+                ++kk;
+                bool pre = false;
+                for (int e = 0; e < it.n && ok; ++e, ++s) {
+                    const int slot = s % kSlots, buf = s % kBufs;
+                    if (!pre) {  // not already seen ready by the look-ahead of the entry before
+                        ok = mbar_wait_warp(bar_full(slot), (s / kSlots) & 1, ctl, 222 + kMode, s);
+                        // the arithmetic warps hold the last S and dP in registers (dQ pass: seen before the dP of entry s - 1)
+                        if (ok && kMode == 1) ok = mbar_wait_warp(bar_s_free(0), (s & 1) ^ 1, ctl, 226, s);
+                        if (!ok) break;
+                    }
+                    tc_fence_after();
+                    const uint32_t tile = sbase + Ly::offB + slot * 2 * Ly::bTile;
+                    const uint64_t b1d = smem_desc(tile, 16, 1024), b2d = smem_desc(tile + Ly::bTile, 16, 1024);
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        // 32 bytes per 16-column step inside a 64-column half; 8 TMEM columns per step
+                        const uint64_t off = (uint64_t)(((j >> 2) * Ly::bHalf + (j & 3) * 32) >> 4);
+                        tc_mma_ts(tmem + C::s(buf), tmem + C::own1 + 8u * j, b1d + off, idesc_ss, j > 0);
+                    }
+                    // look ahead: probe the next entry's barriers between the two contractions and read the answer after them
+                    bool nf = false, ns = kMode == 0;
+                    if (e + 1 < it.n) {
+                        nf = mbar_test(bar_full((s + 1) % kSlots), ((s + 1) / kSlots) & 1);
+                        if (kMode == 1) ns = mbar_test(bar_s_free(0), ((s + 1) & 1) ^ 1);
+                    }
+                    tc_fence_after();
+                    if (kMode == 0 && s > 0) {  // dP of the entry before is in registers
+                        ok = mbar_wait_warp(bar_s_free((s - 1) & 1), ((s - 1) >> 1) & 1, ctl, 227, s);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        const uint64_t off = (uint64_t)(((j >> 2) * Ly::bHalf + (j & 3) * 32) >> 4);
+                        const uint64_t aoff = (uint64_t)(((j >> 2) * Ly::aHalf + (j & 3) * 32) >> 4);
+                        if (kMode == 1) tc_mma(tmem + C::dp, a2d + aoff, b2d + off, idesc_ss, j > 0);
+                        else tc_mma_ts(tmem + C::dp, tmem + C::own2 + 8u * j, b2d + off, idesc_ss, j > 0);
+                    }
+                    tc_commit(bar_s_full(buf));
+                    if (e == it.n - 1) {  // the own tiles have been read
+                        tc_commit(bar_at_free);
+                        if (kMode == 1) tc_commit(bar_a_empty);
+                    }
+                    __syncwarp();
+                    pre = __all_sync(0xffffffffu, nf && ns);
+                }
+            }
+        } else if (warp == 10) {
+            // ================================================================== issuer of the gradient MMAs: A from TMEM (8 columns
+            // per 16-row step), B the streamed tile, MN-major (64-column halves apart = LBO, 8-row groups 1 KiB apart = SBO, 16
+            // rows = 2 KiB per step)
+            const uint32_t idesc_ts = instr_desc(kBf16, kM, D, 1);
+            bool ok = true;
+            unsigned s = 0, kk = 0;
+            for (unsigned k = 0; ok; ++k) {
+                const Item it = take_item(k);
+                if (it.bh < 0) break;
+                if (it.n == 0) continue;
+                ok = mbar_wait_warp(bar_acc_free, (kk & 1) ^ 1, ctl, 244, kk);  // the gradients of the item before have been read
+                ++kk;
+                bool pre = false;
+                for (int e = 0; e < it.n && ok; ++e, ++s) {
+                    const int slot = s % kSlots, buf = s % kBufs;
+                    if (!pre) {
+                        ok = mbar_wait_warp(bar_full(slot), (s / kSlots) & 1, ctl, 228 + kMode, s);
+                        if (!ok) break;
+                    }
+                    unsigned char* const tiles = smem + Ly::offB + slot * 2 * Ly::bTile;
+                    // dQ pass: K is summed over; dK/dV pass: Q and dO
+                    constexpr int kLook = kMode == 0 ? Ly::bTile : 2 * Ly::bTile;
+                    bool bad = false;
+                    if (kMode == 0 ? mixed_keys(it, e) : mixed_queries(it, seen_of_slot(slot)[kBlk])) {
+#pragma unroll 8
+                        for (int c = lane; c < kLook / 16; c += 32) bad |= chunk_nonfinite<T>(reinterpret_cast<const uint4*>(tiles)[c]);
+                        bad = __any_sync(0xffffffffu, bad);
+                    }
+                    if (!pre) {
+                        ok = mbar_wait_warp(bar_x_full(buf), (s / kBufs) & 1, ctl, 224 + kMode, s);
+                        if (!ok) break;
+                    }
+                    if (LCBSA_UNLIKELY(bad)) {  // the arithmetic warps have S and dP, so their MMAs have read the tiles
+#pragma unroll 1
+                        for (int c = lane; c < kLook / 4; c += 32) {
+                            uint32_t* p = reinterpret_cast<uint32_t*>(tiles) + c;
+                            *p = zero_nonfinite<T>(*p);
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                    bool nf = false, nx = false;
+                    if (e + 1 < it.n) {
+                        nf = mbar_test(bar_full((s + 1) % kSlots), ((s + 1) / kSlots) & 1);
+                        nx = mbar_test(bar_x_full((s + 1) % kBufs), ((s + 1) / kBufs) & 1);
+                    }
+                    tc_fence_after();
+                    const uint32_t tile = sbase + Ly::offB + slot * 2 * Ly::bTile;
+                    const uint64_t b1m = smem_desc(tile, Ly::bHalf, 1024), b2m = smem_desc(tile + Ly::bTile, Ly::bHalf, 1024);
+                    if (kMode == 1) {
+#pragma unroll
+                        for (int j = 0; j < kBlk / 16; ++j)  // dV += P^T dO
+                            tc_mma_ts(tmem + C::acc2, tmem + C::xp + 8u * j, b2m + (uint64_t)((j * 2048) >> 4), idesc_ts, (e > 0 || j > 0) ? 1u : 0u);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kBlk / 16; ++j)  // dQ += dS K, or dK += dS^T Q
+                        tc_mma_ts(tmem + C::acc1, tmem + C::xd(buf) + 8u * j, b1m + (uint64_t)((j * 2048) >> 4), idesc_ts, (e > 0 || j > 0) ? 1u : 0u);
+                    tc_commit(bar_empty(slot));  // the streamed tiles are free once these MMAs have read them
+                    tc_commit(bar_ts_done(buf)); // and so are P and dS
+                    if (e == it.n - 1) tc_commit(bar_acc_done);
+                    __syncwarp();
+                    pre = __all_sync(0xffffffffu, nf && nx);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMath));
+        // ================================================================== arithmetic warps
+        const int wg = warp >> 2;  // dQ pass: entries wg, wg + 2, ...; dK/dV pass: columns 32 wg .. 32 wg + 31 of every entry
+        const int wq = warp & 3;   // TMEM quadrant of this warp
+        const int row = wq * 32 + lane;  // row of the own tile = TMEM lane
+        const uint32_t t_lane = (uint32_t)(wq * 32) << 16;
+        bool ok = start_ok;
+        unsigned s0 = 0, kk = 0;  // entries before the current item, items with entries before it
+        // The own tiles go from shared memory to TMEM, where they are the A operands of every S and dP.  dQ pass: warpgroup g moves A1 (0) or
+        // A2 (1); dK/dV pass: half g of A1.
+        auto own_to_tmem = [&](unsigned item) -> bool {
+            if (!mbar_wait_warp(bar_a_full, item & 1, ctl, 242, item)) return false;
+            if (item > 0 && !mbar_wait_warp(bar_at_free, (item - 1) & 1, ctl, 243, item)) return false;
+            tc_fence_after();
+            const int tile = kMode == 0 ? wg : 0;
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) {
+                if (kMode == 1 && half != wg) continue;
+                const unsigned char* src = smem + Ly::offA + tile * Ly::aTile + half * Ly::aHalf + row * 128;
+                uint32_t ar[32];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(src + ((c ^ (row & 7)) << 4));
+                    ar[4 * c + 0] = v.x;
+                    ar[4 * c + 1] = v.y;
+                    ar[4 * c + 2] = v.z;
+                    ar[4 * c + 3] = v.w;
+                }
+                tc_st32(tmem + (tile == 1 ? C::own2 : C::own1) + 32u * half + t_lane, ar);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            mbar_arrive_elect(bar_at_full);
+            mbar_arrive_elect(bar_a_empty);
+            return true;
+        };
+        const float2 sc = make_float2(P.scale, P.scale);
+        // Two scores and two dP -> P and dS.  nl, nd: -lse * log2(e) and -delta; far: distances.
+        auto pair = [&](float2 s, float2 dp, float2 nl, float2 nd, float2 far, float slope2, bool large, float2& p, float2& ds) {
+            float2 slack, x;
+            if (kCap) {
+                x = large ? capped_any(P.shape, s, slack) : capped_small(P.shape, s, slack);
+                if (kBias) x = __ffma2_rn(far, make_float2(-slope2, -slope2), x);
+                x = __fadd2_rn(x, nl);
+            } else {
+                if (kBias) nl = __ffma2_rn(far, make_float2(-slope2, -slope2), nl);
+                x = __ffma2_rn(s, make_float2(P.shape.mul, P.shape.mul), nl);
+            }
+            p = make_float2(ex2(x.x), ex2(x.y));
+            ds = __fmul2_rn(__fmul2_rn(p, __fadd2_rn(dp, nd)), sc);
+            if (kCap) ds = __fmul2_rn(ds, slack);
+        };
+        auto two = [](uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); };
+        // dQ pass: what this thread's query sees, its -lse * log2(e) and -delta, the slope of its head; dK/dV pass: nothing yet
+        struct Row {
+            int4 see;
+            float nl, nd, slope2;
+        };
+        auto row_of = [&](const Item& it) {
+            Row r{make_int4(0, 0, 0, 0), 0.f, 0.f, 0.f};
+            if (kMode == 0) {
+                const int b = it.bh / P.heads, h = it.bh % P.heads, i = it.own * kM + row, u = i / kBlk;
+                if (u < P.n_u) {
+                    r.see = P.seen[((long long)b * P.n_u + u) * kSeenPitch + i % kBlk];
+                    const float* st = P.stats + ((long long)it.bh * P.n_u + u) * (2 * kBlk) + i % kBlk;
+                    r.nl = st[0];
+                    r.nd = st[kBlk];
+                }
+                if (kBias) r.slope2 = __ldg(P.slopes + h) * kLog2e;
+            }
+            return r;
+        };
+        auto entries = [&](const Item& it, const Row& me) {
+            const unsigned n = it.n;
+            if constexpr (kMode == 0) {
+                for (unsigned i = s0 + ((s0 ^ wg) & 1); i < s0 + n && ok; i += 2) {  // buffer i & 1 = wg
+                    const unsigned r = i >> 1;
+                    const int key0 = it.first + kBlk * (int)(i - s0);
+                    ok = mbar_wait_warp(bar_s_full(wg), r & 1, ctl, 230 + wg, i);
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint32_t xd[32], sr[64], dr[64];
+                    tc_ld64(tmem + C::s(wg) + t_lane, sr);
+                    tc_ld64(tmem + C::dp + t_lane, dr);
+                    tc_wait_ld();
+                    tc_fence_before();
+                    mbar_arrive_elect(bar_s_free(wg));  // dP may be overwritten by that of entry i + 1, S by that of entry i + 2
+                    const bool large = kCap && any_large(sr, P.shape.inv);
+                    const bool mixed = mixed_keys(it, (int)(i - s0));
+                    const float at = (float)(me.see.z - key0);
+                    const int lo = me.see.x - key0, hi = me.see.y - key0;
+                    auto all = [&](bool lg, bool mx) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            float2 p, ds, far = make_float2(0.f, 0.f);
+                            if (kBias) far = make_float2(fabsf(at - (float)(2 * k)), fabsf(at - (float)(2 * k + 1)));
+                            pair(two(sr[2 * k], sr[2 * k + 1]), two(dr[2 * k], dr[2 * k + 1]), make_float2(me.nl, me.nl), make_float2(me.nd, me.nd), far,
+                                 me.slope2, lg, p, ds);
+                            if (mx) {
+                                if (2 * k < lo || 2 * k >= hi) ds.x = 0.f;
+                                if (2 * k + 1 < lo || 2 * k + 1 >= hi) ds.y = 0.f;
+                            }
+                            xd[k] = pack2(kBf16, ds.x, ds.y);
+                        }
+                    };
+                    if (kCap && LCBSA_UNLIKELY(large)) all(true, true);
+                    else if (mixed) all(false, true);
+                    else all(false, false);
+                    // TS of entry i - 2 has read the columns
+                    ok = mbar_wait_warp(bar_ts_done(wg), (r & 1) ^ 1, ctl, 236 + wg, i);
+                    if (!ok) break;
+                    tc_fence_after();
+                    tc_st32(tmem + C::xd(wg) + t_lane, xd);
+                    tc_wait_st();
+                    tc_fence_before();
+                    mbar_arrive_elect(bar_x_full(wg));
+                }
+            } else {
+                const int key = it.own * kM + row;
+                const int h0 = (it.bh % P.heads) * P.group;
+                int unit = 0, head = 0;  // of the entry, relative to the item's first
+                float slope2 = kBias ? __ldg(P.slopes + h0) * kLog2e : 0.f;
+                for (unsigned i = s0; i < s0 + n && ok; ++i) {  // columns 32 wg .. 32 wg + 31 of every entry
+                    const int slot = i % kSlots;
+                    // what came with the slot's tiles
+                    ok = mbar_wait_warp(bar_full(slot), (i / kSlots) & 1, ctl, 234 + wg, i);
+                    if (ok) ok = mbar_wait_warp(bar_s_full(0), i & 1, ctl, 232 + wg, i);
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint32_t sr[32], dr[32];
+                    tc_ld32(tmem + C::s(0) + 32u * wg + t_lane, sr);
+                    tc_ld32(tmem + C::dp + 32u * wg + t_lane, dr);
+                    tc_wait_ld();
+                    tc_fence_before();
+                    mbar_arrive_elect(bar_s_free(0));  // S^T and dP^T may be overwritten by the next entry's
+                    const float2* st2 = reinterpret_cast<const float2*>(smem + Ly::offExtra + slot * Ly::extra) + 16 * wg;
+                    const int4* const see = seen_of_slot(slot);
+                    const bool large = kCap && any_large(sr, P.shape.inv);
+                    const bool mixed = mixed_queries(it, see[kBlk]);
+                    // the queries of a whole entry belong to one document, so their places follow one another
+                    const float at = kBias ? (float)(see[0].z + 32 * wg - key) : 0.f;
+                    uint32_t xp[16], xd[16];
+                    auto all = [&](bool lg, bool mx) {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            float2 p, ds, far = make_float2(0.f, 0.f);
+                            const float2 nl = st2[k], nd = st2[k + kBlk / 2];
+                            int4 a = make_int4(0, 0, 0, 0), c = a;
+                            if (mx) {
+                                a = see[32 * wg + 2 * k];
+                                c = see[32 * wg + 2 * k + 1];
+                            }
+                            if (kBias) {
+                                far = make_float2(fabsf(at + (float)(2 * k)), fabsf(at + (float)(2 * k + 1)));
+                                if (mx) far = make_float2(fabsf((float)(a.z - key)), fabsf((float)(c.z - key)));
+                            }
+                            pair(two(sr[2 * k], sr[2 * k + 1]), two(dr[2 * k], dr[2 * k + 1]), nl, nd, far, slope2, lg, p, ds);
+                            if (mx) {
+                                if (!isfinite(nd.x)) p.x = __int_as_float(0x7fc00000);  // dO is not finite
+                                if (!isfinite(nd.y)) p.y = __int_as_float(0x7fc00000);
+                                if (key < a.x || key >= a.y) p.x = ds.x = 0.f;
+                                if (key < c.x || key >= c.y) p.y = ds.y = 0.f;
+                            }
+                            xp[k] = pack2(kBf16, p.x, p.y);
+                            xd[k] = pack2(kBf16, ds.x, ds.y);
+                        }
+                    };
+                    if (kCap && LCBSA_UNLIKELY(large)) all(true, true);
+                    else if (mixed) all(false, true);
+                    else all(false, false);
+                    if (++unit == it.span) {
+                        unit = 0;
+                        ++head;
+                        if (kBias && head < P.group) slope2 = __ldg(P.slopes + h0 + head) * kLog2e;
+                    }
+                    // TS of entry i - 1 has read the columns
+                    ok = mbar_wait_warp(bar_ts_done(0), (i & 1) ^ 1, ctl, 238 + wg, i);
+                    if (!ok) break;
+                    tc_fence_after();
+                    // 32 columns of the tile are 16 columns of 16-bit pairs
+                    tc_st16(tmem + C::xp + 16u * wg + t_lane, xp);
+                    tc_st16(tmem + C::xd(0) + 16u * wg + t_lane, xd);
+                    tc_wait_st();
+                    tc_fence_before();
+                    mbar_arrive_elect(bar_x_full(0));
+                }
+            }
+            s0 += n;
+        };
+        // The accumulated gradients of an item's rows: TMEM -> registers, which frees the accumulators -> global memory.  dQ pass: warpgroup
+        // g stores half g of dQ; dK/dV pass: warpgroup 0 dK, 1 dV.
+        auto store_item = [&](const Item& it, unsigned item) -> bool {
+            const int b = it.bh / P.heads, h = it.bh % P.heads, i = it.own * kM + row;
+            const bool second = kMode == 1 && wg == 1;
+            unsigned char* base = static_cast<unsigned char*>(second ? P.out2 : P.out1);
+            const long long sb = second ? P.o2_sb : P.o1_sb, sh = second ? P.o2_sh : P.o1_sh, ss = second ? P.o2_ss : P.o1_ss;
+            unsigned char* row_ptr = base + ((long long)b * sb + (long long)h * sh + (long long)i * ss) * 2;
+            const uint32_t t_acc = tmem + (second ? C::acc2 : C::acc1) + t_lane;
+            if (it.n > 0) {
+                if (!mbar_wait_warp(bar_acc_done, item & 1, ctl, 240 + kMode, item)) return false;
+            }
+            tc_fence_after();
+            constexpr int kParts = kMode == 1 ? kHalves : 1;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+                const int half = kMode == 1 ? part : wg;
+                uint32_t acc[64];
+                if (it.n > 0) {
+                    tc_ld64(t_acc + 64u * (half < kHalves ? half : 0), acc);
+                    tc_wait_ld();
+                    if (part == kParts - 1) {
+                        tc_fence_before();
+                        mbar_arrive_elect(bar_acc_free);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) acc[j] = 0u;  // nobody sees these rows, or they see nothing
+                }
+                if (i < P.rows && half < kHalves) store_row64<kBf16>(row_ptr, 64 * half, acc);
+            }
+            return true;
+        };
+        // Item by item; the own tiles and row values of the next one are fetched before the gradients of this one are stored.
+        unsigned k = 0;
+        Item cur{-1, 0, 0, 0, 0, 0, 0};
+        if (ok) cur = take_item(k++);
+        bool moved = false;
+        Row me = row_of(Item{0, P.n_own, 0, 0, 0, 0, 0}), me_n = me;
+        while (ok && cur.bh >= 0) {
+            if (cur.n > 0 && !moved) {
+                me = row_of(cur);
+                ok = own_to_tmem(kk);
+                if (!ok) break;
+            }
+            if (cur.n > 0) {
+                entries(cur, me);
+                if (!ok) break;
+            }
+            const Item nx = take_item(k++);
+            moved = cur.n > 0 && nx.bh >= 0 && nx.n > 0;
+            if (moved) {
+                me_n = row_of(nx);
+                ok = own_to_tmem(kk + 1);
+                if (!ok) break;
+            }
+            ok = store_item(cur, kk);
+            if (cur.n > 0) ++kk;
+            if (moved) me = me_n;
+            cur = nx;
+        }
+    }
+
+    // ---- teardown
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0) ctl_report(ctl);
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+template <bool kBf16, int D, int kMode, bool kCap, bool kBias>
+cudaError_t pass_launch(const BwdParams& P, cudaStream_t st) {
+    static thread_local unsigned long long raised = 0;  // devices (below 64) whose shared-memory limit this thread has raised for this kernel
+    int dev = 0, sm_count = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    if (dev > 63 || !((raised >> dev) & 1)) {
+        e = cudaFuncSetAttribute(dense_bwd_tc_kernel<kBf16, D, kMode, kCap, kBias>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::smem);
+        if (e != cudaSuccess) return e;
+        if (dev <= 63) raised |= 1ull << dev;
+    }
+    const int usable = sm_count - attn_sm_reserve() > 0 ? sm_count - attn_sm_reserve() : 1;
+    dense_bwd_tc_kernel<kBf16, D, kMode, kCap, kBias><<<P.n_items < usable ? P.n_items : usable, kThreads, Lay<D>::smem, st>>>(P);
+    return cudaGetLastError();
+}
+
+template <bool kBf16, int D, int kMode>
+cudaError_t pass_shape(const BwdParams& P, bool cap, cudaStream_t st) {
+    if (cap) return P.slopes ? pass_launch<kBf16, D, kMode, true, true>(P, st) : pass_launch<kBf16, D, kMode, true, false>(P, st);
+    return P.slopes ? pass_launch<kBf16, D, kMode, false, true>(P, st) : pass_launch<kBf16, D, kMode, false, false>(P, st);
+}
+
+template <bool kBf16, int D>
+cudaError_t passes(const DenseArgs& a, cudaStream_t st, const char** why) {
+    using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+    cudaError_t e = launch_dense_plan(a, st);
+    if (e != cudaSuccess) return e;
+    const long long total = (long long)a.B * a.Hq * dense_units(a.Sq) * kBlk;
+    constexpr int kRowsPerCta = 256 / (D / 8);
+    if (total > 0) {
+        if ((total + kRowsPerCta - 1) / kRowsPerCta > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+        dense_stats_kernel<T, D><<<(unsigned)((total + kRowsPerCta - 1) / kRowsPerCta), 256, 0, st>>>(a, total);
+        e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    BwdParams P{};
+    P.seen = a.seen; P.hulls = a.hulls; P.stats = a.stats; P.slopes = a.slopes; P.status = a.status;
+    P.B = a.B; P.Hq = a.Hq; P.Hk = a.Hk; P.group = a.group; P.n_u = dense_units(a.Sq); P.n_k = dense_units(a.Sk);
+    P.scale = a.scale;
+    P.shape = score_shape(a.scale, a.cap);
+    auto map = [&](CUtensorMap* tm, const View& v, int H, int S, int box, int* fold) {
+        if (S == 0 || dense_rows_map(tm, a.dtype, v, a.B, H, S, D, box, fold)) return true;
+        *why = "cuTensorMapEncodeTiled rejected a tensor";
+        return false;
+    };
+    const bool cap = a.cap > 0.f;
+    if (a.Sq > 0) {  // a call without keys still writes dq
+        if (!map(&P.tm_a1, a.q, a.Hq, a.Sq, kM, &P.fold_a1) || !map(&P.tm_a2, a.dout, a.Hq, a.Sq, kM, &P.fold_a2) ||
+            !map(&P.tm_b1, a.k, a.Hk, a.Sk, kBlk, &P.fold_b1) || !map(&P.tm_b2, a.v, a.Hk, a.Sk, kBlk, &P.fold_b2))
+            return cudaErrorInvalidValue;
+        P.out1 = const_cast<void*>(a.dq.data);
+        P.o1_sb = a.dq.sb; P.o1_sh = a.dq.sh; P.o1_ss = a.dq.ss;
+        P.heads = a.Hq; P.n_own = (a.Sq + kM - 1) / kM; P.rows = a.Sq;
+        P.n_items = a.B * a.Hq * P.n_own;
+        P.next_item = a.next_item;
+        e = pass_shape<kBf16, D, 0>(P, cap, st);
+        if (e != cudaSuccess) return e;
+    }
+    if (a.Sk > 0) {
+        if (!map(&P.tm_a1, a.k, a.Hk, a.Sk, kM, &P.fold_a1) || !map(&P.tm_a2, a.v, a.Hk, a.Sk, kM, &P.fold_a2) ||
+            !map(&P.tm_b1, a.q, a.Hq, a.Sq, kBlk, &P.fold_b1) || !map(&P.tm_b2, a.dout, a.Hq, a.Sq, kBlk, &P.fold_b2))
+            return cudaErrorInvalidValue;
+        P.out1 = const_cast<void*>(a.dk.data);
+        P.o1_sb = a.dk.sb; P.o1_sh = a.dk.sh; P.o1_ss = a.dk.ss;
+        P.out2 = const_cast<void*>(a.dv.data);
+        P.o2_sb = a.dv.sb; P.o2_sh = a.dv.sh; P.o2_ss = a.dv.ss;
+        P.heads = a.Hk; P.n_own = (a.Sk + kM - 1) / kM; P.rows = a.Sk;
+        P.n_items = a.B * a.Hk * P.n_own;
+        P.next_item = a.next_item + 1;
+        e = pass_shape<kBf16, D, 1>(P, cap, st);
+    }
+    return e;
+}
+
+}  // namespace
+
+// Operands are read through tensor maps: rows a stride apart.
+bool dense_bwd_supported(const DenseArgs& a, const char** why) {
+    const View* vs[4] = {&a.q, &a.dout, &a.k, &a.v};
+    const int len[4] = {a.Sq, a.Sq, a.Sk, a.Sk};
+    for (int i = 0; i < 4; ++i) {
+        if (len[i] > 1 && vs[i]->ss == 0) { *why = "tokens without a stride"; return false; }
+        if (vs[i]->ss * 2 >= (1ll << 40) || vs[i]->sh * 2 >= (1ll << 40) || vs[i]->sb * 2 >= (1ll << 40)) { *why = "stride too large for a tensor map"; return false; }
+    }
+    if ((long long)a.B * a.Hq * ((a.Sq + kM - 1) / kM) > 0x7fff0000ll || (long long)a.B * a.Hk * ((a.Sk + kM - 1) / kM) > 0x7fff0000ll) {
+        *why = "more tiles than a launch takes";
+        return false;
+    }
+    return true;
+}
+
+size_t dense_bwd_workspace_bytes(const DenseArgs& a) {
+    return dense_plan_bytes(a, true) + (size_t)a.B * a.Hq * dense_units(a.Sq) * kStatsBytes;
+}
+
+cudaError_t launch_dense_bwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why) {
+    if (a.B * a.Hq == 0) return cudaSuccess;
+    dense_plan_carve(a, workspace, true);
+    a.stats = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + dense_plan_bytes(a, true));
+    const cudaError_t e = a.dtype == LCBSA_BF16 ? (a.D == 128 ? passes<true, 128>(a, st, why) : passes<true, 64>(a, st, why))
+                                                : (a.D == 128 ? passes<false, 128>(a, st, why) : passes<false, 64>(a, st, why));
+    if (e == cudaErrorInvalidConfiguration) *why = "more CTAs than a launch takes";
+    return e;
+}
+
+}  // namespace lcbsa

@@ -7,12 +7,15 @@
 // query see ONE run of keys, so a mask is three numbers per query, and a tile of scores is whole, mixed or empty by four
 // numbers per 64 queries.  Kernels work in units of log2: scores carry a factor log2(e), exp is ex2.
 #pragma once
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace lcbsa {
 
 constexpr int kDenseCounters = 2;
-constexpr int kDenseUnit = 64;  // rows of a query unit, keys of a key unit
+constexpr int kDenseUnit = 64;              // rows of a query unit, keys of a key unit
+constexpr int kSeenPitch = kDenseUnit + 1;  // int4 of a query unit in the plan
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // What a query sees: keys [lo, hi); pos is its position among the keys.
@@ -38,10 +41,10 @@ struct DenseArgs {
     void* rest;            // nullable, dense [B, Hq, Sq, D] in the input type: what rounding the output left, for delta
     unsigned int* status;
     // carved out of the workspace (see dense_plan_kernel)
-    int4* rows;            // [B, units * 64]: lo, hi, pos, 0 of every query; rows behind the last query see nothing
-    int4* units;           // [B, units]: min lo, max hi over the rows of a unit that see a key, max lo, min hi over all of them
+    int4* seen;            // [B, units, 65]: lo, hi, pos, 0 of a unit's 64 queries (those behind the last see nothing), then
+                           // min lo, max hi over the rows that see a key, max lo, min hi over all rows
     int2* hulls;           // [B, key units]: first and one past the last query that can see a key of the unit (backward)
-    float* delta;          // [B*Hq, Sq] (backward)
+    float* stats;          // [B*Hq, units, 2, 64]: -lse * log2(e) and -rowsum(dout * out) of a unit's queries, 0 behind the last (backward)
     int* next_item;        // items taken by the persistent kernels, zero when they start
 };
 
@@ -80,19 +83,30 @@ __device__ __forceinline__ Seen dense_seen(const DenseMask& m, int b, int i, int
     return Seen{k0, hi, pos};
 }
 
-// Score of one pair in units of log2, as the exponent of its probability.  mul: scale * log2(e), with a cap 2 * scale / cap * log2(e).
-//   cap tanh(y) = cap - 2 cap / (1 + exp(2 y)): two special functions, exact at both ends (exp = inf: cap; exp = 0: -cap), off by a few
-//   2^-24 of the cap in between; the machine's own tanh is off by 2^-11, which a cap of 50 would make 2 % of a probability.
+// A score in units of log2, as the exponent of its probability: x2 = scale log2(e) s, with a cap cap log2(e) tanh(y), y = scale s / cap.
+//
+//   Any y: tanh(y) = 1 - t, t = 2 / (1 + exp(2 y)): two special functions, right at both ends (exp = inf: 1; exp = 0: -1), off by a few
+//   2^-24 in between.  (The machine's own tanh is off by 2^-11, which a cap of 50 would make 2 % of a probability.)
+//   |y| <= 0.75: tanh(y) = y p(y^2), p of degree 5 through the Chebyshev nodes of [0, 0.75^2], off by 1.3 * 2^-23 of the value, on the
+//   arithmetic units, which have time where the special functions (16 a clock and SM) are what a tile waits for.
 struct ScoreShape {
-    float mul, cap2, slope2;  // cap2: cap * log2(e), slope2: slope of the head * log2(e)
+    float mul;     // scale * log2(e)
+    float inv;     // scale / cap
+    float mul_ex;  // 2 * scale / cap * log2(e)
+    float cap2;    // cap * log2(e)
+    float slope2;  // slope of the head * log2(e)
 };
 inline ScoreShape score_shape(float scale, float cap) {
+    const double e = 1.4426950408889634;
     ScoreShape s;
-    s.mul = cap > 0.f ? (float)(2.0 * (double)scale / (double)cap * 1.4426950408889634) : scale * kLog2e;
-    s.cap2 = cap * kLog2e;
+    s.mul = (float)(scale * e);
+    s.inv = cap > 0.f ? (float)((double)scale / cap) : 0.f;
+    s.mul_ex = cap > 0.f ? (float)(2.0 * scale / cap * e) : 0.f;
+    s.cap2 = (float)(cap * e);
     s.slope2 = 0.f;
     return s;
 }
+constexpr float kCapSmall = 0.75f;
 __device__ __forceinline__ float dense_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -103,18 +117,24 @@ __device__ __forceinline__ float dense_rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// far: |pos - key| (kBias).  tanh2: 2 / (1 + exp(2 y)), from which the backward has 1 - tanh^2 = tanh2 (2 - tanh2).
-template <bool kCap, bool kBias>
-__device__ __forceinline__ float shaped_score(const ScoreShape& f, float s, float far, float& tanh2) {
-    float x;
-    if (kCap) {
-        tanh2 = 2.f * dense_rcp(1.f + dense_ex2(s * f.mul));
-        x = fmaf(-f.cap2, tanh2, f.cap2);
-    } else {
-        x = s * f.mul;
-    }
-    if (kBias) x = fmaf(-f.slope2, far, x);
-    return x;
+// Two scores -> cap log2(e) tanh(y), and 1 - tanh(y)^2 (used by the backward)
+__device__ __forceinline__ float2 capped_any(const ScoreShape& f, float2 s, float2& slack) {
+    const float2 t = make_float2(2.f * dense_rcp(1.f + dense_ex2(s.x * f.mul_ex)), 2.f * dense_rcp(1.f + dense_ex2(s.y * f.mul_ex)));
+    const float2 c = make_float2(f.cap2, f.cap2), m = make_float2(-f.cap2, -f.cap2);
+    slack = __fmul2_rn(t, __fadd2_rn(make_float2(2.f, 2.f), make_float2(-t.x, -t.y)));
+    return __ffma2_rn(t, m, c);
+}
+__device__ __forceinline__ float2 capped_small(const ScoreShape& f, float2 s, float2& slack) {
+    auto both = [](float x) { return make_float2(x, x); };
+    const float2 y = __fmul2_rn(s, both(f.inv)), z = __fmul2_rn(y, y);
+    float2 p = __ffma2_rn(z, both(-0.004711522255092859f), both(0.019576216116547585f));
+    p = __ffma2_rn(p, z, both(-0.05334111675620079f));
+    p = __ffma2_rn(p, z, both(0.13325339555740356f));
+    p = __ffma2_rn(p, z, both(-0.33332952857017517f));
+    p = __ffma2_rn(p, z, both(1.f));
+    const float2 t = __fmul2_rn(y, p);
+    slack = __ffma2_rn(t, make_float2(-t.x, -t.y), both(1.f));
+    return __fmul2_rn(__fmul2_rn(s, both(f.mul)), p);
 }
 
 // Whether one of the eight 16-bit values of a 16-byte chunk is an infinity or a NaN (all exponent bits set).
@@ -138,13 +158,15 @@ __device__ __forceinline__ uint32_t zero_nonfinite(uint32_t u) {
 size_t dense_plan_bytes(const DenseArgs& a, bool backward);
 void dense_plan_carve(DenseArgs& a, void* workspace, bool backward);
 cudaError_t launch_dense_plan(const DenseArgs& a, cudaStream_t st);
-// dense_tc.cu: the forward on tcgen05
-bool dense_tc_supported(const DenseArgs& a);
-cudaError_t launch_dense_tc(const DenseArgs& a, cudaStream_t st, const char** why);
-// dense_few.cu: any number of queries, made for few of them; dense_bwd.cu: the plan and the backward
+// dense_few.cu: the entry to the forward, and the kernel for few queries; dense_tc.cu: the forward on tcgen05; dense_bwd_tc.cu: the backward
 bool dense_supported(const DenseArgs& a, const char** why);
 size_t dense_fwd_workspace_bytes(const DenseArgs& a);
 cudaError_t launch_dense_fwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why);
+bool dense_tc_supported(const DenseArgs& a);
+cudaError_t launch_dense_tc(const DenseArgs& a, cudaStream_t st, const char** why);
+// a tensor map over [B, H, S, D] rows in boxes of `box` rows x 64 columns (dense_tc.cu)
+bool dense_rows_map(CUtensorMap* tm, int dtype, const View& v, int B, int H, int S, int D, int box, int* fold);
+bool dense_bwd_supported(const DenseArgs& a, const char** why);
 size_t dense_bwd_workspace_bytes(const DenseArgs& a);
 cudaError_t launch_dense_bwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why);
 

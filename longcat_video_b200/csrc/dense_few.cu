@@ -106,10 +106,10 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
 
     const int ra = lane >> 2, rb = ra + 8;  // the thread's two rows
     const int4 sa = seen_s[ra], sb = seen_s[rb];
-    ScoreShape fa = P.shape, fb = P.shape;
+    float slope_a = 0.f, slope_b = 0.f;
     if (kBias) {
-        if (row0 + ra < P.rows) fa.slope2 = __ldg(a.slopes + hk * a.group + (row0 + ra) % a.group) * kLog2e;
-        if (row0 + rb < P.rows) fb.slope2 = __ldg(a.slopes + hk * a.group + (row0 + rb) % a.group) * kLog2e;
+        if (row0 + ra < P.rows) slope_a = __ldg(a.slopes + hk * a.group + (row0 + ra) % a.group) * kLog2e;
+        if (row0 + rb < P.rows) slope_b = __ldg(a.slopes + hk * a.group + (row0 + rb) % a.group) * kLog2e;
     }
 
     float o[D / 8][4];
@@ -171,9 +171,14 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int j = key0 + nt * 8 + 2 * (lane & 3) + e;
-                float t2;
-                float xa = shaped_score<kCap, kBias>(fa, s[nt][e], fabsf((float)(sa.z - j)), t2);
-                float xb = shaped_score<kCap, kBias>(fb, s[nt][2 + e], fabsf((float)(sb.z - j)), t2);
+                float2 x = make_float2(s[nt][e], s[nt][2 + e]), slack;
+                if (kCap) x = capped_any(P.shape, x, slack);
+                else x = make_float2(x.x * P.shape.mul, x.y * P.shape.mul);
+                float xa = x.x, xb = x.y;
+                if (kBias) {
+                    xa = fmaf(-slope_a, fabsf((float)(sa.z - j)), xa);
+                    xb = fmaf(-slope_b, fabsf((float)(sb.z - j)), xb);
+                }
                 if (mixed) {
                     if (j < sa.x || j >= min(sa.y, end)) xa = -INFINITY;
                     if (j < sb.x || j >= min(sb.y, end)) xb = -INFINITY;

@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(128) dense_plan_kernel(const __grid_constant__
             const int i = u * kDenseUnit + e * 32 + lane;
             Seen s{0, 0, 0};
             if (i < a.Sq) s = dense_seen(a.mask, b, i, a.Sq, a.Sk);
-            a.rows[(long long)b * n_u * kDenseUnit + i] = make_int4(s.lo, s.hi, s.pos, 0);
+            a.seen[((long long)b * n_u + u) * kSeenPitch + e * 32 + lane] = make_int4(s.lo, s.hi, s.pos, 0);
             if (s.lo < s.hi) {
                 u_lo = min(u_lo, s.lo);
                 u_hi = max(u_hi, s.hi);
@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(128) dense_plan_kernel(const __grid_constant__
         u_hi = __reduce_max_sync(0xffffffffu, u_hi);
         all_lo = __reduce_max_sync(0xffffffffu, all_lo);
         all_hi = __reduce_min_sync(0xffffffffu, all_hi);
-        if (lane == 0) a.units[(long long)b * n_u + u] = make_int4(min(u_lo, u_hi), u_hi, all_lo, all_hi);
+        if (lane == 0) a.seen[((long long)b * n_u + u) * kSeenPitch + kDenseUnit] = make_int4(min(u_lo, u_hi), u_hi, all_lo, all_hi);
         return;
     }
     const int u = (blockIdx.x - q_ctas) * 128 + threadIdx.x;
@@ -75,7 +75,7 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 size_t dense_plan_bytes(const DenseArgs& a, bool backward) {
     const size_t n_u = dense_units(a.Sq), n_k = dense_units(a.Sk);
-    return 256 + align256(a.B * n_u * kDenseUnit * sizeof(int4)) + align256(a.B * n_u * sizeof(int4)) + (backward ? align256(a.B * n_k * sizeof(int2)) : 0);
+    return 256 + align256(a.B * n_u * kSeenPitch * sizeof(int4)) + (backward ? align256(a.B * n_k * sizeof(int2)) : 0);
 }
 
 void dense_plan_carve(DenseArgs& a, void* workspace, bool backward) {
@@ -83,10 +83,8 @@ void dense_plan_carve(DenseArgs& a, void* workspace, bool backward) {
     unsigned char* w = static_cast<unsigned char*>(workspace);
     a.next_item = reinterpret_cast<int*>(w);
     w += 256;
-    a.rows = reinterpret_cast<int4*>(w);
-    w += align256(a.B * n_u * kDenseUnit * sizeof(int4));
-    a.units = reinterpret_cast<int4*>(w);
-    w += align256(a.B * n_u * sizeof(int4));
+    a.seen = reinterpret_cast<int4*>(w);
+    w += align256(a.B * n_u * kSeenPitch * sizeof(int4));
     a.hulls = backward ? reinterpret_cast<int2*>(w) : nullptr;
 }
 

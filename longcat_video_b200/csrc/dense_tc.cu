@@ -69,7 +69,7 @@ struct Item {  // n: units, -1: no more items.  All rows see the keys [all_lo, a
 struct TcParams {
     CUtensorMap tm_q, tm_kv[2], tm_o;  // tm_kv[0]: K, [1]: V
     int fold_q, fold_k, fold_v, fold_o;  // bit 0: one head in the map, bit 1: one batch entry (axes with stride 0 or length 1)
-    const int4 *rows, *units;
+    const int4* seen;
     const float* slopes;
     int* next_item;
     float* lse;
@@ -83,6 +83,19 @@ struct TcParams {
 };
 
 // ------------------------------------------------------------------------------------------ kernel
+
+__device__ __forceinline__ float2 get2(const uint32_t (&r)[64], int j) { return make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); }
+__device__ __forceinline__ void put2(uint32_t (&r)[64], int j, float2 v) {
+    r[j] = __float_as_uint(v.x);
+    r[j + 1] = __float_as_uint(v.y);
+}
+// the largest magnitude of a row of scores, NaN if there is one
+__device__ __forceinline__ float row_size(const uint32_t (&r)[64]) {
+    uint32_t m[4] = {0u, 0u, 0u, 0u};  // magnitudes order like their bits, NaN above all
+#pragma unroll
+    for (int j = 0; j < 64; ++j) m[j & 3] = max(m[j & 3], r[j] & 0x7fffffffu);
+    return __uint_as_float(max(max(m[0], m[1]), max(m[2], m[3])));
+}
 
 template <bool kBf16, int D, bool kCap, bool kBias>
 __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_constant__ TcParams P) {
@@ -297,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                 if (LCBSA_UNLIKELY(bad)) {  // values of V that are not finite, to the rows that see them in mixed units
                     const int b = cur.bh / P.Hq, h = cur.bh - b * P.Hq;
                     const T* vh = static_cast<const T*>(P.v) + (long long)b * P.v_sb + (long long)(h / P.group) * P.v_sh;
-                    const int4 see = i_row < P.Sq ? P.rows[(long long)b * P.n_u * kDenseUnit + i_row] : make_int4(0, 0, 0, 0);
+                    const int4 see = i_row < P.Sq ? P.seen[((long long)b * P.n_u + i_row / kDenseUnit) * kSeenPitch + i_row % kDenseUnit] : make_int4(0, 0, 0, 0);
 #pragma unroll 1
                     for (int i = 0; i < cur.n; ++i) {
                         if (!mixed_unit(cur, i)) continue;
@@ -375,9 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
             if (idx < bh_total * P.tiles) {
                 it.tile = P.tiles - 1 - idx / bh_total;
                 it.bh = idx % bh_total;
-                const int4* u = P.units + (long long)(it.bh / P.Hq) * P.n_u + 2 * it.tile;
+                const int4* u = P.seen + ((long long)(it.bh / P.Hq) * P.n_u + 2 * it.tile) * kSeenPitch + kDenseUnit;
                 int4 a = __ldg(u), c = make_int4(0, 0, 0, 0x7fffffff);
-                if (2 * it.tile + 1 < P.n_u) c = __ldg(u + 1);
+                if (2 * it.tile + 1 < P.n_u) c = __ldg(u + kSeenPitch);
                 const int lo = min(a.x < a.y ? a.x : 0x7fffffff, c.x < c.y ? c.x : 0x7fffffff), hi = max(a.y, c.y);
                 it.n = hi > lo ? (hi - lo + kBlk - 1) / kBlk : 0;
                 it.key0 = hi > lo ? lo : 0;
@@ -598,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
             if (!ok || cur.n < 0) break;
             const int n_iter = rounds(cur);
             const int b = cur.bh / P.Hq, i_row = cur.tile * kQRows + row;
-            const int4 see = i_row < P.n_u * kDenseUnit ? P.rows[(long long)b * P.n_u * kDenseUnit + i_row] : make_int4(0, 0, 0, 0);
+            const int4 see = i_row < P.n_u * kDenseUnit ? P.seen[((long long)b * P.n_u + i_row / kDenseUnit) * kSeenPitch + i_row % kDenseUnit] : make_int4(0, 0, 0, 0);
             ScoreShape f = P.shape;
             if (kBias) f.slope2 = __ldg(P.slopes + (cur.bh - b * P.Hq)) * kLog2e;
 
@@ -620,12 +633,22 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                 uint4 pk[8];  // this row of P in the input type, 8 keys per 16-byte chunk
                 if (active) {
                     const int key0 = cur.key0 + kBlk * i;
-                    if (kShaped) {
+                    if (kCap) {
+                        float2 slack;
+                        if (__any_sync(0xffffffffu, !(fabsf(f.inv) * row_size(sr) <= kCapSmall))) {  // a NaN too
+#pragma unroll
+                            for (int j = 0; j < 64; j += 2) put2(sr, j, capped_any(f, get2(sr, j), slack));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 64; j += 2) put2(sr, j, capped_small(f, get2(sr, j), slack));
+                        }
+                    }
+                    if (kBias) {
                         const float at = (float)(see.z - key0);
 #pragma unroll
                         for (int j = 0; j < 64; ++j) {
-                            float t2;
-                            sr[j] = __float_as_uint(shaped_score<kCap, kBias>(f, __uint_as_float(sr[j]), fabsf(at - (float)j), t2));
+                            const float x = kCap ? __uint_as_float(sr[j]) : __uint_as_float(sr[j]) * f.mul;
+                            sr[j] = __float_as_uint(fmaf(-f.slope2, fabsf(at - (float)j), x));
                         }
                     }
                     if (mixed_unit(cur, i)) {
@@ -758,22 +781,6 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
     }
 }
 
-// A map over [B, H, S, D] rows, boxes of `box` rows x 64 columns.  Axes of length 1 or stride 0 become one entry (fold).
-bool rows_map(CUtensorMap* tm, int dtype, const View& v, int B, int H, int S, int D, int box, int* fold) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    *fold = (H == 1 || v.sh == 0 ? 1 : 0) | (B == 1 || v.sb == 0 ? 2 : 0);
-    const long long row = S == 1 ? D : v.ss;
-    const cuuint64_t one = (cuuint64_t)row * 2;  // any legal stride for an axis of one entry
-    cuuint64_t dims[5] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)((*fold & 1) ? 1 : H), (cuuint64_t)((*fold & 2) ? 1 : B), 1};
-    cuuint64_t strides[4] = {one, (*fold & 1) ? one : (cuuint64_t)v.sh * 2, (*fold & 2) ? one : (cuuint64_t)v.sb * 2, one};
-    cuuint32_t boxes[5] = {64u, (cuuint32_t)box, 1u, 1u, 1u};
-    cuuint32_t estr[5] = {1u, 1u, 1u, 1u, 1u};
-    const CUtensorMapDataType dt = dtype == LCBSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    return fn(tm, dt, 5, const_cast<void*>(v.data), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <bool kBf16, int D, bool kCap, bool kBias>
 cudaError_t tc_launch(const TcParams& P, int grid, cudaStream_t st) {
     static thread_local unsigned long long raised = 0;  // devices (below 64) whose shared-memory limit this thread has raised for this kernel
@@ -797,6 +804,22 @@ cudaError_t tc_shape(const TcParams& P, bool cap, int grid, cudaStream_t st) {
 
 }  // namespace
 
+// A map over [B, H, S, D] rows, boxes of `box` rows x 64 columns.  Axes of length 1 or stride 0 become one entry (fold).
+bool dense_rows_map(CUtensorMap* tm, int dtype, const View& v, int B, int H, int S, int D, int box, int* fold) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    *fold = (H == 1 || v.sh == 0 ? 1 : 0) | (B == 1 || v.sb == 0 ? 2 : 0);
+    const long long row = S == 1 ? D : v.ss;
+    const cuuint64_t one = (cuuint64_t)row * 2;  // any legal stride for an axis of one entry
+    cuuint64_t dims[5] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)((*fold & 1) ? 1 : H), (cuuint64_t)((*fold & 2) ? 1 : B), 1};
+    cuuint64_t strides[4] = {one, (*fold & 1) ? one : (cuuint64_t)v.sh * 2, (*fold & 2) ? one : (cuuint64_t)v.sb * 2, one};
+    cuuint32_t boxes[5] = {64u, (cuuint32_t)box, 1u, 1u, 1u};
+    cuuint32_t estr[5] = {1u, 1u, 1u, 1u, 1u};
+    const CUtensorMapDataType dt = dtype == LCBSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return fn(tm, dt, 5, const_cast<void*>(v.data), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool dense_tc_supported(const DenseArgs& a) {
     const View* vs[4] = {&a.q, &a.k, &a.v, &a.o};
     const int len[4] = {a.Sq, a.Sk, a.Sk, a.Sq};
@@ -810,14 +833,14 @@ bool dense_tc_supported(const DenseArgs& a) {
 // The plan (rows, units, next_item zeroed) is in place when the kernel runs.
 cudaError_t launch_dense_tc(const DenseArgs& a, cudaStream_t st, const char** why) {
     TcParams P;
-    if (!rows_map(&P.tm_q, a.dtype, a.q, a.B, a.Hq, a.Sq, a.D, kQRows, &P.fold_q) ||
-        !rows_map(&P.tm_kv[0], a.dtype, a.k, a.B, a.Hk, a.Sk, a.D, kBlk, &P.fold_k) ||
-        !rows_map(&P.tm_kv[1], a.dtype, a.v, a.B, a.Hk, a.Sk, a.D, kBlk, &P.fold_v) ||
-        !rows_map(&P.tm_o, a.dtype, a.o, a.B, a.Hq, a.Sq, a.D, kQRows, &P.fold_o)) {
+    if (!dense_rows_map(&P.tm_q, a.dtype, a.q, a.B, a.Hq, a.Sq, a.D, kQRows, &P.fold_q) ||
+        !dense_rows_map(&P.tm_kv[0], a.dtype, a.k, a.B, a.Hk, a.Sk, a.D, kBlk, &P.fold_k) ||
+        !dense_rows_map(&P.tm_kv[1], a.dtype, a.v, a.B, a.Hk, a.Sk, a.D, kBlk, &P.fold_v) ||
+        !dense_rows_map(&P.tm_o, a.dtype, a.o, a.B, a.Hq, a.Sq, a.D, kQRows, &P.fold_o)) {
         *why = "cuTensorMapEncodeTiled rejected a tensor";
         return cudaErrorInvalidValue;
     }
-    P.rows = a.rows; P.units = a.units; P.slopes = a.slopes; P.next_item = a.next_item;
+    P.seen = a.seen; P.slopes = a.slopes; P.next_item = a.next_item;
     P.lse = a.lse; P.rest = a.rest;
     P.v = a.v.data; P.v_sb = a.v.sb; P.v_sh = a.v.sh; P.v_ss = a.v.ss;
     P.status = a.status;

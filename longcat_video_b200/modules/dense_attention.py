@@ -127,7 +127,7 @@ class _DenseAttention(torch.autograd.Function):
     def backward(ctx, dout, _):
         q, k, v, out, lse, rest, *numbers = ctx.saved_tensors
         shape = ctx.shape._replace(**dict(zip(ctx.names, numbers)))
-        q, k, v, out, dout = _as_abi(q), _as_abi(k), _as_abi(v), _as_abi(out), _as_abi(dout)
+        q, k, v, out, dout = (_as_abi(t) if t.shape[2] <= 1 or t.stride(2) else t.contiguous() for t in (q, k, v, out, dout))
         dev = q.device
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
         lib, ref = L.lib(), ctypes.byref

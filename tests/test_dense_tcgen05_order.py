@@ -3,7 +3,7 @@ import pytest
 
 from tests import test_tcgen05_order as order
 
-SOURCES = ["dense_tc.cu"]
+SOURCES = ["dense_tc.cu", "dense_bwd_tc.cu"]
 
 
 @pytest.mark.parametrize("name", SOURCES)
