@@ -33,7 +33,7 @@ using namespace tc;
 
 constexpr int kM = 128;                     // rows of an own tile
 constexpr int kBlk = kDenseUnit;            // rows of a streamed tile
-constexpr int kStatsBytes = 2 * kBlk * 4;   // -lse * log2(e) [64], -delta [64] of a query unit
+constexpr int kStatsBytes = kDenseStats * 4;  // of a query unit
 constexpr int kSeenBytes = kSeenPitch * 16; // what its rows see
 constexpr int kThreads = 384;
 constexpr int kRegsMath = 200, kRegsOther = 104;  // setmaxnreg: (200 + 200 + 104) * 128 = the 63 K registers of the launch
@@ -101,37 +101,6 @@ __device__ __forceinline__ void bulk_load_elect(uint32_t dst, const void* src, u
         "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
         ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
         : "memory");
-}
-
-// rowsum(dout * out) in fp32, out with what its rounding left: a half step of out moves dS by as much as rounding dS does (dq of a
-// causal row of 600 keys, bf16, is off by 1.53 times its own rounding without the rest, 1.46 with it).  D / 8 lanes a row; rows behind the last
-// query of their unit get zeros.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant__ DenseArgs a, long long total) {
-    constexpr int kLanes = D / 8;
-    const int sub = threadIdx.x % kLanes;
-    const long long r = (long long)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;  // (b * Hq + h) * units * 64 + row of the unit
-    const int n_u = dense_units(a.Sq);
-    float s = 0.f;
-    const long long bh = r / ((long long)n_u * kBlk);
-    const int i = (int)(r % ((long long)n_u * kBlk)), b = (int)(bh / a.Hq), h = (int)(bh % a.Hq);
-    const bool there = r < total && i < a.Sq;
-    if (there) {
-        const uint4 o = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o.data) + b * a.o.sb + h * a.o.sh + i * a.o.ss + sub * 8);
-        const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout.data) + b * a.dout.sb + h * a.dout.sh + i * a.dout.ss + sub * 8);
-        uint4 left = make_uint4(0u, 0u, 0u, 0u);
-        if (a.rest != nullptr) left = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.rest) + (bh * a.Sq + i) * D + sub * 8);
-        const T *op = reinterpret_cast<const T*>(&o), *gp = reinterpret_cast<const T*>(&g), *lp = reinterpret_cast<const T*>(&left);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(DType<T>::to_f32(op[e]) + DType<T>::to_f32(lp[e]), DType<T>::to_f32(gp[e]), s);
-    }
-#pragma unroll
-    for (int x = kLanes / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    if (r < total && sub == 0) {
-        float* dst = a.stats + (r / kBlk) * (2 * kBlk) + r % kBlk;
-        dst[0] = there ? -(a.lse[bh * a.Sq + i] * kLog2e) : 0.f;
-        dst[kBlk] = there ? -s : 0.f;
-    }
 }
 
 // 64 columns of this thread's accumulator row -> 128 bytes of the row in global memory (input type)
@@ -356,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                         tma_load_5d_elect(dst + half * Ly::bHalf, tm, bar_full(slot), 64 * half, row, (fold & 1) ? 0 : head, (fold & 2) ? 0 : b, 0);
                     if (more) {
                         const uint32_t x = sbase + Ly::offExtra + slot * Ly::extra;
-                        bulk_load_elect(x, P.stats + (((long long)b * P.Hq + head) * P.n_u + unit) * (2 * kBlk), kStatsBytes, bar_full(slot));
+                        bulk_load_elect(x, P.stats + (((long long)b * P.Hq + head) * P.n_u + unit) * kDenseStats, kStatsBytes, bar_full(slot));
                         bulk_load_elect(x + kStatsBytes, P.seen + ((long long)b * P.n_u + unit) * kSeenPitch, kSeenBytes, bar_full(slot));
                     }
                     if (kMode == 1 && ++unit == it.first + it.span) {
@@ -566,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                 const int b = it.bh / P.heads, h = it.bh % P.heads, i = it.own * kM + row, u = i / kBlk;
                 if (u < P.n_u) {
                     r.see = P.seen[((long long)b * P.n_u + u) * kSeenPitch + i % kBlk];
-                    const float* st = P.stats + ((long long)it.bh * P.n_u + u) * (2 * kBlk) + i % kBlk;
+                    const float* st = P.stats + ((long long)it.bh * P.n_u + u) * kDenseStats + i % kBlk;
                     r.nl = st[0];
                     r.nd = st[kBlk];
                 }
@@ -789,17 +758,8 @@ cudaError_t pass_shape(const BwdParams& P, bool cap, cudaStream_t st) {
 
 template <bool kBf16, int D>
 cudaError_t passes(const DenseArgs& a, cudaStream_t st, const char** why) {
-    using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
     cudaError_t e = launch_dense_plan(a, st);
     if (e != cudaSuccess) return e;
-    const long long total = (long long)a.B * a.Hq * dense_units(a.Sq) * kBlk;
-    constexpr int kRowsPerCta = 256 / (D / 8);
-    if (total > 0) {
-        if ((total + kRowsPerCta - 1) / kRowsPerCta > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-        dense_stats_kernel<T, D><<<(unsigned)((total + kRowsPerCta - 1) / kRowsPerCta), 256, 0, st>>>(a, total);
-        e = cudaGetLastError();
-        if (e != cudaSuccess) return e;
-    }
     BwdParams P{};
     P.seen = a.seen; P.hulls = a.hulls; P.stats = a.stats; P.slopes = a.slopes; P.status = a.status;
     P.B = a.B; P.Hq = a.Hq; P.Hk = a.Hk; P.group = a.group; P.n_u = dense_units(a.Sq); P.n_k = dense_units(a.Sk);

@@ -15,6 +15,7 @@ namespace lcbsa {
 
 constexpr int kDenseCounters = 2;
 constexpr int kDenseUnit = 64;              // rows of a query unit, keys of a key unit
+constexpr int kDenseStats = 2 * kDenseUnit;  // floats of a query unit in the plan of the backward: -lse * log2(e) [64], -delta [64]
 constexpr int kSeenPitch = kDenseUnit + 1;  // int4 of a query unit in the plan
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 

@@ -2,18 +2,19 @@
 //
 // What every query sees, in the order of the queries; per unit of 64 queries the union of the runs of its rows (min lo, max hi) and the
 // run that all see (max lo, min hi); per unit of 64 keys the first and the last query that can see one of them, from the
-// documents at its two ends.  A warp takes a query unit, a thread of the CTAs behind them a key unit.
+// documents at its two ends.  A warp takes a query unit, a thread of the CTAs behind them a key unit.  The backward's row sums need none of it
+// and ride in the same launch.
 #include "dense_common.cuh"
 
 namespace lcbsa {
 
 namespace {
 
-__global__ void __launch_bounds__(128) dense_plan_kernel(const __grid_constant__ DenseArgs a, int q_ctas) {
-    if (a.next_item != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kDenseCounters) a.next_item[threadIdx.x] = 0;
-    const int b = blockIdx.y, lane = threadIdx.x & 31, n_u = dense_units(a.Sq), n_k = dense_units(a.Sk);
-    if ((int)blockIdx.x < q_ctas) {
-        const int u = blockIdx.x * 4 + (threadIdx.x >> 5);
+__device__ __forceinline__ void plan_cta(const DenseArgs& a, int cta, int b, int q_ctas) {
+    if (cta == 0 && b == 0 && threadIdx.x < kDenseCounters) a.next_item[threadIdx.x] = 0;
+    const int lane = threadIdx.x & 31, n_u = dense_units(a.Sq), n_k = dense_units(a.Sk);
+    if (cta < q_ctas) {
+        const int u = cta * 4 + (threadIdx.x >> 5);
         if (u >= n_u) return;
         int u_lo = 0x7fffffff, u_hi = 0, all_lo = 0, all_hi = 0x7fffffff;
 #pragma unroll
@@ -38,7 +39,7 @@ __global__ void __launch_bounds__(128) dense_plan_kernel(const __grid_constant__
         if (lane == 0) a.seen[((long long)b * n_u + u) * kSeenPitch + kDenseUnit] = make_int4(min(u_lo, u_hi), u_hi, all_lo, all_hi);
         return;
     }
-    const int u = (blockIdx.x - q_ctas) * 128 + threadIdx.x;
+    const int u = (cta - q_ctas) * 128 + threadIdx.x;
     if (u >= n_k) return;
     const DenseMask& m = a.mask;
     const int k_first = u * kDenseUnit, k_last = min(k_first + kDenseUnit, a.Sk) - 1;
@@ -69,6 +70,44 @@ __global__ void __launch_bounds__(128) dense_plan_kernel(const __grid_constant__
     a.hulls[(long long)b * n_k + u] = make_int2(q0, min(max(q_end, q0), a.Sq));
 }
 
+// Backward: rowsum(dout * out) in fp32, out with what its rounding left: a half step of out moves dS by as much as rounding dS does (dq
+// of a causal row of 600 keys, bf16, is off by 1.53 times its own rounding without the rest, 1.46 with it).  D / 8 lanes a row; rows
+// behind the last query of their unit get zeros.
+template <typename T, int D>
+__device__ __forceinline__ void stats_cta(const DenseArgs& a, long long cta) {
+    constexpr int kLanes = D / 8;
+    const int sub = threadIdx.x % kLanes;
+    const long long r = cta * (128 / kLanes) + threadIdx.x / kLanes;  // (b * Hq + h) * units * 64 + row of the unit: whole CTAs of them
+    const int n_u = dense_units(a.Sq);
+    float s = 0.f;
+    const long long bh = r / ((long long)n_u * kDenseUnit);
+    const int i = (int)(r % ((long long)n_u * kDenseUnit)), b = (int)(bh / a.Hq), h = (int)(bh % a.Hq);
+    if (i < a.Sq) {
+        const uint4 o = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o.data) + b * a.o.sb + h * a.o.sh + i * a.o.ss + sub * 8);
+        const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout.data) + b * a.dout.sb + h * a.dout.sh + i * a.dout.ss + sub * 8);
+        uint4 left = make_uint4(0u, 0u, 0u, 0u);
+        if (a.rest != nullptr) left = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.rest) + (bh * a.Sq + i) * D + sub * 8);
+        const T *op = reinterpret_cast<const T*>(&o), *gp = reinterpret_cast<const T*>(&g), *lp = reinterpret_cast<const T*>(&left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(DType<T>::to_f32(op[e]) + DType<T>::to_f32(lp[e]), DType<T>::to_f32(gp[e]), s);
+    }
+#pragma unroll
+    for (int x = kLanes / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    if (sub == 0) {
+        float* dst = a.stats + r / kDenseUnit * kDenseStats + r % kDenseUnit;
+        dst[0] = i < a.Sq ? -(a.lse[bh * a.Sq + i] * kLog2e) : 0.f;
+        dst[kDenseUnit] = i < a.Sq ? -s : 0.f;
+    }
+}
+
+// The plan's CTAs first (per batch entry q_ctas for the query units, then those of the key units), the backward's row sums behind them.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) dense_plan_kernel(const __grid_constant__ DenseArgs a, int q_ctas, int entry_ctas) {
+    const int planned = entry_ctas * a.B;
+    if ((int)blockIdx.x < planned) plan_cta(a, blockIdx.x % entry_ctas, blockIdx.x / entry_ctas, q_ctas);
+    else stats_cta<T, D>(a, (long long)blockIdx.x - planned);
+}
+
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
@@ -89,9 +128,18 @@ void dense_plan_carve(DenseArgs& a, void* workspace, bool backward) {
 }
 
 cudaError_t launch_dense_plan(const DenseArgs& a, cudaStream_t st) {
-    if (a.B > 65535) return cudaErrorInvalidConfiguration;
-    const int q_ctas = (dense_units(a.Sq) + 3) / 4, k_ctas = a.hulls != nullptr ? (dense_units(a.Sk) + 127) / 128 : 0;
-    if (q_ctas + k_ctas > 0) dense_plan_kernel<<<dim3(q_ctas + k_ctas, a.B), 128, 0, st>>>(a, q_ctas);
+    const int q_ctas = (dense_units(a.Sq) + 3) / 4, entry_ctas = q_ctas + (a.hulls != nullptr ? (dense_units(a.Sk) + 127) / 128 : 0);
+    const long long rows = a.hulls != nullptr ? (long long)a.B * a.Hq * dense_units(a.Sq) * kDenseUnit : 0;
+    const long long ctas = (long long)entry_ctas * a.B + rows * (a.D / 8) / 128;
+    if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    if (ctas == 0) return cudaSuccess;
+    if (a.dtype == LCBSA_BF16) {
+        if (a.D == 128) dense_plan_kernel<__nv_bfloat16, 128><<<(unsigned)ctas, 128, 0, st>>>(a, q_ctas, entry_ctas);
+        else dense_plan_kernel<__nv_bfloat16, 64><<<(unsigned)ctas, 128, 0, st>>>(a, q_ctas, entry_ctas);
+    } else {
+        if (a.D == 128) dense_plan_kernel<__half, 128><<<(unsigned)ctas, 128, 0, st>>>(a, q_ctas, entry_ctas);
+        else dense_plan_kernel<__half, 64><<<(unsigned)ctas, 128, 0, st>>>(a, q_ctas, entry_ctas);
+    }
     return cudaGetLastError();
 }
 

@@ -9,6 +9,7 @@ All arithmetic is in liblcbsa.so (``lcbsa_dense_attn_fwd`` / ``_bwd``); there is
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import struct
 from typing import NamedTuple, Optional, Tuple, Union
@@ -32,17 +33,23 @@ class _Shape(NamedTuple):
     k_lens: Optional[torch.Tensor]
     prefix: Optional[torch.Tensor]
 
-    def desc(self) -> L.LcbsaScores:
+    def packed(self) -> bytes:
         at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-        docs = 0 if self.cu_q is None else self.cu_q.shape[-1] - 1
-        cu_stride = docs + 1 if self.cu_q is not None and self.cu_q.dim() == 2 else 0
-        prefix_stride = self.prefix.shape[-1] if self.prefix is not None and self.prefix.dim() == 2 else 0
-        return L.LcbsaScores.from_buffer_copy(_PACK_SCORES(self.scale, self.cap, at(self.slopes), at(self.cu_q), at(self.cu_k), at(self.k_lens),
-                                                           at(self.prefix), cu_stride, prefix_stride, docs, int(self.causal)))
+        docs = cu_stride = prefix_stride = 0
+        if self.cu_q is not None:
+            docs = self.cu_q.shape[-1] - 1
+            cu_stride = docs + 1 if self.cu_q.dim() == 2 else 0
+        if self.prefix is not None and self.prefix.dim() == 2:
+            prefix_stride = self.prefix.shape[-1]
+        return _PACK_SCORES(self.scale, self.cap, at(self.slopes), at(self.cu_q), at(self.cu_k), at(self.k_lens), at(self.prefix), cu_stride,
+                            prefix_stride, docs, self.causal)
 
 
-def _as_abi(t: torch.Tensor) -> torch.Tensor:
-    return t if L.abi_ok(t) else t.contiguous()
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(B: int, Hq: int, Hk: int, Sq: int, Sk: int, D: int, backward: int) -> int:
+    """A pure function of the sizes, asked of the library once."""
+    sizes = [L.LcbsaTensor(None, L.LCBSA_BF16, 0, (ctypes.c_int64 * 4)(B, h, n, D)) for h, n in ((Hq, Sq), (Hk, Sk))]
+    return L.lib().lcbsa_dense_attn_workspace_bytes(ctypes.byref(sizes[0]), ctypes.byref(sizes[1]), backward)
 
 
 def _numbers(name: str, t: torch.Tensor, device, shapes) -> torch.Tensor:
@@ -95,50 +102,51 @@ def _shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, sc
     return _Shape(scale, softcap, bool(causal), slopes, cu_q, cu_k, k_lens, prefix_lens)
 
 
+_DENSE = torch.contiguous_format
+
+
 def _forward(q, k, v, shape: _Shape, need_lse: bool, need_rest: bool = False):
-    q, k, v = _as_abi(q), _as_abi(k), _as_abi(v)
     dev = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = torch.empty_like(q, memory_format=_DENSE)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if need_lse else None
-    rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_rest else None
-    lib, ref = L.lib(), ctypes.byref
-    qd, kd, vd, od, sd = L.tensor_desc(q), L.tensor_desc(k), L.tensor_desc(v), L.tensor_desc(out), shape.desc()
-    need = lib.lcbsa_dense_attn_workspace_bytes(ref(qd), ref(kd), 0)
+    rest = torch.empty_like(out) if need_rest else None
+    (q, qd), (k, kd), (v, vd), (_, od) = L.packed_rows(q), L.packed_rows(k), L.packed_rows(v), L.packed_rows(out)
+    B, Hq, Sq, D = q.shape
+    need = _workspace_bytes(B, Hq, k.shape[1], Sq, k.shape[2], D, 0)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     with L.on_device(dev):
-        L.check(lib.lcbsa_dense_attn_fwd(ref(qd), ref(kd), ref(vd), ref(sd), ref(od), None if lse is None else lse.data_ptr(),
-                                         None if rest is None else rest.data_ptr(), None if ws is None else ws.data_ptr(), need, L.current_stream(dev)))
+        L.check(L.lib().lcbsa_dense_attn_fwd(qd, kd, vd, shape.packed(), od, None if lse is None else lse.data_ptr(),
+                                             None if rest is None else rest.data_ptr(), None if ws is None else ws.data_ptr(), need,
+                                             L.current_stream(dev)))
     return out, lse, rest
 
 
 class _DenseAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, shape):
+    def forward(ctx, q, k, v, shape, return_lse):
         out, lse, rest = _forward(q, k, v, shape, True, True)
-        numbers = [t for t in shape if isinstance(t, torch.Tensor)]
-        ctx.save_for_backward(q, k, v, out, lse, rest, *numbers)
-        ctx.shape = shape._replace(**{n: None for n in shape._fields if isinstance(getattr(shape, n), torch.Tensor)})
-        ctx.names = [n for n in shape._fields if isinstance(getattr(shape, n), torch.Tensor)]
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.rest, ctx.shape = rest, shape
+        if not return_lse:
+            return out
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _):
-        q, k, v, out, lse, rest, *numbers = ctx.saved_tensors
-        shape = ctx.shape._replace(**dict(zip(ctx.names, numbers)))
-        q, k, v, out, dout = (_as_abi(t) if t.shape[2] <= 1 or t.stride(2) else t.contiguous() for t in (q, k, v, out, dout))
+    def backward(ctx, dout, *_):
+        q, k, v, out, lse = ctx.saved_tensors
         dev = q.device
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        lib, ref = L.lib(), ctypes.byref
-        qd, kd, vd, od, gd, dqd, dkd, dvd = map(L.tensor_desc, (q, k, v, out, dout, dq, dk, dv))
-        sd = shape.desc()
-        need = lib.lcbsa_dense_attn_workspace_bytes(ref(qd), ref(kd), 1)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        dq, dk, dv = (torch.empty_like(t, memory_format=_DENSE) for t in (q, k, v))
+        (q, qd), (k, kd), (v, vd), (out, od), (dout, gd) = map(L.packed_rows, (q, k, v, out, dout))
+        (_, dqd), (_, dkd), (_, dvd) = map(L.packed_rows, (dq, dk, dv))
+        B, Hq, Sq, D = q.shape
+        need = _workspace_bytes(B, Hq, k.shape[1], Sq, k.shape[2], D, 1)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         with L.on_device(dev):
-            L.check(lib.lcbsa_dense_attn_bwd(ref(qd), ref(kd), ref(vd), ref(od), ref(gd), ref(sd), lse.data_ptr(), rest.data_ptr(), ref(dqd), ref(dkd), ref(dvd),
-                                             ws.data_ptr(), need, L.current_stream(dev)))
-        return dq, dk, dv, None
+            L.check(L.lib().lcbsa_dense_attn_bwd(qd, kd, vd, od, gd, ctx.shape.packed(), lse.data_ptr(), ctx.rest.data_ptr(), dqd, dkd, dvd,
+                                                 ws.data_ptr(), need, L.current_stream(dev)))
+        return dq, dk, dv, None, None
 
 
 @torch.compiler.disable
@@ -168,7 +176,6 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
         raise ValueError(f"q, k, v are on {q.device}, {k.device}, {v.device}")
     shape = _shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _DenseAttention.apply(q, k, v, shape)
-    else:
-        out, lse, _ = _forward(q, k, v, shape, return_lse)
+        return _DenseAttention.apply(q, k, v, shape, return_lse)
+    out, lse, _ = _forward(q, k, v, shape, return_lse)
     return (out, lse) if return_lse else out

@@ -91,16 +91,11 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     return _frequencies(int(rotary_dim), float(base), tuple(sorted((scaling or {}).items())))
 
 
-def _as_abi(t: torch.Tensor) -> torch.Tensor:
-    return t if L.abi_ok(t) else t.contiguous()
-
-
 def _launch(xs, freqs: RotaryFrequencies, positions, offset: int, interleaved: bool, inverse: bool):
-    xs = [_as_abi(x) for x in xs]
     dev = xs[0].device
-    outs = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in xs]
-    n = len(xs)
-    xd, od = (L.LcbsaTensor * n)(*map(L.tensor_desc, xs)), (L.LcbsaTensor * n)(*map(L.tensor_desc, outs))
+    outs = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in xs]
+    packed = [L.packed_rows(x) for x in xs]  # the tensors stay alive with it
+    xd, od, n = b"".join(p[1] for p in packed), b"".join(L.packed_rows(x)[1] for x in outs), len(xs)
     ptr, bits, sb, ss = None, 32, 0, 0
     if positions is not None:
         ptr, bits = positions.data_ptr(), 64 if positions.dtype == torch.int64 else 32
