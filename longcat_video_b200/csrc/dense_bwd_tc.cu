@@ -48,31 +48,34 @@ template <int D> struct Lay {
     static constexpr int offB = offA + 2 * aTile;
     static constexpr int offExtra = offB + slots * 2 * bTile;
     static constexpr int offBar = offExtra + slots * extra;
-    // barriers: full[slots], empty[slots], s_full[2], s_free[2], x_full[2], ts_done[2], a_full, a_empty, at_full, at_free, acc_done,
+    // barriers: full[slots], empty[slots], s_full[2], s_free[2], x_full[3], ts_done[3], a_full, a_empty, at_full, at_free, acc_done,
     //           acc_free, item_full[kItemRing], item_empty[kItemRing]
-    static constexpr int numBars = 2 * slots + 8 + 6 + 2 * kItemRing;
+    static constexpr int numBars = 2 * slots + 10 + 6 + 2 * kItemRing;
     static constexpr int offMisc = (offBar + numBars * 8 + 15) / 16 * 16;  // abort flag, TMEM base
     static constexpr int offItems = offMisc + 64;
     static constexpr int smem = offItems + kItemRing * 32;
 };
 static_assert(Lay<128>::offExtra % 16 == 0 && Lay<128>::extra % 16 == 0 && Lay<128>::offBar % 8 == 0, "bulk copies and barriers are aligned");
 
-// TMEM columns.  dQ pass: dQ 0, S 128 and 192, dP 256 (one buffer), dS 320 and 352, Q 384, dO 448.  dK/dV pass: dK 0, dV 128, S^T 256,
-// dP^T 320, P^T 384, dS^T 416 (one buffer each), K 448; V stays in shared memory.
+// TMEM columns.  dP has one buffer, which is free once its entry's values are in registers.
+// dQ pass: dQ 0, S 128 and 192, dP 256, dS 320 and 352, Q 384, dO 448.
+// dK/dV pass: dK 0, dV 128, three buffers of S^T 256, 320, 384, dP^T 448; P^T and dS^T take the columns of the S^T they come from, 32 each.
+// K and V stay in shared memory: with K in TMEM there is room for two such buffers, and S^T of entry s + 2 then waits for the gradient MMAs
+// of entry s, a chain through everything (16 heads sharing 8, 8192 tokens: 556 us; with both warpgroups on one entry and single buffers 467 us).
 template <int kMode> struct Cols;
 template <> struct Cols<0> {
-    static constexpr uint32_t acc1 = 0, acc2 = 0, own1 = 384, own2 = 448;
-    static constexpr int bufs = 2;
+    static constexpr uint32_t acc1 = 0, acc2 = 0, own1 = 384, own2 = 448, dp = 256;
+    static constexpr unsigned bufs = 2;
     __device__ static __forceinline__ uint32_t s(int buf) { return 128u + 64u * buf; }
-    static constexpr uint32_t dp = 256, xp = 0;
+    __device__ static __forceinline__ uint32_t xp(int) { return 0u; }
     __device__ static __forceinline__ uint32_t xd(int buf) { return 320u + 32u * buf; }
 };
 template <> struct Cols<1> {
-    static constexpr uint32_t acc1 = 0, acc2 = 128, own1 = 448, own2 = 0;
-    static constexpr int bufs = 1;
-    __device__ static __forceinline__ uint32_t s(int) { return 256u; }
-    static constexpr uint32_t dp = 320, xp = 384;
-    __device__ static __forceinline__ uint32_t xd(int) { return 416u; }
+    static constexpr uint32_t acc1 = 0, acc2 = 128, own1 = 0, own2 = 0, dp = 448;
+    static constexpr unsigned bufs = 3;
+    __device__ static __forceinline__ uint32_t s(int buf) { return 256u + 64u * buf; }
+    __device__ static __forceinline__ uint32_t xp(int buf) { return s(buf); }
+    __device__ static __forceinline__ uint32_t xd(int buf) { return s(buf) + 32u; }
 };
 
 struct BwdParams {
@@ -88,6 +91,9 @@ struct BwdParams {
     long long o1_sb, o1_sh, o1_ss, o2_sb, o2_sh, o2_ss;
     int B, Hq, Hk, group, n_u, n_k;  // query units, key units of an entry
     int heads, n_own, rows;          // heads, own tiles of a head and rows of the own axis
+    // dK/dV pass: the query heads of a group are split over `splits` items of `walk` heads each, whose sums go to part [2][B * Hk * splits][Sk][D]
+    int splits, walk;
+    float* part;
     int n_items;
     float scale;
     ScoreShape shape;
@@ -133,22 +139,24 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
     using C = Cols<kMode>;
     using Ly = Lay<D>;
     using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
-    constexpr int kSlots = Ly::slots, kB = 2 * kSlots, kBufs = C::bufs, kHalves = D / 64;
+    constexpr int kSlots = Ly::slots, kB = 2 * kSlots, kHalves = D / 64;
+    constexpr unsigned kBufs = C::bufs;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t sbase = smem_u32(smem);
     const uint32_t bar0 = sbase + Ly::offBar;
-    // Entries are numbered over the whole kernel: entry s uses ring slot s % kSlots, S, P and dS of buffer s % kBufs.  Items with entries
+    // Entries are numbered over the whole kernel: entry s uses ring slot s % kSlots, S, P and dS of buffer s % kBufs, and is
+    // worked on by warpgroup s % 2.  Items with entries
     // are numbered too, for the barriers that turn once an item.
     auto bar_full = [&](int s) { return bar0 + 8u * s; };
     auto bar_empty = [&](int s) { return bar0 + 8u * (kSlots + s); };
     auto bar_s_full = [&](int buf) { return bar0 + 8u * (kB + buf); };
     auto bar_s_free = [&](int buf) { return bar0 + 8u * (kB + 2 + buf); };
     auto bar_x_full = [&](int buf) { return bar0 + 8u * (kB + 4 + buf); };
-    auto bar_ts_done = [&](int buf) { return bar0 + 8u * (kB + 6 + buf); };
-    const uint32_t bar_a_full = bar0 + 8u * (kB + 8), bar_a_empty = bar0 + 8u * (kB + 9), bar_at_full = bar0 + 8u * (kB + 10);
-    const uint32_t bar_at_free = bar0 + 8u * (kB + 11), bar_acc_done = bar0 + 8u * (kB + 12), bar_acc_free = bar0 + 8u * (kB + 13);
-    auto bar_item_full = [&](int k) { return bar0 + 8u * (kB + 14 + k); };
-    auto bar_item_empty = [&](int k) { return bar0 + 8u * (kB + 14 + kItemRing + k); };
+    auto bar_ts_done = [&](int buf) { return bar0 + 8u * (kB + 7 + buf); };
+    const uint32_t bar_a_full = bar0 + 8u * (kB + 10), bar_a_empty = bar0 + 8u * (kB + 11), bar_at_full = bar0 + 8u * (kB + 12);
+    const uint32_t bar_at_free = bar0 + 8u * (kB + 13), bar_acc_done = bar0 + 8u * (kB + 14), bar_acc_free = bar0 + 8u * (kB + 15);
+    auto bar_item_full = [&](int k) { return bar0 + 8u * (kB + 16 + k); };
+    auto bar_item_empty = [&](int k) { return bar0 + 8u * (kB + 16 + kItemRing + k); };
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Ly::offMisc);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::offMisc + 32);
     int4* items = reinterpret_cast<int4*>(smem + Ly::offItems);
@@ -164,12 +172,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
         }
         for (int buf = 0; buf < 2; ++buf) {
             mbar_init(bar_s_full(buf), 1);
-            mbar_init(bar_s_free(buf), kMode == 1 ? 8 : 4);  // one elected arrival per warp that works on an entry
-            mbar_init(bar_x_full(buf), kMode == 1 ? 8 : 4);
+            mbar_init(bar_s_free(buf), 4);  // one elected arrival per warp that works on an entry
+        }
+        for (int buf = 0; buf < 3; ++buf) {
+            mbar_init(bar_x_full(buf), 4);
             mbar_init(bar_ts_done(buf), 1);
         }
         mbar_init(bar_a_full, 1);
-        mbar_init(bar_a_empty, kMode == 1 ? 9 : 8);  // the arithmetic warps have moved it; dK/dV pass: and the last dP has read A2
+        mbar_init(bar_a_empty, kMode == 1 ? 1 : 8);  // the arithmetic warps have moved it; dK/dV pass: the last S and dP have read it
         mbar_init(bar_at_full, 8);
         mbar_init(bar_at_free, 1);
         mbar_init(bar_acc_done, 1);
@@ -263,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     if (x.x < x.y) {
                         it.first = x.x / kBlk;
                         it.span = (x.y - 1) / kBlk - it.first + 1;
-                        it.n = it.span * P.group;
+                        it.n = it.span * P.walk;
                     }
                 }
                 return it;
@@ -303,14 +313,15 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     mbar_arrive_tx_elect(bar_a_full, 2 * Ly::aTile);
 #pragma unroll
                     for (int half = 0; half < kHalves; ++half) {
+                        const int own_h = kMode == 0 ? h : h / P.splits;
                         tma_load_5d_elect(sbase + Ly::offA + half * Ly::aHalf, &P.tm_a1, bar_a_full, 64 * half, it.own * kM,
-                                          (P.fold_a1 & 1) ? 0 : h, (P.fold_a1 & 2) ? 0 : b, 0);
+                                          (P.fold_a1 & 1) ? 0 : own_h, (P.fold_a1 & 2) ? 0 : b, 0);
                         tma_load_5d_elect(sbase + Ly::offA + Ly::aTile + half * Ly::aHalf, &P.tm_a2, bar_a_full, 64 * half, it.own * kM,
-                                          (P.fold_a2 & 1) ? 0 : h, (P.fold_a2 & 2) ? 0 : b, 0);
+                                          (P.fold_a2 & 1) ? 0 : own_h, (P.fold_a2 & 2) ? 0 : b, 0);
                     }
                 }
                 ++kk;
-                int unit = it.first, head = kMode == 0 ? h / P.group : h * P.group;  // of the entry: dK/dV pass a query unit, dQ pass unused
+                int unit = it.first, head = kMode == 0 ? h / P.group : h * P.walk;  // of the entry: dK/dV pass a query unit, dQ pass unused
                 for (int e = 0; e < it.n; ++e) {
                     const int slot = s % kSlots;
                     ok = mbar_wait_warp(bar_empty(slot), ((s / kSlots) & 1) ^ 1, ctl, 210 + kMode, s);
@@ -348,22 +359,23 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
         } else if (warp == 9) {
             // ================================================================== issuer of S and dP (S^T and dP^T)
             const uint32_t idesc_ss = instr_desc(kBf16, kM, kBlk, 0);
-            const uint64_t a2d = smem_desc(sbase + Ly::offA + Ly::aTile, 16, 1024);  // dK/dV pass
+            const uint64_t a1d = smem_desc(sbase + Ly::offA, 16, 1024), a2d = smem_desc(sbase + Ly::offA + Ly::aTile, 16, 1024);  // dK/dV pass
             bool ok = true;
             unsigned s = 0, kk = 0;
             for (unsigned k = 0; ok; ++k) {
                 const Item it = take_item(k);
                 if (it.bh < 0) break;
                 if (it.n == 0) continue;
-                ok = mbar_wait_warp(bar_at_full, kk & 1, ctl, 220 + kMode, kk);  // the own tiles are in TMEM
+                if (kMode == 0) ok = mbar_wait_warp(bar_at_full, kk & 1, ctl, 220, kk);  // the own tiles are in TMEM
+                else ok = mbar_wait_warp(bar_a_full, kk & 1, ctl, 242, kk);
                 ++kk;
                 bool pre = false;
                 for (int e = 0; e < it.n && ok; ++e, ++s) {
                     const int slot = s % kSlots, buf = s % kBufs;
                     if (!pre) {  // not already seen ready by the look-ahead of the entry before
                         ok = mbar_wait_warp(bar_full(slot), (s / kSlots) & 1, ctl, 222 + kMode, s);
-                        // the arithmetic warps hold the last S and dP in registers (dQ pass: seen before the dP of entry s - 1)
-                        if (ok && kMode == 1) ok = mbar_wait_warp(bar_s_free(0), (s & 1) ^ 1, ctl, 226, s);
+                        // dK/dV pass: the gradient MMAs of entry s - 3 have read P and dS from S's columns
+                        if (ok && kMode == 1) ok = mbar_wait_warp(bar_ts_done(buf), ((s / kBufs) & 1) ^ 1, ctl, 226, s);
                         if (!ok) break;
                     }
                     tc_fence_after();
@@ -373,16 +385,18 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     for (int j = 0; j < D / 16; ++j) {
                         // 32 bytes per 16-column step inside a 64-column half; 8 TMEM columns per step
                         const uint64_t off = (uint64_t)(((j >> 2) * Ly::bHalf + (j & 3) * 32) >> 4);
-                        tc_mma_ts(tmem + C::s(buf), tmem + C::own1 + 8u * j, b1d + off, idesc_ss, j > 0);
+                        const uint64_t aoff = (uint64_t)(((j >> 2) * Ly::aHalf + (j & 3) * 32) >> 4);
+                        if (kMode == 1) tc_mma(tmem + C::s(buf), a1d + aoff, b1d + off, idesc_ss, j > 0);
+                        else tc_mma_ts(tmem + C::s(buf), tmem + C::own1 + 8u * j, b1d + off, idesc_ss, j > 0);
                     }
                     // look ahead: probe the next entry's barriers between the two contractions and read the answer after them
                     bool nf = false, ns = kMode == 0;
                     if (e + 1 < it.n) {
                         nf = mbar_test(bar_full((s + 1) % kSlots), ((s + 1) / kSlots) & 1);
-                        if (kMode == 1) ns = mbar_test(bar_s_free(0), ((s + 1) & 1) ^ 1);
+                        if (kMode == 1) ns = mbar_test(bar_ts_done((s + 1) % kBufs), (((s + 1) / kBufs) & 1) ^ 1);
                     }
                     tc_fence_after();
-                    if (kMode == 0 && s > 0) {  // dP of the entry before is in registers
+                    if (s > 0) {  // dP of the entry before is in registers
                         ok = mbar_wait_warp(bar_s_free((s - 1) & 1), ((s - 1) >> 1) & 1, ctl, 227, s);
                         if (!ok) break;
                         tc_fence_after();
@@ -394,11 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                         if (kMode == 1) tc_mma(tmem + C::dp, a2d + aoff, b2d + off, idesc_ss, j > 0);
                         else tc_mma_ts(tmem + C::dp, tmem + C::own2 + 8u * j, b2d + off, idesc_ss, j > 0);
                     }
-                    tc_commit(bar_s_full(buf));
-                    if (e == it.n - 1) {  // the own tiles have been read
-                        tc_commit(bar_at_free);
-                        if (kMode == 1) tc_commit(bar_a_empty);
-                    }
+                    tc_commit(bar_s_full(s & 1));
+                    if (e == it.n - 1) tc_commit(kMode == 1 ? bar_a_empty : bar_at_free);  // the own tiles have been read
                     __syncwarp();
                     pre = __all_sync(0xffffffffu, nf && ns);
                 }
@@ -456,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     if (kMode == 1) {
 #pragma unroll
                         for (int j = 0; j < kBlk / 16; ++j)  // dV += P^T dO
-                            tc_mma_ts(tmem + C::acc2, tmem + C::xp + 8u * j, b2m + (uint64_t)((j * 2048) >> 4), idesc_ts, (e > 0 || j > 0) ? 1u : 0u);
+                            tc_mma_ts(tmem + C::acc2, tmem + C::xp(buf) + 8u * j, b2m + (uint64_t)((j * 2048) >> 4), idesc_ts, (e > 0 || j > 0) ? 1u : 0u);
                     }
 #pragma unroll
                     for (int j = 0; j < kBlk / 16; ++j)  // dQ += dS K, or dK += dS^T Q
@@ -472,23 +483,22 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMath));
         // ================================================================== arithmetic warps
-        const int wg = warp >> 2;  // dQ pass: entries wg, wg + 2, ...; dK/dV pass: columns 32 wg .. 32 wg + 31 of every entry
+        const int wg = warp >> 2;  // entries of even or odd number
         const int wq = warp & 3;   // TMEM quadrant of this warp
         const int row = wq * 32 + lane;  // row of the own tile = TMEM lane
         const uint32_t t_lane = (uint32_t)(wq * 32) << 16;
         bool ok = start_ok;
         unsigned s0 = 0, kk = 0;  // entries before the current item, items with entries before it
-        // The own tiles go from shared memory to TMEM, where they are the A operands of every S and dP.  dQ pass: warpgroup g moves A1 (0) or
-        // A2 (1); dK/dV pass: half g of A1.
+        // dQ pass: the own tiles go from shared memory to TMEM, where they are the A operands of every S and dP.  Warpgroup g moves A1 (0) or
+        // A2 (1).
         auto own_to_tmem = [&](unsigned item) -> bool {
+            if (kMode == 1) return true;
             if (!mbar_wait_warp(bar_a_full, item & 1, ctl, 242, item)) return false;
             if (item > 0 && !mbar_wait_warp(bar_at_free, (item - 1) & 1, ctl, 243, item)) return false;
             tc_fence_after();
-            const int tile = kMode == 0 ? wg : 0;
 #pragma unroll
             for (int half = 0; half < kHalves; ++half) {
-                if (kMode == 1 && half != wg) continue;
-                const unsigned char* src = smem + Ly::offA + tile * Ly::aTile + half * Ly::aHalf + row * 128;
+                const unsigned char* src = smem + Ly::offA + wg * Ly::aTile + half * Ly::aHalf + row * 128;
                 uint32_t ar[32];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
@@ -498,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     ar[4 * c + 2] = v.z;
                     ar[4 * c + 3] = v.w;
                 }
-                tc_st32(tmem + (tile == 1 ? C::own2 : C::own1) + 32u * half + t_lane, ar);
+                tc_st32(tmem + (wg == 1 ? C::own2 : C::own1) + 32u * half + t_lane, ar);
             }
             tc_wait_st();
             tc_fence_before();
@@ -545,20 +555,40 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
         };
         auto entries = [&](const Item& it, const Row& me) {
             const unsigned n = it.n;
-            if constexpr (kMode == 0) {
-                for (unsigned i = s0 + ((s0 ^ wg) & 1); i < s0 + n && ok; i += 2) {  // buffer i & 1 = wg
-                    const unsigned r = i >> 1;
+            const int key = it.own * kM + row;                 // dK/dV pass
+            const int h0 = (it.bh % P.heads) * P.walk;
+            int unit = (int)((s0 ^ wg) & 1), head = 0;         // of the entry, relative to the item's first
+            float slope2 = me.slope2;
+            auto wrap = [&]() {
+                bool turned = false;
+                while (unit >= it.span && head < P.walk) {
+                    unit -= it.span;
+                    ++head;
+                    turned = true;
+                }
+                return turned;
+            };
+            if (kMode == 1) {
+                wrap();
+                if (kBias && head < P.walk) slope2 = __ldg(P.slopes + h0 + head) * kLog2e;
+            }
+            for (unsigned i = s0 + ((s0 ^ wg) & 1); i < s0 + n && ok; i += 2) {
+                const unsigned r = i >> 1;
+                const int slot = i % kSlots, buf = i % kBufs;
+                // dK/dV pass: what came with the slot's tiles
+                if (kMode == 1) ok = mbar_wait_warp(bar_full(slot), (i / kSlots) & 1, ctl, 234 + wg, i);
+                if (ok) ok = mbar_wait_warp(bar_s_full(wg), r & 1, ctl, 230 + wg, i);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t xp[32], xd[32], sr[64], dr[64];
+                tc_ld64(tmem + C::s(buf) + t_lane, sr);
+                tc_ld64(tmem + C::dp + t_lane, dr);
+                tc_wait_ld();
+                tc_fence_before();
+                mbar_arrive_elect(bar_s_free(wg));  // dP may be overwritten by that of entry i + 1
+                const bool large = kCap && any_large(sr, P.shape.inv);
+                if constexpr (kMode == 0) {
                     const int key0 = it.first + kBlk * (int)(i - s0);
-                    ok = mbar_wait_warp(bar_s_full(wg), r & 1, ctl, 230 + wg, i);
-                    if (!ok) break;
-                    tc_fence_after();
-                    uint32_t xd[32], sr[64], dr[64];
-                    tc_ld64(tmem + C::s(wg) + t_lane, sr);
-                    tc_ld64(tmem + C::dp + t_lane, dr);
-                    tc_wait_ld();
-                    tc_fence_before();
-                    mbar_arrive_elect(bar_s_free(wg));  // dP may be overwritten by that of entry i + 1, S by that of entry i + 2
-                    const bool large = kCap && any_large(sr, P.shape.inv);
                     const bool mixed = mixed_keys(it, (int)(i - s0));
                     const float at = (float)(me.see.z - key0);
                     const int lo = me.see.x - key0, hi = me.see.y - key0;
@@ -568,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                             float2 p, ds, far = make_float2(0.f, 0.f);
                             if (kBias) far = make_float2(fabsf(at - (float)(2 * k)), fabsf(at - (float)(2 * k + 1)));
                             pair(two(sr[2 * k], sr[2 * k + 1]), two(dr[2 * k], dr[2 * k + 1]), make_float2(me.nl, me.nl), make_float2(me.nd, me.nd), far,
-                                 me.slope2, lg, p, ds);
+                                 slope2, lg, p, ds);
                             if (mx) {
                                 if (2 * k < lo || 2 * k >= hi) ds.x = 0.f;
                                 if (2 * k + 1 < lo || 2 * k + 1 >= hi) ds.y = 0.f;
@@ -579,49 +609,27 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     if (kCap && LCBSA_UNLIKELY(large)) all(true, true);
                     else if (mixed) all(false, true);
                     else all(false, false);
-                    // TS of entry i - 2 has read the columns
+                    // the gradient MMAs of entry i - 2 have read the columns
                     ok = mbar_wait_warp(bar_ts_done(wg), (r & 1) ^ 1, ctl, 236 + wg, i);
                     if (!ok) break;
                     tc_fence_after();
-                    tc_st32(tmem + C::xd(wg) + t_lane, xd);
-                    tc_wait_st();
-                    tc_fence_before();
-                    mbar_arrive_elect(bar_x_full(wg));
-                }
-            } else {
-                const int key = it.own * kM + row;
-                const int h0 = (it.bh % P.heads) * P.group;
-                int unit = 0, head = 0;  // of the entry, relative to the item's first
-                float slope2 = kBias ? __ldg(P.slopes + h0) * kLog2e : 0.f;
-                for (unsigned i = s0; i < s0 + n && ok; ++i) {  // columns 32 wg .. 32 wg + 31 of every entry
-                    const int slot = i % kSlots;
-                    // what came with the slot's tiles
-                    ok = mbar_wait_warp(bar_full(slot), (i / kSlots) & 1, ctl, 234 + wg, i);
-                    if (ok) ok = mbar_wait_warp(bar_s_full(0), i & 1, ctl, 232 + wg, i);
-                    if (!ok) break;
-                    tc_fence_after();
-                    uint32_t sr[32], dr[32];
-                    tc_ld32(tmem + C::s(0) + 32u * wg + t_lane, sr);
-                    tc_ld32(tmem + C::dp + 32u * wg + t_lane, dr);
-                    tc_wait_ld();
-                    tc_fence_before();
-                    mbar_arrive_elect(bar_s_free(0));  // S^T and dP^T may be overwritten by the next entry's
-                    const float2* st2 = reinterpret_cast<const float2*>(smem + Ly::offExtra + slot * Ly::extra) + 16 * wg;
+                } else {
+                    const float4* const st4 = reinterpret_cast<const float4*>(smem + Ly::offExtra + slot * Ly::extra);
                     const int4* const see = seen_of_slot(slot);
-                    const bool large = kCap && any_large(sr, P.shape.inv);
                     const bool mixed = mixed_queries(it, see[kBlk]);
                     // the queries of a whole entry belong to one document, so their places follow one another
-                    const float at = kBias ? (float)(see[0].z + 32 * wg - key) : 0.f;
-                    uint32_t xp[16], xd[16];
+                    const float at = kBias ? (float)(see[0].z - key) : 0.f;
                     auto all = [&](bool lg, bool mx) {
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
+                        for (int k = 0; k < 32; ++k) {
+                            const float4 l4 = st4[k >> 1], d4 = st4[16 + (k >> 1)];
+                            const float2 nl = k & 1 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+                            const float2 nd = k & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
                             float2 p, ds, far = make_float2(0.f, 0.f);
-                            const float2 nl = st2[k], nd = st2[k + kBlk / 2];
                             int4 a = make_int4(0, 0, 0, 0), c = a;
                             if (mx) {
-                                a = see[32 * wg + 2 * k];
-                                c = see[32 * wg + 2 * k + 1];
+                                a = see[2 * k];
+                                c = see[2 * k + 1];
                             }
                             if (kBias) {
                                 far = make_float2(fabsf(at + (float)(2 * k)), fabsf(at + (float)(2 * k + 1)));
@@ -641,22 +649,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     if (kCap && LCBSA_UNLIKELY(large)) all(true, true);
                     else if (mixed) all(false, true);
                     else all(false, false);
-                    if (++unit == it.span) {
-                        unit = 0;
-                        ++head;
-                        if (kBias && head < P.group) slope2 = __ldg(P.slopes + h0 + head) * kLog2e;
-                    }
-                    // TS of entry i - 1 has read the columns
-                    ok = mbar_wait_warp(bar_ts_done(0), (i & 1) ^ 1, ctl, 238 + wg, i);
-                    if (!ok) break;
-                    tc_fence_after();
-                    // 32 columns of the tile are 16 columns of 16-bit pairs
-                    tc_st16(tmem + C::xp + 16u * wg + t_lane, xp);
-                    tc_st16(tmem + C::xd(0) + 16u * wg + t_lane, xd);
-                    tc_wait_st();
-                    tc_fence_before();
-                    mbar_arrive_elect(bar_x_full(0));
+                    unit += 2;
+                    if (wrap() && kBias && head < P.walk) slope2 = __ldg(P.slopes + h0 + head) * kLog2e;
+                    tc_st32(tmem + C::xp(buf) + t_lane, xp);  // S's columns: this warp has read its lanes of them
                 }
+                tc_st32(tmem + C::xd(buf) + t_lane, xd);
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive_elect(bar_x_full(buf));
             }
             s0 += n;
         };
@@ -689,7 +689,15 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
 #pragma unroll
                     for (int j = 0; j < 64; ++j) acc[j] = 0u;  // nobody sees these rows, or they see nothing
                 }
-                if (i < P.rows && half < kHalves) store_row64<kBf16>(row_ptr, 64 * half, acc);
+                if (i >= P.rows || half >= kHalves) continue;
+                if (kMode == 1 && P.splits > 1) {
+                    float4* dst = reinterpret_cast<float4*>(P.part + (((long long)(second ? P.B * P.heads : 0) + it.bh) * P.rows + i) * D + 64 * half);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        dst[j] = make_float4(__uint_as_float(acc[4 * j]), __uint_as_float(acc[4 * j + 1]), __uint_as_float(acc[4 * j + 2]), __uint_as_float(acc[4 * j + 3]));
+                } else {
+                    store_row64<kBf16>(row_ptr, 64 * half, acc);
+                }
             }
             return true;
         };
@@ -731,6 +739,41 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
+}
+
+// The split sums of dK and dV, added in order: a thread takes four values of a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) dense_join_kernel(const __grid_constant__ DenseArgs a, const float* part, int splits) {
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x, total = (long long)a.B * a.Hk * a.Sk * (D / 4);
+    if (at >= total) return;
+    const int c = (int)(at % (D / 4));
+    const long long r = at / (D / 4), bh = r / a.Sk;
+    const int i = (int)(r % a.Sk), b = (int)(bh / a.Hk), h = (int)(bh % a.Hk);
+    const long long all = (long long)a.B * a.Hk * splits * a.Sk * D;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int sp = 0; sp < splits; ++sp) {
+            const float4 v = *reinterpret_cast<const float4*>(part + t * all + ((bh * splits + sp) * a.Sk + i) * D + 4 * c);
+            s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+        }
+        const View& o = t ? a.dv : a.dk;
+        uint2 w;
+        w.x = pack2(DType<T>::code == LCBSA_BF16, s.x, s.y);
+        w.y = pack2(DType<T>::code == LCBSA_BF16, s.z, s.w);
+        *reinterpret_cast<uint2*>(static_cast<T*>(const_cast<void*>(o.data)) + b * o.sb + h * o.sh + i * o.ss + 4 * c) = w;
+    }
+}
+
+// Items of the dK/dV pass are few where many query heads share a key head, and as long as all of them together: where there are less than
+// four for an SM the heads are split.  (To be measured.)
+int dkdv_splits(const DenseArgs& a) {
+    const long long items = (long long)a.B * a.Hk * ((a.Sk + kM - 1) / kM);
+    int s = 1;
+    while (s < a.group && items * s < 148 * 4) {
+        do ++s; while (a.group % s != 0);
+    }
+    return s;
 }
 
 template <bool kBf16, int D, int kMode, bool kCap, bool kBias>
@@ -791,10 +834,20 @@ cudaError_t passes(const DenseArgs& a, cudaStream_t st, const char** why) {
         P.o1_sb = a.dk.sb; P.o1_sh = a.dk.sh; P.o1_ss = a.dk.ss;
         P.out2 = const_cast<void*>(a.dv.data);
         P.o2_sb = a.dv.sb; P.o2_sh = a.dv.sh; P.o2_ss = a.dv.ss;
-        P.heads = a.Hk; P.n_own = (a.Sk + kM - 1) / kM; P.rows = a.Sk;
-        P.n_items = a.B * a.Hk * P.n_own;
+        P.splits = dkdv_splits(a);
+        P.walk = a.group / P.splits;
+        P.part = a.part;
+        P.heads = a.Hk * P.splits; P.n_own = (a.Sk + kM - 1) / kM; P.rows = a.Sk;
+        P.n_items = a.B * P.heads * P.n_own;
         P.next_item = a.next_item + 1;
         e = pass_shape<kBf16, D, 1>(P, cap, st);
+        if (e == cudaSuccess && P.splits > 1) {
+            using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+            const long long ctas = ((long long)a.B * a.Hk * a.Sk * (D / 4) + 255) / 256;
+            if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+            dense_join_kernel<T, D><<<(unsigned)ctas, 256, 0, st>>>(a, a.part, P.splits);
+            e = cudaGetLastError();
+        }
     }
     return e;
 }
@@ -817,13 +870,16 @@ bool dense_bwd_supported(const DenseArgs& a, const char** why) {
 }
 
 size_t dense_bwd_workspace_bytes(const DenseArgs& a) {
-    return dense_plan_bytes(a, true) + (size_t)a.B * a.Hq * dense_units(a.Sq) * kStatsBytes;
+    const int splits = dkdv_splits(a);
+    return dense_plan_bytes(a, true) + (size_t)a.B * a.Hq * dense_units(a.Sq) * kStatsBytes +
+           (splits > 1 ? 2 * (size_t)a.B * a.Hk * splits * a.Sk * a.D * sizeof(float) : 0);
 }
 
 cudaError_t launch_dense_bwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why) {
     if (a.B * a.Hq == 0) return cudaSuccess;
     dense_plan_carve(a, workspace, true);
     a.stats = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + dense_plan_bytes(a, true));
+    a.part = a.stats + (size_t)a.B * a.Hq * dense_units(a.Sq) * kDenseStats;
     const cudaError_t e = a.dtype == LCBSA_BF16 ? (a.D == 128 ? passes<true, 128>(a, st, why) : passes<true, 64>(a, st, why))
                                                 : (a.D == 128 ? passes<false, 128>(a, st, why) : passes<false, 64>(a, st, why));
     if (e == cudaErrorInvalidConfiguration) *why = "more CTAs than a launch takes";
