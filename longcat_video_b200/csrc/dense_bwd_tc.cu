@@ -123,14 +123,16 @@ __device__ __forceinline__ void store_row64(unsigned char* row_ptr, int col0, co
     }
 }
 
-// whether one of the n scores is not small enough for the polynomial of the cap (or not a number)
-template <int n>
-__device__ __forceinline__ bool any_large(const uint32_t (&r)[n], float inv) {
-    uint32_t m[4] = {0u, 0u, 0u, 0u};  // magnitudes order like their bits, NaN above all
+// whether one of the scores is too large for the polynomial of the cap (a NaN is passed over: it stays one through it)
+__device__ __forceinline__ bool any_large(const uint32_t (&r)[64], float inv) {
+    float m[4];
 #pragma unroll
-    for (int j = 0; j < n; ++j) m[j & 3] = max(m[j & 3], r[j] & 0x7fffffffu);
-    const float top = __uint_as_float(max(max(m[0], m[1]), max(m[2], m[3])));
-    return __any_sync(0xffffffffu, !(fabsf(inv) * top <= kCapSmall));
+    for (int k = 0; k < 4; ++k) {
+        m[k] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) m[k] = max3(m[k], fabsf(__uint_as_float(r[16 * k + j])), fabsf(__uint_as_float(r[16 * k + j + 1])));
+    }
+    return __any_sync(0xffffffffu, !(fabsf(inv) * fmaxf(max3(m[0], m[1], m[2]), m[3]) <= kCapSmall));
 }
 
 // kMode 0: dQ pass, 1: dK/dV pass.  Persistent, one CTA per SM.

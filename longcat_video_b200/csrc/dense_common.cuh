@@ -126,17 +126,23 @@ __device__ __forceinline__ float2 capped_any(const ScoreShape& f, float2 s, floa
     slack = __fmul2_rn(t, __fadd2_rn(make_float2(2.f, 2.f), make_float2(-t.x, -t.y)));
     return __ffma2_rn(t, m, c);
 }
-__device__ __forceinline__ float2 capped_small(const ScoreShape& f, float2 s, float2& slack) {
+__device__ __forceinline__ float2 cap_poly(float2 z) {
     auto both = [](float x) { return make_float2(x, x); };
-    const float2 y = __fmul2_rn(s, both(f.inv)), z = __fmul2_rn(y, y);
     float2 p = __ffma2_rn(z, both(-0.004711522255092859f), both(0.019576216116547585f));
     p = __ffma2_rn(p, z, both(-0.05334111675620079f));
     p = __ffma2_rn(p, z, both(0.13325339555740356f));
     p = __ffma2_rn(p, z, both(-0.33332952857017517f));
-    p = __ffma2_rn(p, z, both(1.f));
-    const float2 t = __fmul2_rn(y, p);
-    slack = __ffma2_rn(t, make_float2(-t.x, -t.y), both(1.f));
-    return __fmul2_rn(__fmul2_rn(s, both(f.mul)), p);
+    return __ffma2_rn(p, z, both(1.f));
+}
+__device__ __forceinline__ float2 capped_small(const ScoreShape& f, float2 s, float2& slack) {
+    const float2 y = __fmul2_rn(s, make_float2(f.inv, f.inv)), p = cap_poly(__fmul2_rn(y, y)), t = __fmul2_rn(y, p);
+    slack = __ffma2_rn(t, make_float2(-t.x, -t.y), make_float2(1.f, 1.f));
+    return __fmul2_rn(__fmul2_rn(s, make_float2(f.mul, f.mul)), p);
+}
+// the same plus c
+__device__ __forceinline__ float2 capped_small_plus(const ScoreShape& f, float2 s, float2 c) {
+    const float2 y = __fmul2_rn(s, make_float2(f.inv, f.inv));
+    return __ffma2_rn(__fmul2_rn(s, make_float2(f.mul, f.mul)), cap_poly(__fmul2_rn(y, y)), c);
 }
 
 // Whether one of the eight 16-bit values of a 16-byte chunk is an infinity or a NaN (all exponent bits set).

@@ -89,12 +89,16 @@ __device__ __forceinline__ void put2(uint32_t (&r)[64], int j, float2 v) {
     r[j] = __float_as_uint(v.x);
     r[j + 1] = __float_as_uint(v.y);
 }
-// the largest magnitude of a row of scores, NaN if there is one
+// the largest magnitude of a row of scores (a NaN is passed over: it stays one through the polynomial of the cap)
 __device__ __forceinline__ float row_size(const uint32_t (&r)[64]) {
-    uint32_t m[4] = {0u, 0u, 0u, 0u};  // magnitudes order like their bits, NaN above all
+    float m[4];
 #pragma unroll
-    for (int j = 0; j < 64; ++j) m[j & 3] = max(m[j & 3], r[j] & 0x7fffffffu);
-    return __uint_as_float(max(max(m[0], m[1]), max(m[2], m[3])));
+    for (int k = 0; k < 4; ++k) {
+        m[k] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) m[k] = max3(m[k], fabsf(__uint_as_float(r[16 * k + j])), fabsf(__uint_as_float(r[16 * k + j + 1])));
+    }
+    return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
 
 template <bool kBf16, int D, bool kCap, bool kBias>
@@ -600,9 +604,6 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
         const uint32_t t_lane = (uint32_t)(wq * 32) << 16;
         const uint32_t tm_s = tmem + kTmS + 64u * wg + t_lane, tm_p = tmem + kTmP + 32u * wg + t_lane;
         const uint32_t tm_o_mine = tmem + kTmO + 128u * wg + t_lane;
-        // Scores that are neither capped nor biased are scaled where they are exponentiated; the others are shaped first.
-        constexpr bool kShaped = kCap || kBias;
-        const float mul = kShaped ? 1.f : P.shape.mul;
         unsigned rr = 0;  // rounds of this warpgroup over the whole kernel
         bool ok = true;
         Item cur;
@@ -633,43 +634,83 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                 uint4 pk[8];  // this row of P in the input type, 8 keys per 16-byte chunk
                 if (active) {
                     const int key0 = cur.key0 + kBlk * i;
-                    if (kCap) {
-                        float2 slack;
-                        if (__any_sync(0xffffffffu, !(fabsf(f.inv) * row_size(sr) <= kCapSmall))) {  // a NaN too
-#pragma unroll
-                            for (int j = 0; j < 64; j += 2) put2(sr, j, capped_any(f, get2(sr, j), slack));
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 64; j += 2) put2(sr, j, capped_small(f, get2(sr, j), slack));
-                        }
+                    // S -> exponents relative to the reference, in place (0 stands in for it until the row has seen a key)
+                    const float m_eff = first ? 0.f : m_ref;
+                    float2 step = make_float2(0.f, 0.f), base = make_float2(-m_eff, -m_eff);
+                    bool both_sides = false;
+                    const float at = kBias ? (float)(see.z - key0) : 0.f;
+                    if (kBias) {  // keys on one side of the query: the distance is a line in the key's number
+                        const float sl = at >= (float)(kBlk - 1) ? f.slope2 : -f.slope2;
+                        both_sides = __any_sync(0xffffffffu, at > 0.f && at < (float)(kBlk - 1));
+                        step = make_float2(sl, sl);
+                        if (!both_sides) base.x = base.y = fmaf(-sl, at, -m_eff);
                     }
-                    if (kBias) {
-                        const float at = (float)(see.z - key0);
+                    auto exponents = [&](auto capped, bool two_sides) {
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) {
-                            const float x = kCap ? __uint_as_float(sr[j]) : __uint_as_float(sr[j]) * f.mul;
-                            sr[j] = __float_as_uint(fmaf(-f.slope2, fabsf(at - (float)j), x));
+                        for (int j = 0; j < 64; j += 2) {
+                            float2 c = base;
+                            if (kBias) {
+                                if (two_sides) c = __ffma2_rn(make_float2(fabsf(at - (float)j), fabsf(at - (float)(j + 1))), make_float2(-f.slope2, -f.slope2), base);
+                                else c = __ffma2_rn(make_float2((float)j, (float)(j + 1)), step, base);
+                            }
+                            put2(sr, j, capped(get2(sr, j), c));
                         }
+                    };
+                    if constexpr (kCap) {
+                        const bool large = __any_sync(0xffffffffu, !(fabsf(f.inv) * row_size(sr) <= kCapSmall));
+                        auto any = [&](float2 s, float2 c) { float2 slack; return __fadd2_rn(capped_any(f, s, slack), c); };
+                        auto small = [&](float2 s, float2 c) { return capped_small_plus(f, s, c); };
+                        if (LCBSA_UNLIKELY(large)) exponents(any, true);
+                        else if (kBias && both_sides) exponents(small, true);
+                        else exponents(small, false);
+                    } else {
+                        auto plain = [&](float2 s, float2 c) { return __ffma2_rn(s, make_float2(f.mul, f.mul), c); };
+                        if (kBias && both_sides) exponents(plain, true);
+                        else exponents(plain, false);
                     }
                     if (mixed_unit(cur, i)) {
-                        const int lo = see.x - key0, hi = see.y - key0;
+                        const int lo = min(max(see.x - key0, 0), kBlk), hi = min(max(see.y - key0, 0), kBlk);  // a run of bits
+                        const uint64_t sees = hi > lo ? (~0ull >> (kBlk - (hi - lo))) << lo : 0ull;
+                        const uint32_t s_lo = (uint32_t)sees, s_hi = (uint32_t)(sees >> 32);
 #pragma unroll
-                        for (int j = 0; j < 64; ++j)
-                            if (j < lo || j >= hi) sr[j] = 0xff800000u;  // -inf
+                        for (int j = 0; j < 32; ++j) {
+                            if (!((s_lo >> j) & 1u)) sr[j] = 0xff800000u;  // -inf
+                            if (!((s_hi >> j) & 1u)) sr[32 + j] = 0xff800000u;
+                        }
                     }
-                    // One pass: the probabilities are computed against the current reference maximum while the row maximum is
-                    // tracked beside them; only if the maximum has moved by more than 2^8 is the pass repeated with the new
-                    // reference.  The first unit in which the row sees a key takes its own maximum as the reference.
-                    auto probs = [&](float mref, float& rsum) {
-                        const float2 sc2 = make_float2(mul, mul), nm2 = make_float2(-mref, -mref);
+                    auto row_max = [&]() {
+                        float mx8[8];  // eight chains of eight values, three at a time
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            auto sv = [&](int i) { return __uint_as_float(sr[8 * i + k]); };
+                            mx8[k] = fmaxf(max3(max3(max3(sv(0), sv(1), sv(2)), sv(3), sv(4)), sv(5), sv(6)), sv(7));
+                        }
+                        return fmaxf(max3(max3(mx8[0], mx8[1], mx8[2]), mx8[3], mx8[4]), max3(mx8[5], mx8[6], mx8[7]));
+                    };
+                    auto shift = [&](float by) {
+                        const float2 b2 = make_float2(-by, -by);
+#pragma unroll
+                        for (int j = 0; j < 64; j += 2) put2(sr, j, __fadd2_rn(get2(sr, j), b2));
+                    };
+                    // The first unit in which the row sees a key takes its own maximum as the reference.
+                    if (LCBSA_UNLIKELY(first)) {
+                        const float m = row_max();
+                        if (m != -INFINITY) {
+                            m_ref = m;
+                            first = false;
+                            shift(m);
+                        }
+                    }
+                    // The probabilities are computed against the current reference while the row maximum is tracked beside them;
+                    // only if it has moved by more than 2^8 is the pass repeated with the new reference.
+                    auto probs = [&](float& rsum) {
                         float2 r01 = make_float2(0.f, 0.f), r23 = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int cch = 0; cch < 8; ++cch) {
                             float2 e[4];
 #pragma unroll
                             for (int jp = 0; jp < 4; ++jp) {
-                                const float2 s2 = make_float2(__uint_as_float(sr[cch * 8 + 2 * jp]), __uint_as_float(sr[cch * 8 + 2 * jp + 1]));
-                                const float2 x = kShaped ? __fadd2_rn(s2, nm2) : __ffma2_rn(s2, sc2, nm2);
+                                const float2 x = get2(sr, cch * 8 + 2 * jp);
                                 e[jp] = make_float2(ex2(x.x), ex2(x.y));
                             }
                             r01 = __fadd2_rn(r01, e[0]);
@@ -683,30 +724,15 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                         }
                         rsum = (r01.x + r01.y) + (r23.x + r23.y);
                     };
-                    // the row maximum of this unit, in units of log2
-                    auto row_max = [&]() {
-                        float mx8[8];  // eight chains of eight values, three at a time
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            auto sv = [&](int i) { return __uint_as_float(sr[8 * i + k]); };
-                            mx8[k] = fmaxf(max3(max3(max3(sv(0), sv(1), sv(2)), sv(3), sv(4)), sv(5), sv(6)), sv(7));
-                        }
-                        return fmaxf(max3(max3(mx8[0], mx8[1], mx8[2]), mx8[3], mx8[4]), max3(mx8[5], mx8[6], mx8[7])) * mul;
-                    };
                     float rs = 0.f;
-                    float m_new = m_ref;
-                    if (LCBSA_UNLIKELY(first)) {
-                        m_new = row_max();
-                        m_ref = (m_new == -INFINITY) ? 0.f : m_new;
-                    }
-                    first = first && m_new == -INFINITY;  // a unit of which the row sees nothing leaves no reference behind
-                    probs(m_ref, rs);
+                    probs(rs);
                     const float m_top = row_max();
-                    if (LCBSA_UNLIKELY(m_top - m_ref > 8.f)) {
+                    if (LCBSA_UNLIKELY(m_top > 8.f)) {
                         need = true;
-                        alpha = ex2(m_ref - m_top);
-                        m_ref = m_top;
-                        probs(m_ref, rs);
+                        alpha = ex2(-m_top);
+                        m_ref += m_top;
+                        shift(m_top);
+                        probs(rs);
                     }
                     l_sum = l_sum * alpha + rs;  // alpha is 1 unless this row's reference maximum moved
                 }
