@@ -20,6 +20,7 @@
 // that is seen has its NaN from S and dP; for dV it is the query's delta that says that dO is not finite.
 //
 // Every mbarrier wait is bounded; when one runs out the CTA flags the status word, drains its copies, frees TMEM, returns.
+#include <cmath>
 #include <type_traits>
 
 #include "dense_common.cuh"
@@ -35,8 +36,9 @@ constexpr int kM = 128;                     // rows of an own tile
 constexpr int kBlk = kDenseUnit;            // rows of a streamed tile
 constexpr int kStatsBytes = kDenseStats * 4;  // of a query unit
 constexpr int kSeenBytes = kSeenPitch * 16; // what its rows see
-constexpr int kThreads = 384;
-constexpr int kRegsMath = 200, kRegsOther = 104;  // setmaxnreg: (200 + 200 + 104) * 128 = the 63 K registers of the launch
+constexpr int kMathWarps = 16;
+constexpr int kThreads = 32 * (kMathWarps + 4);
+constexpr int kRegsMath = 104, kRegsOther = 64;  // setmaxnreg: (4 * 104 + 64) * 128 = the 60 K registers of the launch
 constexpr int kItemRing = 4;
 
 template <int D> struct Lay {
@@ -48,35 +50,32 @@ template <int D> struct Lay {
     static constexpr int offB = offA + 2 * aTile;
     static constexpr int offExtra = offB + slots * 2 * bTile;
     static constexpr int offBar = offExtra + slots * extra;
-    // barriers: full[slots], empty[slots], s_full[2], s_free[2], x_full[3], ts_done[3], a_full, a_empty, at_full, at_free, acc_done,
-    //           acc_free, item_full[kItemRing], item_empty[kItemRing]
-    static constexpr int numBars = 2 * slots + 10 + 6 + 2 * kItemRing;
+    // barriers: full[slots], empty[slots], s_full[2], s_free[2], d_full[2], p_full[2], x_full[2], ts_done[2], a_full, a_empty, at_full,
+    //           at_free, acc_done, acc_free, item_full[kItemRing], item_empty[kItemRing]
+    static constexpr int numBars = 2 * slots + 12 + 6 + 2 * kItemRing;
     static constexpr int offMisc = (offBar + numBars * 8 + 15) / 16 * 16;  // abort flag, TMEM base
     static constexpr int offItems = offMisc + 64;
     static constexpr int smem = offItems + kItemRing * 32;
 };
 static_assert(Lay<128>::offExtra % 16 == 0 && Lay<128>::extra % 16 == 0 && Lay<128>::offBar % 8 == 0, "bulk copies and barriers are aligned");
 
-// TMEM columns.  dP has one buffer, which is free once its entry's values are in registers.
-// dQ pass: dQ 0, S 128 and 192, dP 256, dS 320 and 352, Q 384, dO 448.
-// dK/dV pass: dK 0, dV 128, three buffers of S^T 256, 320, 384, dP^T 448; P^T and dS^T take the columns of the S^T they come from, 32 each.
-// K and V stay in shared memory: with K in TMEM there is room for two such buffers, and S^T of entry s + 2 then waits for the gradient MMAs
-// of entry s, a chain through everything (16 heads sharing 8, 8192 tokens: 556 us; with both warpgroups on one entry and single buffers 467 us).
+// TMEM columns: two buffers of S and of dP.  P takes the columns of the S it comes from (dK/dV pass) and dS those of its dP, in two pieces of
+// 16: the columns 32 h .. 32 h + 31 belong to the warps that work on half h, which have read them.
+// dQ pass: dQ 0, S 128 and 192, dP 256 and 320, Q 384, dO 448.  dK/dV pass: dK 0, dV 128, S^T 256 and 320, dP^T 384 and 448; K and V stay in
+// shared memory.
 template <int kMode> struct Cols;
 template <> struct Cols<0> {
-    static constexpr uint32_t acc1 = 0, acc2 = 0, own1 = 384, own2 = 448, dp = 256;
-    static constexpr unsigned bufs = 2;
+    static constexpr uint32_t acc1 = 0, acc2 = 0, own1 = 384, own2 = 448;
     __device__ static __forceinline__ uint32_t s(int buf) { return 128u + 64u * buf; }
-    __device__ static __forceinline__ uint32_t xp(int) { return 0u; }
-    __device__ static __forceinline__ uint32_t xd(int buf) { return 320u + 32u * buf; }
+    __device__ static __forceinline__ uint32_t dp(int buf) { return 256u + 64u * buf; }
 };
 template <> struct Cols<1> {
-    static constexpr uint32_t acc1 = 0, acc2 = 128, own1 = 0, own2 = 0, dp = 448;
-    static constexpr unsigned bufs = 3;
+    static constexpr uint32_t acc1 = 0, acc2 = 128, own1 = 0, own2 = 0;
     __device__ static __forceinline__ uint32_t s(int buf) { return 256u + 64u * buf; }
-    __device__ static __forceinline__ uint32_t xp(int buf) { return s(buf); }
-    __device__ static __forceinline__ uint32_t xd(int buf) { return s(buf) + 32u; }
+    __device__ static __forceinline__ uint32_t dp(int buf) { return 384u + 64u * buf; }
 };
+// 16-row step j of P or dS, relative to the columns of its S or dP
+__device__ __forceinline__ uint32_t piece(int j) { return 32u * (j >> 1) + 8u * (j & 1); }
 
 struct BwdParams {
     CUtensorMap tm_a1, tm_a2, tm_b1, tm_b2;
@@ -95,7 +94,8 @@ struct BwdParams {
     int splits, walk;
     float* part;
     int n_items;
-    float scale;
+    float scale, scale_lg;  // log2 of its magnitude
+    float sign;             // of the scale (dQ pass)
     ScoreShape shape;
 };
 
@@ -109,11 +109,11 @@ __device__ __forceinline__ void bulk_load_elect(uint32_t dst, const void* src, u
         : "memory");
 }
 
-// 64 columns of this thread's accumulator row -> 128 bytes of the row in global memory (input type)
+// 32 columns of this thread's accumulator row -> 64 bytes of the row in global memory (input type)
 template <bool kBf16>
-__device__ __forceinline__ void store_row64(unsigned char* row_ptr, int col0, const uint32_t (&r)[64]) {
+__device__ __forceinline__ void store_row32(unsigned char* row_ptr, int col0, const uint32_t (&r)[32]) {
 #pragma unroll
-    for (int q8 = 0; q8 < 8; ++q8) {
+    for (int q8 = 0; q8 < 4; ++q8) {
         uint4 pk;
         pk.x = pack2(kBf16, __uint_as_float(r[q8 * 8 + 0]), __uint_as_float(r[q8 * 8 + 1]));
         pk.y = pack2(kBf16, __uint_as_float(r[q8 * 8 + 2]), __uint_as_float(r[q8 * 8 + 3]));
@@ -124,13 +124,13 @@ __device__ __forceinline__ void store_row64(unsigned char* row_ptr, int col0, co
 }
 
 // whether one of the scores is too large for the polynomial of the cap (a NaN is passed over: it stays one through it)
-__device__ __forceinline__ bool any_large(const uint32_t (&r)[64], float inv) {
+__device__ __forceinline__ bool any_large(const uint32_t (&r)[32], float inv) {
     float m[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         m[k] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) m[k] = max3(m[k], fabsf(__uint_as_float(r[16 * k + j])), fabsf(__uint_as_float(r[16 * k + j + 1])));
+        for (int j = 0; j < 8; j += 2) m[k] = max3(m[k], fabsf(__uint_as_float(r[8 * k + j])), fabsf(__uint_as_float(r[8 * k + j + 1])));
     }
     return __any_sync(0xffffffffu, !(fabsf(inv) * fmaxf(max3(m[0], m[1], m[2]), m[3]) <= kCapSmall));
 }
@@ -142,23 +142,24 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
     using Ly = Lay<D>;
     using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
     constexpr int kSlots = Ly::slots, kB = 2 * kSlots, kHalves = D / 64;
-    constexpr unsigned kBufs = C::bufs;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t sbase = smem_u32(smem);
     const uint32_t bar0 = sbase + Ly::offBar;
-    // Entries are numbered over the whole kernel: entry s uses ring slot s % kSlots, S, P and dS of buffer s % kBufs, and is
-    // worked on by warpgroup s % 2.  Items with entries
+    // Entries are numbered over the whole kernel: entry s uses ring slot s % kSlots, buffer s % 2 of S and dP, and is
+    // worked on by the warpgroups 2 (s % 2) and 2 (s % 2) + 1, half of its columns each.  Items with entries
     // are numbered too, for the barriers that turn once an item.
     auto bar_full = [&](int s) { return bar0 + 8u * s; };
     auto bar_empty = [&](int s) { return bar0 + 8u * (kSlots + s); };
     auto bar_s_full = [&](int buf) { return bar0 + 8u * (kB + buf); };
-    auto bar_s_free = [&](int buf) { return bar0 + 8u * (kB + 2 + buf); };
-    auto bar_x_full = [&](int buf) { return bar0 + 8u * (kB + 4 + buf); };
-    auto bar_ts_done = [&](int buf) { return bar0 + 8u * (kB + 7 + buf); };
-    const uint32_t bar_a_full = bar0 + 8u * (kB + 10), bar_a_empty = bar0 + 8u * (kB + 11), bar_at_full = bar0 + 8u * (kB + 12);
-    const uint32_t bar_at_free = bar0 + 8u * (kB + 13), bar_acc_done = bar0 + 8u * (kB + 14), bar_acc_free = bar0 + 8u * (kB + 15);
-    auto bar_item_full = [&](int k) { return bar0 + 8u * (kB + 16 + k); };
-    auto bar_item_empty = [&](int k) { return bar0 + 8u * (kB + 16 + kItemRing + k); };
+    auto bar_s_free = [&](int buf) { return bar0 + 8u * (kB + 2 + buf); };  // dQ pass: S is in registers; dK/dV pass: P has been read
+    auto bar_d_full = [&](int buf) { return bar0 + 8u * (kB + 4 + buf); };
+    auto bar_p_full = [&](int buf) { return bar0 + 8u * (kB + 6 + buf); };
+    auto bar_x_full = [&](int buf) { return bar0 + 8u * (kB + 8 + buf); };
+    auto bar_ts_done = [&](int buf) { return bar0 + 8u * (kB + 10 + buf); };
+    const uint32_t bar_a_full = bar0 + 8u * (kB + 12), bar_a_empty = bar0 + 8u * (kB + 13), bar_at_full = bar0 + 8u * (kB + 14);
+    const uint32_t bar_at_free = bar0 + 8u * (kB + 15), bar_acc_done = bar0 + 8u * (kB + 16), bar_acc_free = bar0 + 8u * (kB + 17);
+    auto bar_item_full = [&](int k) { return bar0 + 8u * (kB + 18 + k); };
+    auto bar_item_empty = [&](int k) { return bar0 + 8u * (kB + 18 + kItemRing + k); };
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Ly::offMisc);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::offMisc + 32);
     int4* items = reinterpret_cast<int4*>(smem + Ly::offItems);
@@ -174,21 +175,21 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
         }
         for (int buf = 0; buf < 2; ++buf) {
             mbar_init(bar_s_full(buf), 1);
-            mbar_init(bar_s_free(buf), 4);  // one elected arrival per warp that works on an entry
-        }
-        for (int buf = 0; buf < 3; ++buf) {
-            mbar_init(bar_x_full(buf), 4);
+            mbar_init(bar_s_free(buf), kMode == 1 ? 1 : 8);  // one elected arrival per warp that works on an entry
+            mbar_init(bar_d_full(buf), 1);
+            mbar_init(bar_p_full(buf), 8);
+            mbar_init(bar_x_full(buf), 8);
             mbar_init(bar_ts_done(buf), 1);
         }
         mbar_init(bar_a_full, 1);
-        mbar_init(bar_a_empty, kMode == 1 ? 1 : 8);  // the arithmetic warps have moved it; dK/dV pass: the last S and dP have read it
-        mbar_init(bar_at_full, 8);
+        mbar_init(bar_a_empty, kMode == 1 ? 1 : kMathWarps);  // the arithmetic warps have moved it; dK/dV pass: the last S and dP have read it
+        mbar_init(bar_at_full, kMathWarps);
         mbar_init(bar_at_free, 1);
         mbar_init(bar_acc_done, 1);
-        mbar_init(bar_acc_free, 8);
+        mbar_init(bar_acc_free, kMathWarps);
         for (int k = 0; k < kItemRing; ++k) {
             mbar_init(bar_item_full(k), 1);
-            mbar_init(bar_item_empty(k), 11);  // every warp but the one that announces
+            mbar_init(bar_item_empty(k), kMathWarps + 3);  // every warp but the one that announces
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (sbase & 1023u) {  // the swizzled tiles need the base that the declaration asks for
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
             }
         }
     }
-    if (warp == 9) {  // TMEM: all 512 columns, allocated and freed by the issuing warp
+    if (warp == kMathWarps + 1) {  // TMEM: all 512 columns, allocated and freed by the issuing warp
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
     struct Item {
         int bh, own, first, n, all_lo, all_hi, span;
     };
-    auto take_item = [&](unsigned k) {  // item number k of this CTA, for every warp but warp 8
+    auto take_item = [&](unsigned k) {  // item number k of this CTA, for every warp but the one that announces
         Item it{-1, 0, 0, 0, 0, 0, 0};
         if (!mbar_wait_warp(bar_item_full(k % kItemRing), (k / kItemRing) & 1, ctl, 200, k)) return it;
         const int4 a = items[2 * (k % kItemRing)], c = items[2 * (k % kItemRing) + 1];
@@ -234,12 +235,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
     };
     auto seen_of_slot = [&](int slot) { return reinterpret_cast<const int4*>(smem + Ly::offExtra + slot * Ly::extra + kStatsBytes); };
 
-    if (warp >= 8) {
+    if (warp >= kMathWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
         if (!start_ok) {
-        } else if (warp == 8 || warp == 11) {
-            // ================================================================== TMA producers: warp 8 items, own tiles, B1 and what comes with it, warp 11 B2
-            const bool is_b1 = warp == 8;
+        } else if (warp == kMathWarps || warp == kMathWarps + 3) {
+            // ================================================================== TMA producers: one for items, own tiles, B1 and what comes with it, one for B2
+            const bool is_b1 = warp == kMathWarps;
             const CUtensorMap* tm = is_b1 ? &P.tm_b1 : &P.tm_b2;
             const int fold = is_b1 ? P.fold_b1 : P.fold_b2;
             bool ok = true;
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     while (!mbar_try(bar_full(r % kSlots), (r / kSlots) & 1) && clock64() - t0 < 40000000ll) {
                     }
             }
-        } else if (warp == 9) {
+        } else if (warp == kMathWarps + 1) {
             // ================================================================== issuer of S and dP (S^T and dP^T)
             const uint32_t idesc_ss = instr_desc(kBf16, kM, kBlk, 0);
             const uint64_t a1d = smem_desc(sbase + Ly::offA, 16, 1024), a2d = smem_desc(sbase + Ly::offA + Ly::aTile, 16, 1024);  // dK/dV pass
@@ -373,11 +374,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                 ++kk;
                 bool pre = false;
                 for (int e = 0; e < it.n && ok; ++e, ++s) {
-                    const int slot = s % kSlots, buf = s % kBufs;
+                    const int slot = s % kSlots, buf = s & 1;
+                    const uint32_t before = ((s >> 1) & 1) ^ 1;  // parity of the buffer's use before
                     if (!pre) {  // not already seen ready by the look-ahead of the entry before
                         ok = mbar_wait_warp(bar_full(slot), (s / kSlots) & 1, ctl, 222 + kMode, s);
-                        // dK/dV pass: the gradient MMAs of entry s - 3 have read P and dS from S's columns
-                        if (ok && kMode == 1) ok = mbar_wait_warp(bar_ts_done(buf), ((s / kBufs) & 1) ^ 1, ctl, 226, s);
+                        if (ok) ok = mbar_wait_warp(bar_s_free(buf), before, ctl, 226, s);
                         if (!ok) break;
                     }
                     tc_fence_after();
@@ -391,32 +392,33 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                         if (kMode == 1) tc_mma(tmem + C::s(buf), a1d + aoff, b1d + off, idesc_ss, j > 0);
                         else tc_mma_ts(tmem + C::s(buf), tmem + C::own1 + 8u * j, b1d + off, idesc_ss, j > 0);
                     }
-                    // look ahead: probe the next entry's barriers between the two contractions and read the answer after them
-                    bool nf = false, ns = kMode == 0;
-                    if (e + 1 < it.n) {
-                        nf = mbar_test(bar_full((s + 1) % kSlots), ((s + 1) / kSlots) & 1);
-                        if (kMode == 1) ns = mbar_test(bar_ts_done((s + 1) % kBufs), (((s + 1) / kBufs) & 1) ^ 1);
+                    tc_commit(bar_s_full(buf));
+                    __syncwarp();
+                    // the gradient MMAs of entry s - 2 have read dS from dP's columns
+                    if (!__all_sync(0xffffffffu, mbar_test(bar_ts_done(buf), before))) {
+                        ok = mbar_wait_warp(bar_ts_done(buf), before, ctl, 227, s);
+                        if (!ok) break;
                     }
                     tc_fence_after();
-                    if (s > 0) {  // dP of the entry before is in registers
-                        ok = mbar_wait_warp(bar_s_free((s - 1) & 1), ((s - 1) >> 1) & 1, ctl, 227, s);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j) {
                         const uint64_t off = (uint64_t)(((j >> 2) * Ly::bHalf + (j & 3) * 32) >> 4);
                         const uint64_t aoff = (uint64_t)(((j >> 2) * Ly::aHalf + (j & 3) * 32) >> 4);
-                        if (kMode == 1) tc_mma(tmem + C::dp, a2d + aoff, b2d + off, idesc_ss, j > 0);
-                        else tc_mma_ts(tmem + C::dp, tmem + C::own2 + 8u * j, b2d + off, idesc_ss, j > 0);
+                        if (kMode == 1) tc_mma(tmem + C::dp(buf), a2d + aoff, b2d + off, idesc_ss, j > 0);
+                        else tc_mma_ts(tmem + C::dp(buf), tmem + C::own2 + 8u * j, b2d + off, idesc_ss, j > 0);
                     }
-                    tc_commit(bar_s_full(s & 1));
+                    tc_commit(bar_d_full(buf));
                     if (e == it.n - 1) tc_commit(kMode == 1 ? bar_a_empty : bar_at_free);  // the own tiles have been read
                     __syncwarp();
+                    bool nf = false, ns = false;
+                    if (e + 1 < it.n) {
+                        nf = mbar_test(bar_full((s + 1) % kSlots), ((s + 1) / kSlots) & 1);
+                        ns = mbar_test(bar_s_free(buf ^ 1), (((s + 1) >> 1) & 1) ^ 1);
+                    }
                     pre = __all_sync(0xffffffffu, nf && ns);
                 }
             }
-        } else if (warp == 10) {
+        } else if (warp == kMathWarps + 2) {
             // ================================================================== issuer of the gradient MMAs: A from TMEM (8 columns
             // per 16-row step), B the streamed tile, MN-major (64-column halves apart = LBO, 8-row groups 1 KiB apart = SBO, 16
             // rows = 2 KiB per step)
@@ -431,51 +433,67 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                 ++kk;
                 bool pre = false;
                 for (int e = 0; e < it.n && ok; ++e, ++s) {
-                    const int slot = s % kSlots, buf = s % kBufs;
+                    const int slot = s % kSlots, buf = s & 1;
                     if (!pre) {
                         ok = mbar_wait_warp(bar_full(slot), (s / kSlots) & 1, ctl, 228 + kMode, s);
                         if (!ok) break;
                     }
                     unsigned char* const tiles = smem + Ly::offB + slot * 2 * Ly::bTile;
-                    // dQ pass: K is summed over; dK/dV pass: Q and dO
-                    constexpr int kLook = kMode == 0 ? Ly::bTile : 2 * Ly::bTile;
-                    bool bad = false;
-                    if (kMode == 0 ? mixed_keys(it, e) : mixed_queries(it, seen_of_slot(slot)[kBlk])) {
+                    const uint32_t tile = sbase + Ly::offB + slot * 2 * Ly::bTile;
+                    const uint64_t b1m = smem_desc(tile, Ly::bHalf, 1024), b2m = smem_desc(tile + Ly::bTile, Ly::bHalf, 1024);
+                    // Tiles that are summed over (dQ pass: K; dK/dV pass: dO, then Q): whether one holds a value that is not finite
+                    const bool mixed = kMode == 0 ? mixed_keys(it, e) : mixed_queries(it, seen_of_slot(slot)[kBlk]);
+                    auto look_at = [&](int from) {
+                        bool bad = false;
 #pragma unroll 8
-                        for (int c = lane; c < kLook / 16; c += 32) bad |= chunk_nonfinite<T>(reinterpret_cast<const uint4*>(tiles)[c]);
-                        bad = __any_sync(0xffffffffu, bad);
-                    }
-                    if (!pre) {
-                        ok = mbar_wait_warp(bar_x_full(buf), (s / kBufs) & 1, ctl, 224 + kMode, s);
-                        if (!ok) break;
-                    }
-                    if (LCBSA_UNLIKELY(bad)) {  // the arithmetic warps have S and dP, so their MMAs have read the tiles
+                        for (int c = lane; c < Ly::bTile / 16; c += 32) bad |= chunk_nonfinite<T>(reinterpret_cast<const uint4*>(tiles + from)[c]);
+                        return __any_sync(0xffffffffu, bad);
+                    };
+                    // once S and dP of the entry have read the tile
+                    auto clean = [&](int from) {
 #pragma unroll 1
-                        for (int c = lane; c < kLook / 4; c += 32) {
-                            uint32_t* p = reinterpret_cast<uint32_t*>(tiles) + c;
+                        for (int c = lane; c < Ly::bTile / 4; c += 32) {
+                            uint32_t* p = reinterpret_cast<uint32_t*>(tiles + from) + c;
                             *p = zero_nonfinite<T>(*p);
                         }
                         fence_proxy_async();
                         __syncwarp();
+                    };
+                    const bool bad1 = mixed && look_at(0);
+                    if (kMode == 1) {
+                        const bool bad2 = mixed && look_at(Ly::bTile);
+                        if (!__all_sync(0xffffffffu, mbar_test(bar_p_full(buf), (s >> 1) & 1))) {
+                            ok = mbar_wait_warp(bar_p_full(buf), (s >> 1) & 1, ctl, 245, s);
+                            if (!ok) break;
+                        }
+                        if (LCBSA_UNLIKELY(bad2)) {
+                            ok = mbar_wait_warp(bar_d_full(buf), (s >> 1) & 1, ctl, 246, s);  // dP has read dO
+                            if (!ok) break;
+                            clean(Ly::bTile);
+                        }
+                        tc_fence_after();
+#pragma unroll
+                        for (int j = 0; j < kBlk / 16; ++j)  // dV += P^T dO
+                            tc_mma_ts(tmem + C::acc2, tmem + C::s(buf) + piece(j), b2m + (uint64_t)((j * 2048) >> 4), idesc_ts, (e > 0 || j > 0) ? 1u : 0u);
+                        tc_commit(bar_s_free(buf));  // P's columns are S's
+                        __syncwarp();
                     }
+                    if (!pre) {
+                        ok = mbar_wait_warp(bar_x_full(buf), (s >> 1) & 1, ctl, 224 + kMode, s);
+                        if (!ok) break;
+                    }
+                    if (LCBSA_UNLIKELY(bad1)) clean(0);
                     bool nf = false, nx = false;
                     if (e + 1 < it.n) {
                         nf = mbar_test(bar_full((s + 1) % kSlots), ((s + 1) / kSlots) & 1);
-                        nx = mbar_test(bar_x_full((s + 1) % kBufs), ((s + 1) / kBufs) & 1);
+                        nx = mbar_test(bar_x_full(buf ^ 1), ((s + 1) >> 1) & 1);
                     }
                     tc_fence_after();
-                    const uint32_t tile = sbase + Ly::offB + slot * 2 * Ly::bTile;
-                    const uint64_t b1m = smem_desc(tile, Ly::bHalf, 1024), b2m = smem_desc(tile + Ly::bTile, Ly::bHalf, 1024);
-                    if (kMode == 1) {
-#pragma unroll
-                        for (int j = 0; j < kBlk / 16; ++j)  // dV += P^T dO
-                            tc_mma_ts(tmem + C::acc2, tmem + C::xp(buf) + 8u * j, b2m + (uint64_t)((j * 2048) >> 4), idesc_ts, (e > 0 || j > 0) ? 1u : 0u);
-                    }
 #pragma unroll
                     for (int j = 0; j < kBlk / 16; ++j)  // dQ += dS K, or dK += dS^T Q
-                        tc_mma_ts(tmem + C::acc1, tmem + C::xd(buf) + 8u * j, b1m + (uint64_t)((j * 2048) >> 4), idesc_ts, (e > 0 || j > 0) ? 1u : 0u);
+                        tc_mma_ts(tmem + C::acc1, tmem + C::dp(buf) + piece(j), b1m + (uint64_t)((j * 2048) >> 4), idesc_ts, (e > 0 || j > 0) ? 1u : 0u);
                     tc_commit(bar_empty(slot));  // the streamed tiles are free once these MMAs have read them
-                    tc_commit(bar_ts_done(buf)); // and so are P and dS
+                    tc_commit(bar_ts_done(buf)); // and so is dS
                     if (e == it.n - 1) tc_commit(bar_acc_done);
                     __syncwarp();
                     pre = __all_sync(0xffffffffu, nf && nx);
@@ -485,21 +503,20 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMath));
         // ================================================================== arithmetic warps
-        const int wg = warp >> 2;  // entries of even or odd number
+        const int wg = warp >> 3, half = (warp >> 2) & 1;  // entries of even or odd number, columns 32 half .. 32 half + 31 of them
         const int wq = warp & 3;   // TMEM quadrant of this warp
         const int row = wq * 32 + lane;  // row of the own tile = TMEM lane
         const uint32_t t_lane = (uint32_t)(wq * 32) << 16;
         bool ok = start_ok;
         unsigned s0 = 0, kk = 0;  // entries before the current item, items with entries before it
-        // dQ pass: the own tiles go from shared memory to TMEM, where they are the A operands of every S and dP.  Warpgroup g moves A1 (0) or
-        // A2 (1).
+        // dQ pass: the own tiles go from shared memory to TMEM, where they are the A operands of every S and dP.  Warpgroup 2 g + h moves half h
+        // of A1 (g = 0) or A2 (g = 1).
         auto own_to_tmem = [&](unsigned item) -> bool {
             if (kMode == 1) return true;
             if (!mbar_wait_warp(bar_a_full, item & 1, ctl, 242, item)) return false;
             if (item > 0 && !mbar_wait_warp(bar_at_free, (item - 1) & 1, ctl, 243, item)) return false;
             tc_fence_after();
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half) {
+            if (half < kHalves) {
                 const unsigned char* src = smem + Ly::offA + wg * Ly::aTile + half * Ly::aHalf + row * 128;
                 uint32_t ar[32];
 #pragma unroll
@@ -519,21 +536,18 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
             mbar_arrive_elect(bar_a_empty);
             return true;
         };
-        const float2 sc = make_float2(P.scale, P.scale);
-        // Two scores and two dP -> P and dS.  nl, nd: -lse * log2(e) and -delta; far: distances.
-        auto pair = [&](float2 s, float2 dp, float2 nl, float2 nd, float2 far, float slope2, bool large, float2& p, float2& ds) {
-            float2 slack, x;
+        // Two scores -> P, and 1 - tanh^2 with a cap.  nl: -lse * log2(e) (dQ pass: of the scale's magnitude more, so that P times dP - delta is
+        // dS); far: distances.
+        auto probs = [&](float2 s, float2 nl, float2 far, float slope2, bool large, float2& slack) {
+            float2 x;
+            if (kBias) nl = __ffma2_rn(far, make_float2(-slope2, -slope2), nl);
             if (kCap) {
                 x = large ? capped_any(P.shape, s, slack) : capped_small(P.shape, s, slack);
-                if (kBias) x = __ffma2_rn(far, make_float2(-slope2, -slope2), x);
                 x = __fadd2_rn(x, nl);
             } else {
-                if (kBias) nl = __ffma2_rn(far, make_float2(-slope2, -slope2), nl);
                 x = __ffma2_rn(s, make_float2(P.shape.mul, P.shape.mul), nl);
             }
-            p = make_float2(ex2(x.x), ex2(x.y));
-            ds = __fmul2_rn(__fmul2_rn(p, __fadd2_rn(dp, nd)), sc);
-            if (kCap) ds = __fmul2_rn(ds, slack);
+            return make_float2(ex2(x.x), ex2(x.y));
         };
         auto two = [](uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); };
         // dQ pass: what this thread's query sees, its -lse * log2(e) and -delta, the slope of its head; dK/dV pass: nothing yet
@@ -548,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                 if (u < P.n_u) {
                     r.see = P.seen[((long long)b * P.n_u + u) * kSeenPitch + i % kBlk];
                     const float* st = P.stats + ((long long)it.bh * P.n_u + u) * kDenseStats + i % kBlk;
-                    r.nl = st[0];
+                    r.nl = st[0] + P.scale_lg;
                     r.nd = st[kBlk];
                 }
                 if (kBias) r.slope2 = __ldg(P.slopes + h) * kLog2e;
@@ -576,76 +590,79 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
             }
             for (unsigned i = s0 + ((s0 ^ wg) & 1); i < s0 + n && ok; i += 2) {
                 const unsigned r = i >> 1;
-                const int slot = i % kSlots, buf = i % kBufs;
+                const int slot = i % kSlots;
                 // dK/dV pass: what came with the slot's tiles
                 if (kMode == 1) ok = mbar_wait_warp(bar_full(slot), (i / kSlots) & 1, ctl, 234 + wg, i);
                 if (ok) ok = mbar_wait_warp(bar_s_full(wg), r & 1, ctl, 230 + wg, i);
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t xp[32], xd[32], sr[64], dr[64];
-                tc_ld64(tmem + C::s(buf) + t_lane, sr);
-                tc_ld64(tmem + C::dp + t_lane, dr);
+                uint32_t x[32], out[16];  // S, then dP
+                float2 p[16];      // what dP - delta is multiplied by: P times 1 - tanh^2 and, dK/dV pass, the scale
+                tc_ld32(tmem + C::s(wg) + 32u * half + t_lane, x);
                 tc_wait_ld();
-                tc_fence_before();
-                mbar_arrive_elect(bar_s_free(wg));  // dP may be overwritten by that of entry i + 1
-                const bool large = kCap && any_large(sr, P.shape.inv);
+                if (kMode == 0) {
+                    tc_fence_before();
+                    mbar_arrive_elect(bar_s_free(wg));
+                }
+                const bool large = kCap && any_large(x, P.shape.inv);
+                bool mixed;
+                const float4* const st4 = reinterpret_cast<const float4*>(smem + Ly::offExtra + slot * Ly::extra) + 8 * half;  // dK/dV pass
                 if constexpr (kMode == 0) {
-                    const int key0 = it.first + kBlk * (int)(i - s0);
-                    const bool mixed = mixed_keys(it, (int)(i - s0));
-                    const float at = (float)(me.see.z - key0);
-                    const int lo = me.see.x - key0, hi = me.see.y - key0;
-                    auto all = [&](bool lg, bool mx) {
+                    const int first = it.first + kBlk * (int)(i - s0) + 32 * half;  // key of the warp's first column
+                    mixed = mixed_keys(it, (int)(i - s0));
+                    const float at = (float)(me.see.z - first);
+                    auto all = [&](bool lg) {
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            float2 p, ds, far = make_float2(0.f, 0.f);
+                        for (int k = 0; k < 16; ++k) {
+                            float2 far = make_float2(0.f, 0.f);
                             if (kBias) far = make_float2(fabsf(at - (float)(2 * k)), fabsf(at - (float)(2 * k + 1)));
-                            pair(two(sr[2 * k], sr[2 * k + 1]), two(dr[2 * k], dr[2 * k + 1]), make_float2(me.nl, me.nl), make_float2(me.nd, me.nd), far,
-                                 slope2, lg, p, ds);
-                            if (mx) {
-                                if (2 * k < lo || 2 * k >= hi) ds.x = 0.f;
-                                if (2 * k + 1 < lo || 2 * k + 1 >= hi) ds.y = 0.f;
-                            }
-                            xd[k] = pack2(kBf16, ds.x, ds.y);
+                            float2 slack;
+                            p[k] = probs(two(x[2 * k], x[2 * k + 1]), make_float2(me.nl, me.nl), far, slope2, lg, slack);
+                            if (kCap) p[k] = __fmul2_rn(p[k], slack);
                         }
                     };
-                    if (kCap && LCBSA_UNLIKELY(large)) all(true, true);
-                    else if (mixed) all(false, true);
-                    else all(false, false);
-                    // the gradient MMAs of entry i - 2 have read the columns
-                    ok = mbar_wait_warp(bar_ts_done(wg), (r & 1) ^ 1, ctl, 236 + wg, i);
-                    if (!ok) break;
-                    tc_fence_after();
+                    if (kCap && LCBSA_UNLIKELY(large)) all(true);
+                    else all(false);
+                    if (mixed) {
+                        const int lo = min(max(me.see.x - first, 0), 32), hi = min(max(me.see.y - first, 0), 32);  // a run of bits
+                        const uint32_t sees = hi > lo ? (~0u >> (32 - (hi - lo))) << lo : 0u;
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            if (!((sees >> (2 * k)) & 1u)) p[k].x = 0.f;
+                            if (!((sees >> (2 * k + 1)) & 1u)) p[k].y = 0.f;
+                        }
+                    }
                 } else {
-                    const float4* const st4 = reinterpret_cast<const float4*>(smem + Ly::offExtra + slot * Ly::extra);
                     const int4* const see = seen_of_slot(slot);
-                    const bool mixed = mixed_queries(it, see[kBlk]);
+                    mixed = mixed_queries(it, see[kBlk]);
                     // the queries of a whole entry belong to one document, so their places follow one another
-                    const float at = kBias ? (float)(see[0].z - key) : 0.f;
+                    const float at = kBias ? (float)(see[0].z + 32 * half - key) : 0.f;
                     auto all = [&](bool lg, bool mx) {
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const float4 l4 = st4[k >> 1], d4 = st4[16 + (k >> 1)];
-                            const float2 nl = k & 1 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
-                            const float2 nd = k & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
-                            float2 p, ds, far = make_float2(0.f, 0.f);
+                        for (int k = 0; k < 16; ++k) {
+                            const float4 l4 = st4[k >> 1];
+                            float2 far = make_float2(0.f, 0.f);
                             int4 a = make_int4(0, 0, 0, 0), c = a;
                             if (mx) {
-                                a = see[2 * k];
-                                c = see[2 * k + 1];
+                                a = see[32 * half + 2 * k];
+                                c = see[32 * half + 2 * k + 1];
                             }
                             if (kBias) {
                                 far = make_float2(fabsf(at + (float)(2 * k)), fabsf(at + (float)(2 * k + 1)));
                                 if (mx) far = make_float2(fabsf((float)(a.z - key)), fabsf((float)(c.z - key)));
                             }
-                            pair(two(sr[2 * k], sr[2 * k + 1]), two(dr[2 * k], dr[2 * k + 1]), nl, nd, far, slope2, lg, p, ds);
+                            float2 slack;
+                            p[k] = probs(two(x[2 * k], x[2 * k + 1]), k & 1 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y), far, slope2, lg, slack);
                             if (mx) {
-                                if (!isfinite(nd.x)) p.x = __int_as_float(0x7fc00000);  // dO is not finite
-                                if (!isfinite(nd.y)) p.y = __int_as_float(0x7fc00000);
-                                if (key < a.x || key >= a.y) p.x = ds.x = 0.f;
-                                if (key < c.x || key >= c.y) p.y = ds.y = 0.f;
+                                const float4 d4 = st4[16 + (k >> 1)];
+                                if (!isfinite(k & 1 ? d4.z : d4.x)) p[k].x = __int_as_float(0x7fc00000);  // dO is not finite
+                                if (!isfinite(k & 1 ? d4.w : d4.y)) p[k].y = __int_as_float(0x7fc00000);
+                                if (key < a.x || key >= a.y) p[k].x = 0.f;
+                                if (key < c.x || key >= c.y) p[k].y = 0.f;
                             }
-                            xp[k] = pack2(kBf16, p.x, p.y);
-                            xd[k] = pack2(kBf16, ds.x, ds.y);
+                            out[k] = pack2(kBf16, p[k].x, p[k].y);
+                            p[k] = __fmul2_rn(p[k], make_float2(P.scale, P.scale));
+                            if (kCap) p[k] = __fmul2_rn(p[k], slack);
                         }
                     };
                     if (kCap && LCBSA_UNLIKELY(large)) all(true, true);
@@ -653,17 +670,43 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     else all(false, false);
                     unit += 2;
                     if (wrap() && kBias && head < P.walk) slope2 = __ldg(P.slopes + h0 + head) * kLog2e;
-                    tc_st32(tmem + C::xp(buf) + t_lane, xp);  // S's columns: this warp has read its lanes of them
+                    tc_st16(tmem + C::s(wg) + 32u * half + t_lane, out);  // the columns that this thread read
+                    tc_wait_st();
+                    tc_fence_before();
+                    mbar_arrive_elect(bar_p_full(wg));
                 }
-                tc_st32(tmem + C::xd(buf) + t_lane, xd);
+                ok = mbar_wait_warp(bar_d_full(wg), r & 1, ctl, 236 + wg, i);
+                if (!ok) break;
+                tc_fence_after();
+                tc_ld32(tmem + C::dp(wg) + 32u * half + t_lane, x);
+                tc_wait_ld();
+                auto grads = [&](bool mx) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        float2 nd = make_float2(me.nd, me.nd);
+                        if (kMode == 1) {
+                            const float4 d4 = st4[16 + (k >> 1)];
+                            nd = k & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
+                        }
+                        float2 ds = __fmul2_rn(p[k], __fadd2_rn(two(x[2 * k], x[2 * k + 1]), nd));
+                        if (mx) {  // hidden, whatever dP is
+                            if (p[k].x == 0.f) ds.x = 0.f;
+                            if (p[k].y == 0.f) ds.y = 0.f;
+                        }
+                        out[k] = pack2(kBf16, ds.x, ds.y);
+                    }
+                };
+                if (mixed) grads(true);
+                else grads(false);
+                tc_st16(tmem + C::dp(wg) + 32u * half + t_lane, out);
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive_elect(bar_x_full(buf));
+                mbar_arrive_elect(bar_x_full(wg));
             }
             s0 += n;
         };
-        // The accumulated gradients of an item's rows: TMEM -> registers, which frees the accumulators -> global memory.  dQ pass: warpgroup
-        // g stores half g of dQ; dK/dV pass: warpgroup 0 dK, 1 dV.
+        // The accumulated gradients of an item's rows: TMEM -> registers, which frees the accumulators -> global memory, 32 columns at a
+        // time.  dQ pass: warpgroup 2 g + h stores columns 32 (2 g + h) .. of dQ; dK/dV pass: half h of dK (g = 0) or dV (g = 1).
         auto store_item = [&](const Item& it, unsigned item) -> bool {
             const int b = it.bh / P.heads, h = it.bh % P.heads, i = it.own * kM + row;
             const bool second = kMode == 1 && wg == 1;
@@ -676,12 +719,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
             }
             tc_fence_after();
             constexpr int kParts = kMode == 1 ? kHalves : 1;
-#pragma unroll
+#pragma unroll 1
             for (int part = 0; part < kParts; ++part) {
-                const int half = kMode == 1 ? part : wg;
-                uint32_t acc[64];
+                const int col = kMode == 1 ? 32 * (half * kHalves + part) : 32 * (2 * wg + half);
+                uint32_t acc[32];
                 if (it.n > 0) {
-                    tc_ld64(t_acc + 64u * (half < kHalves ? half : 0), acc);
+                    tc_ld32(t_acc + (col < D ? col : 0), acc);
                     tc_wait_ld();
                     if (part == kParts - 1) {
                         tc_fence_before();
@@ -689,16 +732,20 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) acc[j] = 0u;  // nobody sees these rows, or they see nothing
+                    for (int j = 0; j < 32; ++j) acc[j] = 0u;  // nobody sees these rows, or they see nothing
                 }
-                if (i >= P.rows || half >= kHalves) continue;
-                if (kMode == 1 && P.splits > 1) {
-                    float4* dst = reinterpret_cast<float4*>(P.part + (((long long)(second ? P.B * P.heads : 0) + it.bh) * P.rows + i) * D + 64 * half);
+                if (kMode == 0 && P.sign < 0.f) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
+                    for (int j = 0; j < 32; ++j) acc[j] ^= 0x80000000u;
+                }
+                if (i >= P.rows || col >= D) continue;
+                if (kMode == 1 && P.splits > 1) {
+                    float4* dst = reinterpret_cast<float4*>(P.part + (((long long)(second ? P.B * P.heads : 0) + it.bh) * P.rows + i) * D + col);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
                         dst[j] = make_float4(__uint_as_float(acc[4 * j]), __uint_as_float(acc[4 * j + 1]), __uint_as_float(acc[4 * j + 2]), __uint_as_float(acc[4 * j + 3]));
                 } else {
-                    store_row64<kBf16>(row_ptr, 64 * half, acc);
+                    store_row32<kBf16>(row_ptr, col, acc);
                 }
             }
             return true;
@@ -737,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
     tc_fence_before();
     __syncthreads();
     if (tid == 0) ctl_report(ctl);
-    if (warp == 9) {
+    if (warp == kMathWarps + 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
@@ -809,6 +856,8 @@ cudaError_t passes(const DenseArgs& a, cudaStream_t st, const char** why) {
     P.seen = a.seen; P.hulls = a.hulls; P.stats = a.stats; P.slopes = a.slopes; P.status = a.status;
     P.B = a.B; P.Hq = a.Hq; P.Hk = a.Hk; P.group = a.group; P.n_u = dense_units(a.Sq); P.n_k = dense_units(a.Sk);
     P.scale = a.scale;
+    P.scale_lg = log2f(fabsf(a.scale));  // -inf for 0: dQ is 0
+    P.sign = a.scale < 0.f ? -1.f : 1.f;
     P.shape = score_shape(a.scale, a.cap);
     auto map = [&](CUtensorMap* tm, const View& v, int H, int S, int box, int* fold) {
         if (S == 0 || dense_rows_map(tm, a.dtype, v, a.B, H, S, D, box, fold)) return true;
