@@ -15,8 +15,8 @@
 // they are explained.  What differs: the walks are runs, so no lists are read; an entry is whole (all of its pairs are seen) or mixed, and
 // only mixed ones are masked pair by pair; a query unit brings what its rows see along with its lse and delta.
 //
-// Hidden values may be anything.  A hidden pair's P and dS are set to zero; in mixed entries the issuer of the gradient MMAs looks through the
-// tiles that are summed over and, once S and dP have read them, sets values that are not finite to zero (0 * inf is not 0).  A pair
+// Hidden values may be anything.  A hidden pair's P and dS are set to zero; in mixed entries a producer looks through the tiles that are
+// summed over, and once S and dP have read them the issuer of the gradient MMAs sets values that are not finite to zero (0 * inf is not 0).  A pair
 // that is seen has its NaN from S and dP; for dV it is the query's delta that says that dO is not finite.
 //
 // Every mbarrier wait is bounded; when one runs out the CTA flags the status word, drains its copies, frees TMEM, returns.
@@ -51,10 +51,10 @@ template <int D> struct Lay {
     static constexpr int offExtra = offB + slots * 2 * bTile;
     static constexpr int offBar = offExtra + slots * extra;
     // barriers: full[slots], empty[slots], s_full[2], s_free[2], d_full[2], p_full[2], x_full[2], ts_done[2], a_full, a_empty, at_full,
-    //           at_free, acc_done, acc_free, item_full[kItemRing], item_empty[kItemRing]
-    static constexpr int numBars = 2 * slots + 12 + 6 + 2 * kItemRing;
+    //           at_free, acc_done, acc_free, item_full[kItemRing], item_empty[kItemRing], looked[slots]
+    static constexpr int numBars = 3 * slots + 12 + 6 + 2 * kItemRing;
     static constexpr int offMisc = (offBar + numBars * 8 + 15) / 16 * 16;  // abort flag, TMEM base
-    static constexpr int offItems = offMisc + 64;
+    static constexpr int offItems = offMisc + 80;
     static constexpr int smem = offItems + kItemRing * 32;
 };
 static_assert(Lay<128>::offExtra % 16 == 0 && Lay<128>::extra % 16 == 0 && Lay<128>::offBar % 8 == 0, "bulk copies and barriers are aligned");
@@ -93,7 +93,7 @@ struct BwdParams {
     // dK/dV pass: the query heads of a group are split over `splits` items of `walk` heads each, whose sums go to part [2][B * Hk * splits][Sk][D]
     int splits, walk;
     float* part;
-    int n_items;
+    int n_items, wave;
     float scale, scale_lg;  // log2 of its magnitude
     float sign;             // of the scale (dQ pass)
     ScoreShape shape;
@@ -124,7 +124,7 @@ __device__ __forceinline__ void store_row32(unsigned char* row_ptr, int col0, co
 }
 
 // whether one of the scores is too large for the polynomial of the cap (a NaN is passed over: it stays one through it)
-__device__ __forceinline__ bool any_large(const uint32_t (&r)[32], float inv) {
+__device__ __forceinline__ bool any_large(const uint32_t (&r)[32], float s_small) {
     float m[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -132,7 +132,7 @@ __device__ __forceinline__ bool any_large(const uint32_t (&r)[32], float inv) {
 #pragma unroll
         for (int j = 0; j < 8; j += 2) m[k] = max3(m[k], fabsf(__uint_as_float(r[8 * k + j])), fabsf(__uint_as_float(r[8 * k + j + 1])));
     }
-    return __any_sync(0xffffffffu, !(fabsf(inv) * fmaxf(max3(m[0], m[1], m[2]), m[3]) <= kCapSmall));
+    return __any_sync(0xffffffffu, !(fmaxf(max3(m[0], m[1], m[2]), m[3]) <= s_small));
 }
 
 // kMode 0: dQ pass, 1: dK/dV pass.  Persistent, one CTA per SM.
@@ -160,8 +160,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
     const uint32_t bar_at_free = bar0 + 8u * (kB + 15), bar_acc_done = bar0 + 8u * (kB + 16), bar_acc_free = bar0 + 8u * (kB + 17);
     auto bar_item_full = [&](int k) { return bar0 + 8u * (kB + 18 + k); };
     auto bar_item_empty = [&](int k) { return bar0 + 8u * (kB + 18 + kItemRing + k); };
+    auto bar_looked = [&](int s) { return bar0 + 8u * (kB + 18 + 2 * kItemRing + s); };
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Ly::offMisc);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::offMisc + 32);
+    volatile int* slot_bad = reinterpret_cast<volatile int*>(smem + Ly::offMisc + 36);  // [slots] bit 0: B1, 1: B2 holds a value that is not finite
     int4* items = reinterpret_cast<int4*>(smem + Ly::offItems);
     const Ctl ctl{abort_flag, P.status};
 
@@ -172,6 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(bar_full(s), 2);  // one arrival per producer
             mbar_init(bar_empty(s), 1);
+            mbar_init(bar_looked(s), 1);
         }
         for (int buf = 0; buf < 2; ++buf) {
             mbar_init(bar_s_full(buf), 1);
@@ -251,11 +254,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
             auto look = [&](int id) {
                 Item it{-1, 0, 0, 0, 0, 0, 0};
                 if (id >= P.n_items) return it;
-                const int heads = P.B * P.heads;
-                it.bh = id % heads;
+                dense_item(id, P.B * P.heads, P.n_own, P.wave, it.bh, it.own);
                 const int b = it.bh / P.heads;
                 if (kMode == 0) {  // the last queries first: with a causal order they have most keys
-                    it.own = P.n_own - 1 - id / heads;
+                    it.own = P.n_own - 1 - it.own;
                     const int4* u = P.seen + ((long long)b * P.n_u + 2 * it.own) * kSeenPitch + kBlk;
                     int4 x = __ldg(u), y = make_int4(0, 0, 0, 0x7fffffff);
                     if (2 * it.own + 1 < P.n_u) y = __ldg(u + kSeenPitch);
@@ -265,7 +267,6 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     it.all_lo = max(x.z, y.z);
                     it.all_hi = min(x.w, y.w);
                 } else {  // the first keys first
-                    it.own = id / heads;
                     const int2* hu = P.hulls + (long long)b * P.n_k + 2 * it.own;
                     int2 x = __ldg(hu);
                     if (2 * it.own + 1 < P.n_k) {
@@ -324,6 +325,27 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     }
                 }
                 ++kk;
+                int e_done = 0;  // entries of the item requested
+                // Tiles of mixed entries that are summed over (dQ pass: K; dK/dV pass: Q and dO) are looked through behind the copies, two entries
+                // later, when they have come, and well before their dS.
+                auto look_at = [&](int e) -> bool {
+                    const unsigned g = s - e_done + e;  // number of entry e over the whole kernel
+                    const int ls = g % kSlots;
+                    bool mixed = kMode == 0 && mixed_keys(it, e);
+                    if (kMode == 1 || mixed) {
+                        if (!mbar_wait_warp(bar_full(ls), (g / kSlots) & 1, ctl, 214 + kMode, g)) return false;
+                        if (kMode == 1) mixed = mixed_queries(it, seen_of_slot(ls)[kBlk]);
+                    }
+                    if (mixed) {
+                        const uint4* t = reinterpret_cast<const uint4*>(smem + Ly::offB + ls * 2 * Ly::bTile);
+                        int bad = tile_nonfinite<T, Ly::bTile / 16>(t, lane) ? 1 : 0;
+                        if (kMode == 1 && tile_nonfinite<T, Ly::bTile / 16>(t + Ly::bTile / 16, lane)) bad |= 2;
+                        if (lane == 0) slot_bad[ls] = bad;
+                        __syncwarp();
+                    }
+                    mbar_arrive_elect(bar_looked(ls));
+                    return true;
+                };
                 int unit = it.first, head = kMode == 0 ? h / P.group : h * P.walk;  // of the entry: dK/dV pass a query unit, dQ pass unused
                 for (int e = 0; e < it.n; ++e) {
                     const int slot = s % kSlots;
@@ -346,8 +368,15 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                         unit = it.first;
                         ++head;
                     }
+                    e_done = e + 1;
+                    if (!is_b1 && e >= 2) {
+                        ok = look_at(e - 2);
+                        if (!ok) break;
+                    }
                     if (is_b1 && e == it.n - 1) step();  // behind the item's last copies, none of which waits for the counter
                 }
+                if (!is_b1)
+                    for (int e = max(it.n - 2, 0); e < it.n && ok; ++e) ok = look_at(e);
                 if (!ok) break;
             }
             if ((!ok || *abort_flag != 0) && lane == 0) {
@@ -441,14 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     unsigned char* const tiles = smem + Ly::offB + slot * 2 * Ly::bTile;
                     const uint32_t tile = sbase + Ly::offB + slot * 2 * Ly::bTile;
                     const uint64_t b1m = smem_desc(tile, Ly::bHalf, 1024), b2m = smem_desc(tile + Ly::bTile, Ly::bHalf, 1024);
-                    // Tiles that are summed over (dQ pass: K; dK/dV pass: dO, then Q): whether one holds a value that is not finite
                     const bool mixed = kMode == 0 ? mixed_keys(it, e) : mixed_queries(it, seen_of_slot(slot)[kBlk]);
-                    auto look_at = [&](int from) {
-                        bool bad = false;
-#pragma unroll 8
-                        for (int c = lane; c < Ly::bTile / 16; c += 32) bad |= chunk_nonfinite<T>(reinterpret_cast<const uint4*>(tiles + from)[c]);
-                        return __any_sync(0xffffffffu, bad);
-                    };
                     // once S and dP of the entry have read the tile
                     auto clean = [&](int from) {
 #pragma unroll 1
@@ -459,14 +481,18 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                         fence_proxy_async();
                         __syncwarp();
                     };
-                    const bool bad1 = mixed && look_at(0);
+                    int bad = 0;
+                    if (mixed) {
+                        ok = mbar_wait_warp(bar_looked(slot), (s / kSlots) & 1, ctl, 247, s);
+                        if (!ok) break;
+                        bad = slot_bad[slot];
+                    }
                     if (kMode == 1) {
-                        const bool bad2 = mixed && look_at(Ly::bTile);
                         if (!__all_sync(0xffffffffu, mbar_test(bar_p_full(buf), (s >> 1) & 1))) {
                             ok = mbar_wait_warp(bar_p_full(buf), (s >> 1) & 1, ctl, 245, s);
                             if (!ok) break;
                         }
-                        if (LCBSA_UNLIKELY(bad2)) {
+                        if (LCBSA_UNLIKELY(bad & 2)) {
                             ok = mbar_wait_warp(bar_d_full(buf), (s >> 1) & 1, ctl, 246, s);  // dP has read dO
                             if (!ok) break;
                             clean(Ly::bTile);
@@ -482,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                         ok = mbar_wait_warp(bar_x_full(buf), (s >> 1) & 1, ctl, 224 + kMode, s);
                         if (!ok) break;
                     }
-                    if (LCBSA_UNLIKELY(bad1)) clean(0);
+                    if (LCBSA_UNLIKELY(bad & 1)) clean(0);
                     bool nf = false, nx = false;
                     if (e + 1 < it.n) {
                         nf = mbar_test(bar_full((s + 1) % kSlots), ((s + 1) / kSlots) & 1);
@@ -536,17 +562,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
             mbar_arrive_elect(bar_a_empty);
             return true;
         };
-        // Two scores -> P, and 1 - tanh^2 with a cap.  nl: -lse * log2(e) (dQ pass: of the scale's magnitude more, so that P times dP - delta is
-        // dS); far: distances.
-        auto probs = [&](float2 s, float2 nl, float2 far, float slope2, bool large, float2& slack) {
+        // Two scores -> P, and 1 - tanh^2 with a cap.  c: -lse * log2(e) (dQ pass: and log2 of the scale's magnitude, so that P times
+        // dP - delta is dS), with a bias less the distance times the slope.
+        auto probs = [&](float2 s, float2 c, bool large, float2& slack) {
             float2 x;
-            if (kBias) nl = __ffma2_rn(far, make_float2(-slope2, -slope2), nl);
-            if (kCap) {
-                x = large ? capped_any(P.shape, s, slack) : capped_small(P.shape, s, slack);
-                x = __fadd2_rn(x, nl);
-            } else {
-                x = __ffma2_rn(s, make_float2(P.shape.mul, P.shape.mul), nl);
-            }
+            if (kCap) x = __fadd2_rn(large ? capped_any(P.shape, s, slack) : capped_small(P.shape, s, slack), c);
+            else x = __ffma2_rn(s, make_float2(P.shape.mul, P.shape.mul), c);
             return make_float2(ex2(x.x), ex2(x.y));
         };
         auto two = [](uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); };
@@ -604,25 +625,31 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     tc_fence_before();
                     mbar_arrive_elect(bar_s_free(wg));
                 }
-                const bool large = kCap && any_large(x, P.shape.inv);
+                const bool large = kCap && any_large(x, P.shape.s_small);
                 bool mixed;
                 const float4* const st4 = reinterpret_cast<const float4*>(smem + Ly::offExtra + slot * Ly::extra) + 8 * half;  // dK/dV pass
                 if constexpr (kMode == 0) {
                     const int first = it.first + kBlk * (int)(i - s0) + 32 * half;  // key of the warp's first column
                     mixed = mixed_keys(it, (int)(i - s0));
                     const float at = (float)(me.see.z - first);
-                    auto all = [&](bool lg) {
+                    const bool both_sides = kBias && __any_sync(0xffffffffu, at > 0.f && at < 31.f);
+                    auto all = [&](bool lg, bool two_sides) {
+                        BiasLine line;
+                        if (kBias && !two_sides) line = bias_line(at, slope2, me.nl);
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
-                            float2 far = make_float2(0.f, 0.f);
-                            if (kBias) far = make_float2(fabsf(at - (float)(2 * k)), fabsf(at - (float)(2 * k + 1)));
-                            float2 slack;
-                            p[k] = probs(two(x[2 * k], x[2 * k + 1]), make_float2(me.nl, me.nl), far, slope2, lg, slack);
+                            float2 c = make_float2(me.nl, me.nl), slack;
+                            if (kBias) {
+                                if (two_sides) c = __ffma2_rn(make_float2(fabsf(at - (float)(2 * k)), fabsf(at - (float)(2 * k + 1))), make_float2(-slope2, -slope2), c);
+                                else c = bias_next(line, k);
+                            }
+                            p[k] = probs(two(x[2 * k], x[2 * k + 1]), c, lg, slack);
                             if (kCap) p[k] = __fmul2_rn(p[k], slack);
                         }
                     };
-                    if (kCap && LCBSA_UNLIKELY(large)) all(true);
-                    else all(false);
+                    if (kCap && LCBSA_UNLIKELY(large)) all(true, true);
+                    else if (kBias && both_sides) all(false, true);
+                    else all(false, false);
                     if (mixed) {
                         const int lo = min(max(me.see.x - first, 0), 32), hi = min(max(me.see.y - first, 0), 32);  // a run of bits
                         const uint32_t sees = hi > lo ? (~0u >> (32 - (hi - lo))) << lo : 0u;
@@ -636,38 +663,43 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     const int4* const see = seen_of_slot(slot);
                     mixed = mixed_queries(it, see[kBlk]);
                     // the queries of a whole entry belong to one document, so their places follow one another
-                    const float at = kBias ? (float)(see[0].z + 32 * half - key) : 0.f;
-                    auto all = [&](bool lg, bool mx) {
+                    const float at = kBias ? (float)(key - see[0].z - 32 * half) : 0.f;  // distance to column k: |at - k|
+                    const bool both_sides = kBias && __any_sync(0xffffffffu, at > 0.f && at < 31.f);
+                    auto all = [&](bool lg, bool mx, bool two_sides) {
+                        BiasLine line;
+                        if (kBias && !two_sides) line = bias_line(at, slope2, 0.f);
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
                             const float4 l4 = st4[k >> 1];
-                            float2 far = make_float2(0.f, 0.f);
-                            int4 a = make_int4(0, 0, 0, 0), c = a;
+                            float2 c = k & 1 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y), slack;
+                            int4 a = make_int4(0, 0, 0, 0), d = a;
                             if (mx) {
                                 a = see[32 * half + 2 * k];
-                                c = see[32 * half + 2 * k + 1];
+                                d = see[32 * half + 2 * k + 1];
                             }
                             if (kBias) {
-                                far = make_float2(fabsf(at + (float)(2 * k)), fabsf(at + (float)(2 * k + 1)));
-                                if (mx) far = make_float2(fabsf((float)(a.z - key)), fabsf((float)(c.z - key)));
+                                float2 far = make_float2(fabsf(at - (float)(2 * k)), fabsf(at - (float)(2 * k + 1)));
+                                if (mx) far = make_float2(fabsf((float)(a.z - key)), fabsf((float)(d.z - key)));
+                                if (two_sides) c = __ffma2_rn(far, make_float2(-slope2, -slope2), c);
+                                else c = __fadd2_rn(c, bias_next(line, k));
                             }
-                            float2 slack;
-                            p[k] = probs(two(x[2 * k], x[2 * k + 1]), k & 1 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y), far, slope2, lg, slack);
+                            p[k] = probs(two(x[2 * k], x[2 * k + 1]), c, lg, slack);
                             if (mx) {
                                 const float4 d4 = st4[16 + (k >> 1)];
                                 if (!isfinite(k & 1 ? d4.z : d4.x)) p[k].x = __int_as_float(0x7fc00000);  // dO is not finite
                                 if (!isfinite(k & 1 ? d4.w : d4.y)) p[k].y = __int_as_float(0x7fc00000);
                                 if (key < a.x || key >= a.y) p[k].x = 0.f;
-                                if (key < c.x || key >= c.y) p[k].y = 0.f;
+                                if (key < d.x || key >= d.y) p[k].y = 0.f;
                             }
                             out[k] = pack2(kBf16, p[k].x, p[k].y);
                             p[k] = __fmul2_rn(p[k], make_float2(P.scale, P.scale));
                             if (kCap) p[k] = __fmul2_rn(p[k], slack);
                         }
                     };
-                    if (kCap && LCBSA_UNLIKELY(large)) all(true, true);
-                    else if (mixed) all(false, true);
-                    else all(false, false);
+                    if (kCap && LCBSA_UNLIKELY(large)) all(true, true, true);
+                    else if (mixed) all(false, true, true);
+                    else if (kBias && both_sides) all(false, false, true);
+                    else all(false, false, false);
                     unit += 2;
                     if (wrap() && kBias && head < P.walk) slope2 = __ldg(P.slopes + h0 + head) * kLog2e;
                     tc_st16(tmem + C::s(wg) + 32u * half + t_lane, out);  // the columns that this thread read
@@ -873,6 +905,7 @@ cudaError_t passes(const DenseArgs& a, cudaStream_t st, const char** why) {
         P.o1_sb = a.dq.sb; P.o1_sh = a.dq.sh; P.o1_ss = a.dq.ss;
         P.heads = a.Hq; P.n_own = (a.Sq + kM - 1) / kM; P.rows = a.Sq;
         P.n_items = a.B * a.Hq * P.n_own;
+        P.wave = dense_wave(a.B * a.Hq, 4.0 * a.Sk * D / a.group);
         P.next_item = a.next_item;
         e = pass_shape<kBf16, D, 0>(P, cap, st);
         if (e != cudaSuccess) return e;
@@ -890,6 +923,7 @@ cudaError_t passes(const DenseArgs& a, cudaStream_t st, const char** why) {
         P.part = a.part;
         P.heads = a.Hk * P.splits; P.n_own = (a.Sk + kM - 1) / kM; P.rows = a.Sk;
         P.n_items = a.B * P.heads * P.n_own;
+        P.wave = dense_wave(a.B * P.heads, 4.0 * a.Sq * D * P.walk);
         P.next_item = a.next_item + 1;
         e = pass_shape<kBf16, D, 1>(P, cap, st);
         if (e == cudaSuccess && P.splits > 1) {

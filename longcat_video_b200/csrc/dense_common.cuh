@@ -9,6 +9,8 @@
 #pragma once
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace lcbsa {
@@ -89,26 +91,30 @@ __device__ __forceinline__ Seen dense_seen(const DenseMask& m, int b, int i, int
 //
 //   Any y: tanh(y) = 1 - t, t = 2 / (1 + exp(2 y)): two special functions, right at both ends (exp = inf: 1; exp = 0: -1), off by a few
 //   2^-24 in between.  (The machine's own tanh is off by 2^-11, which a cap of 50 would make 2 % of a probability.)
-//   |y| <= 0.75: tanh(y) = y p(y^2), p of degree 5 through the Chebyshev nodes of [0, 0.75^2], off by 1.3 * 2^-23 of the value, on the
-//   arithmetic units, which have time where the special functions (16 a clock and SM) are what a tile waits for.
+//   |y| <= 1/2: tanh(y) = y p(y^2), p of degree 3 through the Chebyshev nodes of [0, 1/4], off by 4.6 * 2^-23 of the value; with the powers of
+//   scale / cap in its coefficients x2 = s (c0 + t (c1 + t (c2 + t c3))), t = s^2: five operations of the arithmetic units, where the special
+//   functions (16 a clock and SM, one per score already) would take twice as long as the rest of a tile.
 struct ScoreShape {
     float mul;     // scale * log2(e)
-    float inv;     // scale / cap
     float mul_ex;  // 2 * scale / cap * log2(e)
     float cap2;    // cap * log2(e)
+    float c[4];
+    float s_small; // scores up to this magnitude go through the polynomial
     float slope2;  // slope of the head * log2(e)
 };
 inline ScoreShape score_shape(float scale, float cap) {
-    const double e = 1.4426950408889634;
+    const double e = 1.4426950408889634, y = cap > 0.f ? (double)scale / cap : 0.0;
+    const double p[4] = {0.9999994510270873, -0.3332628423141673, 0.13189939425594957, -0.044392738432622175};
     ScoreShape s;
     s.mul = (float)(scale * e);
-    s.inv = cap > 0.f ? (float)((double)scale / cap) : 0.f;
-    s.mul_ex = cap > 0.f ? (float)(2.0 * scale / cap * e) : 0.f;
+    s.mul_ex = (float)(2.0 * y * e);
     s.cap2 = (float)(cap * e);
+    double f = scale * e;
+    for (int i = 0; i < 4; ++i, f *= y * y) s.c[i] = (float)(f * p[i]);
+    s.s_small = y != 0.0 ? (float)(0.5 / (y < 0 ? -y : y)) : 0.f;
     s.slope2 = 0.f;
     return s;
 }
-constexpr float kCapSmall = 0.75f;
 __device__ __forceinline__ float dense_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -126,23 +132,42 @@ __device__ __forceinline__ float2 capped_any(const ScoreShape& f, float2 s, floa
     slack = __fmul2_rn(t, __fadd2_rn(make_float2(2.f, 2.f), make_float2(-t.x, -t.y)));
     return __ffma2_rn(t, m, c);
 }
-__device__ __forceinline__ float2 cap_poly(float2 z) {
+// the same for small scores, plus c
+__device__ __forceinline__ float2 capped_small_plus(const ScoreShape& f, float2 s, float2 c) {
     auto both = [](float x) { return make_float2(x, x); };
-    float2 p = __ffma2_rn(z, both(-0.004711522255092859f), both(0.019576216116547585f));
-    p = __ffma2_rn(p, z, both(-0.05334111675620079f));
-    p = __ffma2_rn(p, z, both(0.13325339555740356f));
-    p = __ffma2_rn(p, z, both(-0.33332952857017517f));
-    return __ffma2_rn(p, z, both(1.f));
+    const float2 t = __fmul2_rn(s, s);
+    float2 p = __ffma2_rn(t, both(f.c[3]), both(f.c[2]));
+    p = __ffma2_rn(p, t, both(f.c[1]));
+    p = __ffma2_rn(p, t, both(f.c[0]));
+    return __ffma2_rn(s, p, c);
 }
 __device__ __forceinline__ float2 capped_small(const ScoreShape& f, float2 s, float2& slack) {
-    const float2 y = __fmul2_rn(s, make_float2(f.inv, f.inv)), p = cap_poly(__fmul2_rn(y, y)), t = __fmul2_rn(y, p);
+    const float2 x = capped_small_plus(f, s, make_float2(0.f, 0.f));
+    const float i = 1.f / f.cap2;
+    const float2 t = __fmul2_rn(x, make_float2(i, i));
     slack = __ffma2_rn(t, make_float2(-t.x, -t.y), make_float2(1.f, 1.f));
-    return __fmul2_rn(__fmul2_rn(s, make_float2(f.mul, f.mul)), p);
+    return x;
 }
-// the same plus c
-__device__ __forceinline__ float2 capped_small_plus(const ScoreShape& f, float2 s, float2 c) {
-    const float2 y = __fmul2_rn(s, make_float2(f.inv, f.inv));
-    return __ffma2_rn(__fmul2_rn(s, make_float2(f.mul, f.mul)), cap_poly(__fmul2_rn(y, y)), c);
+
+// The bias of n columns whose keys lie on one side of the query, plus a constant: plus - slope |at - j| is a line in the column's number j.
+// Four chains of pairs, eight columns a step.
+struct BiasLine {
+    float2 c[4], step8;
+};
+// at <= 0: the keys are ahead; at >= n - 1: behind
+__device__ __forceinline__ BiasLine bias_line(float at, float slope2, float plus) {
+    const float sl = at > 0.f ? slope2 : -slope2, base = fmaf(-sl, at, plus);
+    BiasLine l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) l.c[k] = make_float2(fmaf(sl, (float)(2 * k), base), fmaf(sl, (float)(2 * k + 1), base));
+    l.step8 = make_float2(8.f * sl, 8.f * sl);
+    return l;
+}
+// pair number k (columns 2k, 2k + 1), called once for each in ascending order
+__device__ __forceinline__ float2 bias_next(BiasLine& l, int k) {
+    const float2 v = l.c[k & 3];
+    l.c[k & 3] = __fadd2_rn(v, l.step8);
+    return v;
 }
 
 // Whether one of the eight 16-bit values of a 16-byte chunk is an infinity or a NaN (all exponent bits set).
@@ -154,12 +179,45 @@ __device__ __forceinline__ bool chunk_nonfinite(const uint4& v) {
     auto hot = [](uint32_t u) { return (((u & kExp) >> 1) + (kLow >> 1)) & 0x40004000u; };
     return (hot(v.x) | hot(v.y) | hot(v.z) | hot(v.w)) != 0;
 }
+// A warp: whether a tile of n 16-byte chunks holds one.  Every pair of values times zero is added up: 0, or NaN from the first infinity or
+// NaN on; one instruction a pair (the test of the exponents takes four), so a tile of 16 KB takes some 170 instructions.
+template <typename T, int n>
+__device__ __forceinline__ bool tile_nonfinite(const uint4* tile, int lane) {
+    using T2 = typename std::conditional<DType<T>::code == LCBSA_BF16, __nv_bfloat162, __half2>::type;
+    const uint32_t z = 0u;
+    const T2 zero = *reinterpret_cast<const T2*>(&z);
+    T2 a0 = zero, a1 = zero, a2 = zero, a3 = zero;
+#pragma unroll 8
+    for (int c = lane; c < n; c += 32) {
+        const uint4 v = tile[c];
+        a0 = __hfma2(*reinterpret_cast<const T2*>(&v.x), zero, a0);
+        a1 = __hfma2(*reinterpret_cast<const T2*>(&v.y), zero, a1);
+        a2 = __hfma2(*reinterpret_cast<const T2*>(&v.z), zero, a2);
+        a3 = __hfma2(*reinterpret_cast<const T2*>(&v.w), zero, a3);
+    }
+    const T2 a = __hadd2(__hadd2(a0, a1), __hadd2(a2, a3));
+    return __any_sync(0xffffffffu, !__hbeq2(a, a));
+}
 template <typename T>
 __device__ __forceinline__ uint32_t zero_nonfinite(uint32_t u) {
     constexpr uint32_t kExp = DType<T>::code == LCBSA_BF16 ? 0x7f80u : 0x7c00u;
     if ((u & kExp) == kExp) u &= 0xffff0000u;
     if (((u >> 16) & kExp) == kExp) u &= 0x0000ffffu;
     return u;
+}
+
+// The order of the items of a persistent kernel: waves of `wave` heads, in a wave tile by tile over its heads, so that the tiles with most work
+// can come first and the last items are short.  One wave, unless what the heads stream (bytes each) does not fit the L2 together: then
+// as few waves of as many heads as possible.  37 heads of 4096 tokens, 77 MB of keys and values: dQ 375 us in one wave, 336 us in waves of 10;
+// 16 heads of 8192 tokens, 33 MB, causal: 343 us in one wave, 367 us in waves of 5, whose last one starts its longest items last.
+inline int dense_wave(int heads, double bytes) {
+    const int waves = (int)(heads * bytes / 48e6) + 1;
+    return heads * bytes <= 64e6 ? heads : (heads + waves - 1) / waves;
+}
+__device__ __forceinline__ void dense_item(int idx, int heads, int tiles, int wave, int& bh, int& tile) {
+    const int first = idx / (wave * tiles) * wave, rest = idx % (wave * tiles), n = min(wave, heads - first);
+    tile = rest / n;
+    bh = first + rest % n;
 }
 
 // the plan of a call (dense_plan.cu)

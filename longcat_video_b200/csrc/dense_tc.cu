@@ -2,7 +2,8 @@
 //
 // One persistent CTA per SM; a work item is one tile of 128 queries of one head, and its keys are the union of the runs that its rows
 // see, in units of 64 from the first such key on.  The items are taken off a counter (their lengths are known on the GPU
-// alone), the last queries first, since with a causal order they have most keys; the first warp announces them in a ring.
+// alone), wave by wave of heads and in each the last queries first, since with a causal order they have most keys; one warp announces
+// them in a ring.
 //
 //   warps 0-3, 4-7 : softmax warpgroups 0 and 1 (units of even / odd number; thread = one query row)
 //   warp 8 : items, TMA producer of Q and K   warp 9 : S = Q K^T issuer   warp 10 : O += P V issuer   warp 11: TMA producer of V
@@ -15,8 +16,8 @@
 // functions per score with a cap, which is then what bounds the kernel).
 //
 // Hidden values may be anything.  A score that is not finite stays in its column and is replaced there.  V enters the product of every row
-// of the tile, so in mixed units the issuer of PV looks through the tile first: values that are not finite are set to zero, and the
-// epilogue adds them by hand to the rows that see them.
+// of the tile, so in mixed units its producer looks through the tile first: values that are not finite are set to zero, and the epilogue adds
+// them by hand to the rows that see them.
 //
 // Every wait on an mbarrier is bounded, as in attn_tc.cu.
 #include <type_traits>
@@ -53,10 +54,10 @@ template <int D> struct Lay {
     static constexpr int offV = offK + kKSlots * tile;
     static constexpr int offBar = offV + kVSlots * tile;
     // barriers: k_full[6] k_empty[6] v_full[6] v_empty[6] q_full q_free s_full[2] s_free[2] p_full[2] pv_done[2]
-    //           ml_ready o_free o_staged qt_full qt_free looked item_full[4] item_empty[4]
-    static constexpr int numBars = 2 * kKSlots + 2 * kVSlots + 2 + 8 + 6 + 2 * kItemRing;
+    //           ml_ready o_free o_staged qt_full qt_free looked item_full[4] item_empty[4] v_ok[6]
+    static constexpr int numBars = 2 * kKSlots + 3 * kVSlots + 2 + 8 + 6 + 2 * kItemRing;
     static constexpr int offMisc = offBar + numBars * 8;  // abort flag, TMEM base, whether a mixed unit held values that are not finite
-    static constexpr int offItems = (offMisc + 64 + 31) / 32 * 32;  // [4] Item
+    static constexpr int offItems = (offMisc + 96 + 31) / 32 * 32;  // [4] Item
     static constexpr int offMl = offItems + kItemRing * 32;         // [2 warpgroups][128 lanes] (maximum, row sum)
     static constexpr int smem = offMl + 2 * 128 * 8;
 };
@@ -77,7 +78,7 @@ struct TcParams {
     const void* v;
     long long v_sb, v_sh, v_ss;
     unsigned int* status;
-    int B, Hq, group, Sq, n_u, tiles;
+    int B, Hq, group, Sq, n_u, tiles, wave;
     uint32_t q_sign;        // flips the sign of Q: a negative scale
     ScoreShape shape;       // of the magnitude of the scale
 };
@@ -123,9 +124,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
     const uint32_t bar_qt_full = bar0 + 8u * (kB1 + 3), bar_qt_free = bar0 + 8u * (kB1 + 4), bar_looked = bar0 + 8u * (kB1 + 5);
     auto bar_item_full = [&](unsigned n) { return bar0 + 8u * (kB1 + 6 + n % kItemRing); };
     auto bar_item_empty = [&](unsigned n) { return bar0 + 8u * (kB1 + 6 + kItemRing + n % kItemRing); };
+    auto bar_v_ok = [&](int s) { return bar0 + 8u * (kB1 + 6 + 2 * kItemRing + s); };
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Ly::offMisc);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Ly::offMisc + 32);
     volatile int* found_bad = reinterpret_cast<volatile int*>(smem + Ly::offMisc + 40);
+    volatile int* slot_bad = reinterpret_cast<volatile int*>(smem + Ly::offMisc + 44);  // [6] of the tile in a V slot
     Item* items = reinterpret_cast<Item*>(smem + Ly::offItems);
     float2* ml = reinterpret_cast<float2*>(smem + Ly::offMl);  // [2][128]
     const Ctl ctl{abort_flag, P.status};
@@ -142,6 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
         for (int s = 0; s < kVSlots; ++s) {
             mbar_init(bar_v_full(s), 1);
             mbar_init(bar_v_empty(s), 1);
+            mbar_init(bar_v_ok(s), 1);
         }
         mbar_init(bar_q_full, 1);
         mbar_init(bar_q_free, 1);
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
         const CUtensorMap* const tm = &P.tm_kv[is_k ? 0 : 1];
         const int fold = is_k ? P.fold_k : P.fold_v;
         unsigned gk = 0, wk = 0, nq_issued = 0;  // gk: units requested over the whole kernel
-        int slot = 0;
+        int slot = 0, n_iter_done = 0;  // units of the item requested
         unsigned parity = 1;  // of the wait on an empty slot: the ring starts empty
         bool ok = true;
         auto request_q = [&](const Item& it) {  // Q tile of an item into the Q buffer
@@ -390,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
             it.n = -1;
             it.bh = it.tile = it.key0 = it.all_lo = it.all_hi = 0;
             if (idx < bh_total * P.tiles) {
-                it.tile = P.tiles - 1 - idx / bh_total;
-                it.bh = idx % bh_total;
+                dense_item(idx, bh_total, P.tiles, P.wave, it.bh, it.tile);
+                it.tile = P.tiles - 1 - it.tile;
                 const int4* u = P.seen + ((long long)(it.bh / P.Hq) * P.n_u + 2 * it.tile) * kSeenPitch + kDenseUnit;
                 int4 a = __ldg(u), c = make_int4(0, 0, 0, 0x7fffffff);
                 if (2 * it.tile + 1 < P.n_u) c = __ldg(u + kSeenPitch);
@@ -430,6 +434,28 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
             const int b = cur.bh / P.Hq, h = (cur.bh - b * P.Hq) / P.group;
             const int ch = (fold & 1) ? 0 : h, cb = (fold & 2) ? 0 : b;
             const int n_iter = rounds(cur);
+            // V of mixed units is looked through here, behind the copies: three units later, when it has come, and well before its P.
+            auto look_at = [&](int j) -> bool {
+                const unsigned g = gk - n_iter_done + j;  // number of unit j over the whole kernel
+                const int vs = g % kVSlots;
+                if (j < cur.n && mixed_unit(cur, j)) {
+                    if (!mbar_wait_warp(bar_v_full(vs), (g / kVSlots) & 1, ctl, 24, g)) return false;
+                    unsigned char* const v = smem + Ly::offV + vs * Ly::tile;
+                    const bool bad = tile_nonfinite<T, Ly::tile / 16>(reinterpret_cast<const uint4*>(v), lane);
+                    if (LCBSA_UNLIKELY(bad)) {
+#pragma unroll 1
+                        for (int c = lane; c < Ly::tile / 4; c += 32) {
+                            uint32_t* p = reinterpret_cast<uint32_t*>(v) + c;
+                            *p = zero_nonfinite<T>(*p);
+                        }
+                        fence_proxy_async();
+                    }
+                    if (lane == 0) slot_bad[vs] = bad;
+                    __syncwarp();
+                }
+                mbar_arrive_elect(bar_v_ok(vs));
+                return true;
+            };
             bool q_due = is_k && nx.n >= 0;  // Q of the next item has not been requested yet
 #pragma unroll 1
             for (int j = 0; j < n_iter; ++j) {
@@ -456,11 +482,18 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                     for (int half = 0; half < D / 64; ++half) tma_load_5d_elect(dst + half * Ly::half, tm, bar, 64 * half, cur.key0 + kBlk * j, ch, cb, 0);
                 }
                 ++gk;
+                n_iter_done = j + 1;
                 if (++slot == kKSlots) {
                     slot = 0;
                     parity ^= 1;
                 }
+                if (!is_k && j >= 3) {
+                    ok = look_at(j - 3);
+                    if (!ok) break;
+                }
             }
+            if (!is_k)
+                for (int j = max(n_iter - 3, 0); j < n_iter && ok; ++j) ok = look_at(j);
             cur = nx;
             ++wk;
         }
@@ -544,21 +577,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                     ok = mbar_wait_warp(bar_v_full(slot), (gb / kVSlots) & 1, ctl, 60, gb);
                     if (!ok) break;
                 }
-                if (i < cur.n && mixed_unit(cur, i)) {  // under the softmax of the unit: its P is not there yet
-                    unsigned char* const v = smem + Ly::offV + slot * Ly::tile;
-                    bool bad = false;
-#pragma unroll 8
-                    for (int c = lane; c < Ly::tile / 16; c += 32) bad |= chunk_nonfinite<T>(reinterpret_cast<const uint4*>(v)[c]);
-                    if (LCBSA_UNLIKELY(__any_sync(0xffffffffu, bad))) {
-                        bad_item = 1;
-#pragma unroll 1
-                        for (int c = lane; c < Ly::tile / 4; c += 32) {
-                            uint32_t* p = reinterpret_cast<uint32_t*>(v) + c;
-                            *p = zero_nonfinite<T>(*p);
-                        }
-                        fence_proxy_async();
-                        __syncwarp();
-                    }
+                if (i < cur.n && mixed_unit(cur, i)) {
+                    ok = mbar_wait_warp(bar_v_ok(slot), (gb / kVSlots) & 1, ctl, 62, gb);
+                    if (!ok) break;
+                    bad_item |= slot_bad[slot];
                 }
                 if (i == n_iter - 1) {
                     if (lane == 0) {
@@ -636,28 +658,24 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                     const int key0 = cur.key0 + kBlk * i;
                     // S -> exponents relative to the reference, in place (0 stands in for it until the row has seen a key)
                     const float m_eff = first ? 0.f : m_ref;
-                    float2 step = make_float2(0.f, 0.f), base = make_float2(-m_eff, -m_eff);
-                    bool both_sides = false;
+                    const float2 base = make_float2(-m_eff, -m_eff);
                     const float at = kBias ? (float)(see.z - key0) : 0.f;
-                    if (kBias) {  // keys on one side of the query: the distance is a line in the key's number
-                        const float sl = at >= (float)(kBlk - 1) ? f.slope2 : -f.slope2;
-                        both_sides = __any_sync(0xffffffffu, at > 0.f && at < (float)(kBlk - 1));
-                        step = make_float2(sl, sl);
-                        if (!both_sides) base.x = base.y = fmaf(-sl, at, -m_eff);
-                    }
-                    auto exponents = [&](auto capped, bool two_sides) {
+                    const bool both_sides = kBias && __any_sync(0xffffffffu, at > 0.f && at < (float)(kBlk - 1));
+                    auto exponents = [&](auto shaped, bool two_sides) {
+                        BiasLine line;
+                        if (kBias && !two_sides) line = bias_line(at, f.slope2, -m_eff);
 #pragma unroll
                         for (int j = 0; j < 64; j += 2) {
                             float2 c = base;
                             if (kBias) {
                                 if (two_sides) c = __ffma2_rn(make_float2(fabsf(at - (float)j), fabsf(at - (float)(j + 1))), make_float2(-f.slope2, -f.slope2), base);
-                                else c = __ffma2_rn(make_float2((float)j, (float)(j + 1)), step, base);
+                                else c = bias_next(line, j / 2);
                             }
-                            put2(sr, j, capped(get2(sr, j), c));
+                            put2(sr, j, shaped(get2(sr, j), c));
                         }
                     };
                     if constexpr (kCap) {
-                        const bool large = __any_sync(0xffffffffu, !(fabsf(f.inv) * row_size(sr) <= kCapSmall));
+                        const bool large = __any_sync(0xffffffffu, !(row_size(sr) <= f.s_small));
                         auto any = [&](float2 s, float2 c) { float2 slack; return __fadd2_rn(capped_any(f, s, slack), c); };
                         auto small = [&](float2 s, float2 c) { return capped_small_plus(f, s, c); };
                         if (LCBSA_UNLIKELY(large)) exponents(any, true);
@@ -872,6 +890,7 @@ cudaError_t launch_dense_tc(const DenseArgs& a, cudaStream_t st, const char** wh
     P.status = a.status;
     P.B = a.B; P.Hq = a.Hq; P.group = a.group; P.Sq = a.Sq; P.n_u = dense_units(a.Sq);
     P.tiles = (a.Sq + kQRows - 1) / kQRows;
+    P.wave = dense_wave(a.B * a.Hq, 4.0 * a.Sk * a.D / a.group);
     P.q_sign = a.scale < 0.f ? 0x80008000u : 0u;
     P.shape = score_shape(a.scale < 0.f ? -a.scale : a.scale, a.cap);
     int dev = 0, sm_count = 0;
