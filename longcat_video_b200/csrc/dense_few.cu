@@ -1,13 +1,14 @@
 // Dense attention forward for few queries (see dense_common.cuh for the formulas): a token, or a few drafted ones, of every sequence
 // behind a long cache.  Bound by HBM: each key and value is read once for all queries and all heads that share it.
 //
-// The rows of one 16-row MMA tile are (query, head of the group) pairs, so a group of four heads and one query fill four of
-// them and the cache is still read once.  The keys are split over CTAs in chunks of a fixed number (an even load whatever the
-// lengths; a chunk behind the last key that any row sees ends at once), and inside a CTA over four warps that take every fourth
-// tile of 32 keys: a warp has a ring of its own in shared memory and nothing in the loop waits for another warp.  S, P and O
+// The rows of a CTA's one or two 16-row MMA tiles are (query, head of the group) pairs, so a group of four heads and one query fill
+// four of them and the cache is still read once.  The keys that the rows see are split evenly over the CTAs of a cluster, which join
+// their partial results (fp32, relative to their maxima) through each other's shared memory: one launch, no workspace, one order.
+// Where clusters of eight leave the chip idle and the keys are many, chunks of a fixed number of keys go to CTAs of their own
+// instead, and a second kernel joins partial results from the workspace.  Inside a CTA four warps take every fourth tile of 16
+// (head_dim 64: 32) keys: a warp has a ring of its own in shared memory and nothing in the loop waits for another warp.  S, P and O
 // stay in registers (mma.sync m16n8k16, fp32 accumulators; P is rounded to the input type for the product with V, as in the
-// other attention kernels, the row sum is taken before the rounding); running maximum and sum per row in fp32, merged over the
-// warps through shared memory and over the chunks by a second kernel from fp32 partial results.
+// other attention kernels, the row sum is taken before the rounding); running maximum and sum per row in fp32.
 //
 // Masked places hold anything: keys outside the union of the rows' runs are not loaded, a masked score is replaced (not
 // multiplied), and in a tile that only some rows see the values that are not finite are added by hand to the rows that see
@@ -19,51 +20,83 @@ namespace lcbsa {
 
 namespace {
 
-constexpr int kRows = 16;       // (query, head) rows of a CTA
 constexpr int kFewWarps = 4;
-constexpr int kKeys = 32;       // keys of a warp's tile
-constexpr int kFewStages = 2;
+constexpr int kFewStages = 3;   // tiles of a warp's ring, of K and V each
+template <int D> constexpr int kKeys = D == 64 ? 32 : 16;  // keys of a warp's tile: 4 KB of K and of V
+constexpr int kMaxCluster = 8;  // CTAs of a cluster (16, which have to be asked for, start one after another: 20 us became 32)
 constexpr int kMaxSplits = 256;
+constexpr int few_step(int D) { return kFewWarps * (D == 64 ? 32 : 16); }  // keys of a CTA's round
 
 struct FewParams {
     DenseArgs a;
     ScoreShape shape;
     int rows;               // group * Sq rows of one key head
-    int tiles;              // 16-row tiles of them
-    int splits, chunk;      // chunks of the keys, keys of a chunk
-    float* part_o;          // [B*Hk*rows][splits][D], not yet divided by the row sum; null: one chunk, straight to the output
+    int mt;                 // 16-row tiles of a CTA
+    int tiles;              // CTAs' worth of rows
+    int splits, chunk;      // CTAs that share the keys; chunk: keys of each, 0: a cluster, which splits evenly what its rows see
+    float* part_o;          // [B*Hk*rows][splits][D], not yet divided by the row sum (chunks)
     float2* part_ml;        // [B*Hk*rows][splits]: maximum (log2), row sum
 };
 
-template <int D>
+template <int D, int MT>
 constexpr int few_smem() {
-    return kRows * D * 2 + kFewWarps * kFewStages * 2 * kKeys * D * 2 + kRows * 16;
+    return 16 * MT * D * 2 + kFewWarps * kFewStages * 2 * kKeys<D> * D * 2 + 16 * MT * 16;
 }
 
-// `n` rows of D values from row `first` on into a swizzled tile; rows at `end` or behind are zero
+// rows from `first` on into a swizzled tile; rows at `end` or behind are zero
 template <typename T, int D>
 __device__ __forceinline__ void load_keys(uint32_t tile, const T* head, long long ss, int first, int end, int lane) {
     constexpr int CPR = D * 2 / 16;
 #pragma unroll
-    for (int v = lane; v < kKeys * CPR; v += 32) {
+    for (int v = lane; v < kKeys<D> * CPR; v += 32) {
         const int row = v / CPR, c = v % CPR;
         const bool there = first + row < end;
         mm::cp_async16(tile + row * (D * 2) + ((c ^ (row & 7)) << 4), head + (there ? (long long)(first + row) * ss : 0) + c * 8, there);
     }
 }
 
-template <typename T, int D, bool kCap, bool kBias>
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a float4 of another CTA's shared memory, at the address it has in this one
+__device__ __forceinline__ float4 peer_float4(const void* mine, unsigned rank) {
+    uint32_t at;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mm::smem_u32(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+// Row `row` (of the key head's rows) of the result: n values per lane from column c on
+template <typename T, int n>
+__device__ __forceinline__ void write_row(const DenseArgs& a, int b, int hk, int row, int c, const float* x, float l, float m, int D, bool first_lane) {
+    const int i = row / a.group, h = hk * a.group + row % a.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* dst = static_cast<T*>(const_cast<void*>(a.o.data)) + (long long)b * a.o.sb + (long long)h * a.o.sh + (long long)i * a.o.ss + c;
+    const long long at = ((long long)b * a.Hq + h) * a.Sq + i;
+#pragma unroll
+    for (int e = 0; e < n; ++e) {
+        const float v = x[e] * inv;
+        const T r = DType<T>::from_f32(v);
+        dst[e] = r;
+        if (a.rest != nullptr) static_cast<T*>(a.rest)[at * D + c + e] = DType<T>::from_f32(v - DType<T>::to_f32(r));
+    }
+    if (a.lse != nullptr && first_lane) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <typename T, int D, int MT, bool kCap, bool kBias>
 __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_constant__ FewParams P) {
-    constexpr int kTileBytes = kKeys * D * 2;
+    constexpr int kN = kKeys<D>, kTileBytes = kN * D * 2, kRows = 16 * MT, kStages = kFewStages, kStep = few_step(D);
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* const ring0 = smem + kRows * D * 2;
-    int4* const seen_s = reinterpret_cast<int4*>(ring0 + kFewWarps * kFewStages * 2 * kTileBytes);  // [16] lo, hi, pos
+    int4* const seen_s = reinterpret_cast<int4*>(ring0 + kFewWarps * kStages * 2 * kTileBytes);  // [rows] lo, hi, pos
     const DenseArgs& a = P.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int split = blockIdx.x % P.splits;
-    const unsigned rest = blockIdx.x / P.splits;
-    const int tile = rest % P.tiles;
-    const int bh = rest / P.tiles, b = bh / a.Hk, hk = bh % a.Hk;
+    const int split = blockIdx.x % P.splits;  // in a cluster: the CTA's rank
+    const unsigned others = blockIdx.x / P.splits;
+    const int tile = others % P.tiles;
+    const int bh = others / P.tiles, b = bh / a.Hk, hk = bh % a.Hk;
     const int row0 = tile * kRows;
 
     const T* const qb = static_cast<const T*>(a.q.data) + (long long)b * a.q.sb;
@@ -82,261 +115,295 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
             if (row0 + tid < P.rows) s = dense_seen(a.mask, b, (row0 + tid) / a.group, a.Sq, a.Sk);
             seen_s[tid] = make_int4(s.lo, s.hi, s.pos, 0);
         }
-        mm::cp_async_wait<0>();
         __syncthreads();
     }
-    // union of the rows' runs, and the run that all rows see
+    // union of the rows' runs, and the run that all rows see (rows that do not exist are masked out, nothing more)
     int u_lo = 0x7fffffff, u_hi = 0, all_lo = 0, all_hi = 0x7fffffff;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
+    for (int r = lane; r < kRows && row0 + r < P.rows; r += 32) {
         const int4 s = seen_s[r];
-        if (row0 + r >= P.rows) continue;
         if (s.x < s.y) {
-            u_lo = min(u_lo, s.x);
-            u_hi = max(u_hi, s.y);
-            all_lo = max(all_lo, s.x);
-            all_hi = min(all_hi, s.y);
+            u_lo = s.x;
+            u_hi = s.y;
+            all_lo = s.x;
+            all_hi = s.y;
         } else {
             all_hi = 0;
         }
     }
-    const long long c_lo = (long long)u_lo + (long long)split * P.chunk;
-    const int first = (int)min(c_lo, (long long)u_hi), end = (int)min(c_lo + P.chunk, (long long)u_hi);  // keys of this chunk
-    const int n_tiles = end > first ? (end - first + kKeys - 1) / kKeys : 0;
-
-    const int ra = lane >> 2, rb = ra + 8;  // the thread's two rows
-    const int4 sa = seen_s[ra], sb = seen_s[rb];
-    float slope_a = 0.f, slope_b = 0.f;
-    if (kBias) {
-        if (row0 + ra < P.rows) slope_a = __ldg(a.slopes + hk * a.group + (row0 + ra) % a.group) * kLog2e;
-        if (row0 + rb < P.rows) slope_b = __ldg(a.slopes + hk * a.group + (row0 + rb) % a.group) * kLog2e;
-    }
-
-    float o[D / 8][4];
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
+    u_lo = __reduce_min_sync(0xffffffffu, u_lo);
+    u_hi = __reduce_max_sync(0xffffffffu, u_hi);
+    all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+    all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+    int chunk = P.chunk;
+    if (chunk == 0) chunk = u_hi > u_lo ? ((u_hi - u_lo + P.splits - 1) / P.splits + kStep - 1) / kStep * kStep : kStep;
+    const long long c_lo = (long long)u_lo + (long long)split * chunk;
+    const int first = (int)min(c_lo, (long long)u_hi), end = (int)min(c_lo + chunk, (long long)u_hi);  // keys of this CTA
+    const int n_tiles = end > first ? (end - first + kN - 1) / kN : 0;
 
     const T* const kh = static_cast<const T*>(a.k.data) + (long long)b * a.k.sb + (long long)hk * a.k.sh;
     const T* const vh = static_cast<const T*>(a.v.data) + (long long)b * a.v.sb + (long long)hk * a.v.sh;
-    unsigned char* const ring = ring0 + warp * kFewStages * 2 * kTileBytes;
+    unsigned char* const ring = ring0 + warp * kStages * 2 * kTileBytes;
     auto request = [&](int t, int slot) {
-        const uint32_t dst = mm::smem_u32(ring) + slot * 2 * kTileBytes;
-        load_keys<T, D>(dst, kh, a.k.ss, first + t * kKeys, end, lane);
-        load_keys<T, D>(dst + kTileBytes, vh, a.v.ss, first + t * kKeys, end, lane);
-    };
-    if (warp < n_tiles) request(warp, 0);
-    mm::cp_async_commit();
-
-    uint32_t qf[D / 16][4];
-    {
-        const int row = lane & 15;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            const int c = 2 * ks + (lane >> 4);
-            mm::ldsm_x4(qf[ks], mm::smem_u32(smem) + row * (D * 2) + ((c ^ (row & 7)) << 4));
+        if (t < n_tiles) {
+            const uint32_t dst = mm::smem_u32(ring) + slot * 2 * kTileBytes;
+            load_keys<T, D>(dst, kh, a.k.ss, first + t * kN, end, lane);
+            load_keys<T, D>(dst + kTileBytes, vh, a.v.ss, first + t * kN, end, lane);
         }
+        mm::cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i + 1 < kStages; ++i) request(warp + i * kFewWarps, i);
+    mm::cp_async_wait<kStages - 1>();  // the queries
+    __syncthreads();
+
+    // the thread's rows: lane / 4 + 8 k of the tiles, k = 0 .. 2 MT - 1
+    constexpr int kMine = 2 * MT;
+    int4 see[kMine];
+    float slope[kMine], m[kMine], l[kMine];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+        const int r = (lane >> 2) + 8 * k;
+        see[k] = seen_s[r];
+        slope[k] = kBias && row0 + r < P.rows ? __ldg(a.slopes + hk * a.group + (row0 + r) % a.group) * kLog2e : 0.f;
+        m[k] = -INFINITY;
+        l[k] = 0.f;
+    }
+    float o[MT][D / 8][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+    // the queries' fragments: in registers for one tile, read again for every tile of keys for two
+    uint32_t qf[MT == 1 ? D / 16 : 1][4];
+    auto load_q = [&](int t, int ks, uint32_t (&f)[4]) {
+        const int row = 16 * t + (lane & 15), c = 2 * ks + (lane >> 4);
+        mm::ldsm_x4(f, mm::smem_u32(smem) + row * (D * 2) + ((c ^ (row & 7)) << 4));
+    };
+    if (MT == 1) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) load_q(0, ks, qf[MT == 1 ? ks : 0]);
     }
 
     int slot = 0;
-    for (int t = warp; t < n_tiles; t += kFewWarps, slot ^= 1) {
-        if (t + kFewWarps < n_tiles) request(t + kFewWarps, slot ^ 1);
-        mm::cp_async_commit();
-        mm::cp_async_wait<1>();
+    for (int t = warp; t < n_tiles; t += kFewWarps) {
+        request(t + (kStages - 1) * kFewWarps, slot >= 1 ? slot - 1 : kStages - 1);
+        mm::cp_async_wait<kStages - 1>();
         __syncwarp();
         unsigned char* const v_ptr = ring + slot * 2 * kTileBytes + kTileBytes;
         const uint32_t kt = mm::smem_u32(ring) + slot * 2 * kTileBytes, vt = kt + kTileBytes;
-        const int key0 = first + t * kKeys;
-        const bool mixed = key0 < all_lo || min(key0 + kKeys, end) > all_hi || key0 + kKeys > end;
+        const int key0 = first + t * kN;
+        const bool mixed = key0 < all_lo || min(key0 + kN, end) > all_hi || key0 + kN > end;
 
-        float s[4][4];
+        float s[MT][kN / 8][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        for (int q = 0; q < MT; ++q)
+#pragma unroll
+            for (int i = 0; i < kN / 8; ++i) s[q][i][0] = s[q][i][1] = s[q][i][2] = s[q][i][3] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t af[MT][4];
 #pragma unroll
-            for (int np = 0; np < 2; ++np) {
-                const int mid = lane >> 3;
-                const int row = np * 16 + (lane & 7) + (mid >> 1) * 8;
-                const int c = 2 * ks + (mid & 1);
+            for (int q = 0; q < MT; ++q) {
+                if (MT > 1) load_q(q, ks, af[q]);
+            }
+#pragma unroll
+            for (int np = 0; np < kN / 16; ++np) {
+                const int mid = lane >> 3, row = np * 16 + (lane & 7) + (mid >> 1) * 8, c = 2 * ks + (mid & 1);
                 uint32_t bf[4];
                 mm::ldsm_x4(bf, kt + row * (D * 2) + ((c ^ (row & 7)) << 4));
-                mm::mma16816<T>(s[2 * np], qf[ks], bf[0], bf[1]);
-                mm::mma16816<T>(s[2 * np + 1], qf[ks], bf[2], bf[3]);
+#pragma unroll
+                for (int q = 0; q < MT; ++q) {
+                    const uint32_t(&f)[4] = MT == 1 ? qf[MT == 1 ? ks : 0] : af[q];
+                    mm::mma16816<T>(s[q][2 * np], f, bf[0], bf[1]);
+                    mm::mma16816<T>(s[q][2 * np + 1], f, bf[2], bf[3]);
+                }
             }
         }
-        float top_a = -INFINITY, top_b = -INFINITY;
+        float top[kMine];  // of this thread's scores
+        bool moved = false;
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
+        for (int k = 0; k < kMine; ++k) {
+            const int q = k >> 1, e0 = 2 * (k & 1);  // row k's values: s[q][nt][e0], s[q][nt][e0 + 1]
+            top[k] = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int j = key0 + nt * 8 + 2 * (lane & 3) + e;
-                float2 x = make_float2(s[nt][e], s[nt][2 + e]), slack;
+            for (int nt = 0; nt < kN / 8; ++nt) {
+                const int j = key0 + nt * 8 + 2 * (lane & 3);
+                float2 x = make_float2(s[q][nt][e0], s[q][nt][e0 + 1]), slack;
                 if (kCap) x = capped_any(P.shape, x, slack);
                 else x = make_float2(x.x * P.shape.mul, x.y * P.shape.mul);
-                float xa = x.x, xb = x.y;
                 if (kBias) {
-                    xa = fmaf(-slope_a, fabsf((float)(sa.z - j)), xa);
-                    xb = fmaf(-slope_b, fabsf((float)(sb.z - j)), xb);
+                    x.x = fmaf(-slope[k], fabsf((float)(see[k].z - j)), x.x);
+                    x.y = fmaf(-slope[k], fabsf((float)(see[k].z - j - 1)), x.y);
                 }
                 if (mixed) {
-                    if (j < sa.x || j >= min(sa.y, end)) xa = -INFINITY;
-                    if (j < sb.x || j >= min(sb.y, end)) xb = -INFINITY;
+                    const int hi = min(see[k].y, end);
+                    if (j < see[k].x || j >= hi) x.x = -INFINITY;
+                    if (j + 1 < see[k].x || j + 1 >= hi) x.y = -INFINITY;
                 }
-                s[nt][e] = xa;
-                s[nt][2 + e] = xb;
-                top_a = fmaxf(top_a, xa);
-                top_b = fmaxf(top_b, xb);
+                s[q][nt][e0] = x.x;
+                s[q][nt][e0 + 1] = x.y;
+                top[k] = fmaxf(top[k], fmaxf(x.x, x.y));
+            }
+            moved |= top[k] > m[k] + 8.f;
+        }
+        // The rows' references move only when a score is more than 2^8 above one (or the first that is seen): the maximum over the four
+        // threads of a row, the sums and the accumulators are only touched then.
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int k = 0; k < kMine; ++k) {
+                float n = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+                n = fmaxf(m[k], fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 2)));
+                const float alpha = dense_ex2(m[k] - (n == -INFINITY ? 0.f : n));
+                m[k] = n;
+                l[k] *= alpha;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    o[k >> 1][i][2 * (k & 1)] *= alpha;
+                    o[k >> 1][i][2 * (k & 1) + 1] *= alpha;
+                }
             }
         }
 #pragma unroll
-        for (int x = 1; x <= 2; x <<= 1) {
-            top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, x));
-            top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, x));
-        }
-        const float n_a = fmaxf(m_a, top_a), n_b = fmaxf(m_b, top_b);
-        const float base_a = n_a == -INFINITY ? 0.f : n_a, base_b = n_b == -INFINITY ? 0.f : n_b;
-        const float al_a = dense_ex2(m_a - base_a), al_b = dense_ex2(m_b - base_b);
-        m_a = n_a;
-        m_b = n_b;
-        float sum_a = 0.f, sum_b = 0.f;
+        for (int k = 0; k < kMine; ++k) {
+            const int q = k >> 1, e0 = 2 * (k & 1);
+            const float base = m[k] == -INFINITY ? 0.f : m[k];
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                s[nt][e] = dense_ex2(s[nt][e] - base_a);
-                s[nt][2 + e] = dense_ex2(s[nt][2 + e] - base_b);
-                sum_a += s[nt][e];
-                sum_b += s[nt][2 + e];
+            for (int nt = 0; nt < kN / 8; ++nt) {
+                s[q][nt][e0] = dense_ex2(s[q][nt][e0] - base);
+                s[q][nt][e0 + 1] = dense_ex2(s[q][nt][e0 + 1] - base);
+                l[k] += s[q][nt][e0] + s[q][nt][e0 + 1];  // this thread's keys; added up over the four threads of a row at the end
             }
         }
-        l_a = l_a * al_a + sum_a;  // this thread's keys; added up over the four threads of a row at the end
-        l_b = l_b * al_b + sum_b;
-        if (__any_sync(0xffffffffu, al_a != 1.f || al_b != 1.f)) {
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                o[i][0] *= al_a;
-                o[i][1] *= al_a;
-                o[i][2] *= al_b;
-                o[i][3] *= al_b;
-            }
-        }
-        if (mixed) {
-            bool bad = false;
-#pragma unroll 4
-            for (int v = lane; v < kTileBytes / 16; v += 32) bad |= chunk_nonfinite<T>(*reinterpret_cast<const uint4*>(v_ptr + 16 * v));
-            if (__any_sync(0xffffffffu, bad)) {
+        if (mixed && tile_nonfinite<T, kTileBytes / 16>(reinterpret_cast<const uint4*>(v_ptr), lane)) {
 #pragma unroll 1
-                for (int r = 0; r < kKeys; ++r) {
-                    const int j = key0 + r;
-                    const bool ga = j >= sa.x && j < min(sa.y, end), gb = j >= sb.x && j < min(sb.y, end);
+            for (int r = 0; r < kN; ++r) {
+                const int j = key0 + r;
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        const T* p = reinterpret_cast<const T*>(v_ptr + r * (D * 2) + ((i ^ (r & 7)) << 4)) + 2 * (lane & 3);
-                        const float x0 = DType<T>::to_f32(p[0]), x1 = DType<T>::to_f32(p[1]);
-                        if (!isfinite(x0)) {
-                            if (ga) o[i][0] += x0;
-                            if (gb) o[i][2] += x0;
-                        }
-                        if (!isfinite(x1)) {
-                            if (ga) o[i][1] += x1;
-                            if (gb) o[i][3] += x1;
-                        }
+                for (int i = 0; i < D / 8; ++i) {
+                    const T* p = reinterpret_cast<const T*>(v_ptr + r * (D * 2) + ((i ^ (r & 7)) << 4)) + 2 * (lane & 3);
+                    const float x0 = DType<T>::to_f32(p[0]), x1 = DType<T>::to_f32(p[1]);
+#pragma unroll
+                    for (int k = 0; k < kMine; ++k) {
+                        const bool sees = j >= see[k].x && j < min(see[k].y, end);
+                        if (sees && !isfinite(x0)) o[k >> 1][i][2 * (k & 1)] += x0;
+                        if (sees && !isfinite(x1)) o[k >> 1][i][2 * (k & 1) + 1] += x1;
                     }
                 }
-                __syncwarp();
-                for (int v = lane; v < kTileBytes / 4; v += 32) {
-                    uint32_t* p = reinterpret_cast<uint32_t*>(v_ptr) + v;
-                    *p = zero_nonfinite<T>(*p);
-                }
-                __syncwarp();
             }
+            __syncwarp();
+            for (int v = lane; v < kTileBytes / 4; v += 32) {
+                uint32_t* p = reinterpret_cast<uint32_t*>(v_ptr) + v;
+                *p = zero_nonfinite<T>(*p);
+            }
+            __syncwarp();
         }
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            uint32_t pa[4];
-            pa[0] = mm::pack2(T(), s[2 * kk][0], s[2 * kk][1]);
-            pa[1] = mm::pack2(T(), s[2 * kk][2], s[2 * kk][3]);
-            pa[2] = mm::pack2(T(), s[2 * kk + 1][0], s[2 * kk + 1][1]);
-            pa[3] = mm::pack2(T(), s[2 * kk + 1][2], s[2 * kk + 1][3]);
+        for (int kk = 0; kk < kN / 16; ++kk) {
+            uint32_t pa[MT][4];
+#pragma unroll
+            for (int q = 0; q < MT; ++q) {
+                pa[q][0] = mm::pack2(T(), s[q][2 * kk][0], s[q][2 * kk][1]);
+                pa[q][1] = mm::pack2(T(), s[q][2 * kk][2], s[q][2 * kk][3]);
+                pa[q][2] = mm::pack2(T(), s[q][2 * kk + 1][0], s[q][2 * kk + 1][1]);
+                pa[q][3] = mm::pack2(T(), s[q][2 * kk + 1][2], s[q][2 * kk + 1][3]);
+            }
 #pragma unroll
             for (int dp = 0; dp < D / 16; ++dp) {
-                const int mid = lane >> 3;
-                const int row = kk * 16 + (lane & 7) + (mid & 1) * 8;
-                const int c = 2 * dp + (mid >> 1);
+                const int mid = lane >> 3, row = kk * 16 + (lane & 7) + (mid & 1) * 8, c = 2 * dp + (mid >> 1);
                 uint32_t bf[4];
                 mm::ldsm_x4_t(bf, vt + row * (D * 2) + ((c ^ (row & 7)) << 4));
-                mm::mma16816<T>(o[2 * dp], pa, bf[0], bf[1]);
-                mm::mma16816<T>(o[2 * dp + 1], pa, bf[2], bf[3]);
+#pragma unroll
+                for (int q = 0; q < MT; ++q) {
+                    mm::mma16816<T>(o[q][2 * dp], pa[q], bf[0], bf[1]);
+                    mm::mma16816<T>(o[q][2 * dp + 1], pa[q], bf[2], bf[3]);
+                }
             }
         }
         __syncwarp();  // all lanes are through with the slot that the next round's request overwrites
+        if (++slot == kStages) slot = 0;
     }
     mm::cp_async_wait<0>();
 #pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
-        l_a += __shfl_xor_sync(0xffffffffu, l_a, x);
-        l_b += __shfl_xor_sync(0xffffffffu, l_b, x);
+    for (int k = 0; k < kMine; ++k) {
+        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
+        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
     }
 
-    // ---- merge of the four warps: their accumulators in the ring, [warp][16][D + 4] fp32, and (m, l) behind them
+    // ---- join of the four warps: their accumulators in the ring, [warp][rows][D + 4] fp32, and (m, l) behind them
     __syncthreads();
     constexpr int kPitch = D + 4;
     float* const acc_s = reinterpret_cast<float*>(ring0);
     float2* const ml_s = reinterpret_cast<float2*>(ring0 + kFewWarps * kRows * kPitch * 4);
-    static_assert(kFewWarps * kRows * kPitch * 4 + kFewWarps * kRows * 8 <= kFewWarps * kFewStages * 2 * kTileBytes, "the merge fits the ring");
+    static_assert(kFewWarps * kRows * kPitch * 4 + kFewWarps * kRows * 8 <= kFewWarps * kStages * 2 * kTileBytes, "the join fits the ring");
     {
         float* const mine = acc_s + warp * kRows * kPitch;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            const int col = i * 8 + 2 * (lane & 3);
-            *reinterpret_cast<float2*>(mine + ra * kPitch + col) = make_float2(o[i][0], o[i][1]);
-            *reinterpret_cast<float2*>(mine + rb * kPitch + col) = make_float2(o[i][2], o[i][3]);
-        }
-        if ((lane & 3) == 0) {
-            ml_s[warp * kRows + ra] = make_float2(m_a, l_a);
-            ml_s[warp * kRows + rb] = make_float2(m_b, l_b);
+        for (int k = 0; k < kMine; ++k) {
+            const int r = (lane >> 2) + 8 * k;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+                *reinterpret_cast<float2*>(mine + r * kPitch + i * 8 + 2 * (lane & 3)) = make_float2(o[k >> 1][i][2 * (k & 1)], o[k >> 1][i][2 * (k & 1) + 1]);
+            if ((lane & 3) == 0) ml_s[warp * kRows + r] = make_float2(m[k], l[k]);
         }
     }
     __syncthreads();
     constexpr int kPer = D / 32;  // values of a lane, a warp takes rows warp, warp + 4, ...
+    const bool cluster = P.chunk == 0 && P.splits > 1;
     for (int r = warp; r < kRows && row0 + r < P.rows; r += kFewWarps) {
-        float m = -INFINITY;
+        float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, ml_s[w * kRows + r].x);
-        const float base = m == -INFINITY ? 0.f : m;
-        float l = 0.f, x[kPer];
+        for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, ml_s[w * kRows + r].x);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, x[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) x[e] = 0.f;
 #pragma unroll
         for (int w = 0; w < kFewWarps; ++w) {
             const float2 ml = ml_s[w * kRows + r];
             const float f = dense_ex2(ml.x - base);
-            l += ml.y * f;
+            sum += ml.y * f;
             const float* src = acc_s + (w * kRows + r) * kPitch + lane * kPer;
 #pragma unroll
             for (int e = 0; e < kPer; ++e) x[e] += src[e] * f;
         }
-        const long long gr = (long long)bh * P.rows + row0 + r;
-        if (P.part_o != nullptr) {
+        if (cluster) {  // the CTA's result of the row takes the place of the first warp's
+            float* dst = acc_s + r * kPitch + lane * kPer;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) dst[e] = x[e];
+            __syncwarp();
+            if (lane == 0) *reinterpret_cast<float2*>(acc_s + r * kPitch + D) = make_float2(top, sum);
+        } else if (P.part_o != nullptr) {
+            const long long gr = (long long)bh * P.rows + row0 + r;
             float* dst = P.part_o + (gr * P.splits + split) * D + lane * kPer;
 #pragma unroll
             for (int e = 0; e < kPer; ++e) dst[e] = x[e];
-            if (lane == 0) P.part_ml[gr * P.splits + split] = make_float2(m, l);
+            if (lane == 0) P.part_ml[gr * P.splits + split] = make_float2(top, sum);
         } else {
-            const int i = (row0 + r) / a.group, h = hk * a.group + (row0 + r) % a.group;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            T* dst = static_cast<T*>(const_cast<void*>(a.o.data)) + (long long)b * a.o.sb + (long long)h * a.o.sh + (long long)i * a.o.ss + lane * kPer;
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const float v = x[e] * inv;
-                dst[e] = DType<T>::from_f32(v);
-                if (a.rest != nullptr)
-                    static_cast<T*>(a.rest)[(((long long)b * a.Hq + h) * a.Sq + i) * D + lane * kPer + e] = DType<T>::from_f32(v - DType<T>::to_f32(dst[e]));
-            }
-            if (a.lse != nullptr && lane == 0) a.lse[((long long)b * a.Hq + h) * a.Sq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+            write_row<T, kPer>(a, b, hk, row0 + r, lane * kPer, x, sum, top, D, lane == 0);
         }
     }
+    if (!cluster) return;
+    // ---- join of the cluster: CTA c takes rows c, c + splits, ..., D / 4 lanes a row
+    cluster_sync();
+    constexpr int kLanes = D / 4, kAtOnce = kFewWarps * 32 / kLanes;
+    const int c4 = tid % kLanes;
+    for (int r = split + P.splits * (tid / kLanes); r < kRows && row0 + r < P.rows; r += P.splits * kAtOnce) {
+        float top = -INFINITY;
+        for (int c = 0; c < P.splits; ++c) top = fmaxf(top, peer_float4(acc_s + r * kPitch + D, c).x);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < P.splits; ++c) {
+            const float4 ml = peer_float4(acc_s + r * kPitch + D, c), v = peer_float4(acc_s + r * kPitch + 4 * c4, c);
+            const float f = dense_ex2(ml.x - base);
+            sum += ml.y * f;
+            x[0] += v.x * f;
+            x[1] += v.y * f;
+            x[2] += v.z * f;
+            x[3] += v.w * f;
+        }
+        write_row<T, 4>(a, b, hk, row0 + r, 4 * c4, x, sum, top, D, c4 == 0);
+    }
+    cluster_sync();  // nobody leaves while another CTA reads its shared memory
 }
 
 // One warp per row: the chunks' partial results, relative to the row's maximum, in ascending order.
@@ -365,63 +432,71 @@ __global__ void __launch_bounds__(128) dense_combine_kernel(const __grid_constan
 #pragma unroll
         for (int e = 0; e < kPer; ++e) acc[e] += src[e] * f;
     }
-    const int bh = (int)(gr / P.rows), row = (int)(gr % P.rows);
-    const int b = bh / a.Hk, h = bh % a.Hk * a.group + row % a.group, i = row / a.group;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* dst = static_cast<T*>(const_cast<void*>(a.o.data)) + (long long)b * a.o.sb + (long long)h * a.o.sh + (long long)i * a.o.ss + lane * kPer;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const float v = acc[e] * inv;
-        dst[e] = DType<T>::from_f32(v);
-        if (a.rest != nullptr)
-            static_cast<T*>(a.rest)[(((long long)b * a.Hq + h) * a.Sq + i) * D + lane * kPer + e] = DType<T>::from_f32(v - DType<T>::to_f32(dst[e]));
-    }
-    if (a.lse != nullptr && lane == 0) a.lse[((long long)b * a.Hq + h) * a.Sq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+    const int bh = (int)(gr / P.rows);
+    write_row<T, kPer>(a, bh / a.Hk, bh % a.Hk, (int)(gr % P.rows), lane * kPer, acc, l, m, D, lane == 0);
 }
 
-// Chunks: about eight CTAs for every SM, none below 128 keys (a tile for each of the four warps).
+// How the keys are shared out.
 void few_plan(const DenseArgs& a, FewParams& P) {
+    const int kStep = few_step(a.D);
     P.rows = a.group * a.Sq;
-    P.tiles = (P.rows + kRows - 1) / kRows;
+    P.mt = P.rows <= 16 ? 1 : 2;
+    P.tiles = (P.rows + 16 * P.mt - 1) / (16 * P.mt);
     const long long units = (long long)a.B * a.Hk * P.tiles;
-    long long splits = (148 * 8 + units - 1) / (units > 0 ? units : 1);
-    const long long most = (a.Sk + 127) / 128;
+    P.chunk = 0;
+    P.splits = 1;
+    while (P.splits < kMaxCluster && units * P.splits < 148 * 8 && P.splits * kStep < a.Sk) P.splits *= 2;
+    if (units * P.splits >= 148 || a.Sk <= kMaxCluster * 16 * kStep) return;
+    // clusters leave SMs idle, with more than 16 rounds to a CTA: chunks, some four for every SM
+    long long splits = (148 * 4 + units - 1) / (units > 0 ? units : 1);
+    const long long most = (a.Sk + 2 * kStep - 1) / (2 * kStep);
     splits = splits < most ? splits : most;
     splits = splits < kMaxSplits ? splits : kMaxSplits;
-    if (splits < 1) splits = 1;
-    P.chunk = (int)(((a.Sk + splits - 1) / splits + 127) / 128 * 128);
-    if (P.chunk < 128) P.chunk = 128;
-    P.splits = a.Sk > 0 ? (int)((a.Sk + P.chunk - 1) / P.chunk) : 1;
+    P.chunk = (int)(((a.Sk + splits - 1) / splits + kStep - 1) / kStep * kStep);
+    P.splits = (int)((a.Sk + P.chunk - 1) / P.chunk);
 }
 
-template <typename T, int D, bool kCap, bool kBias>
+template <typename T, int D, int MT, bool kCap, bool kBias>
 cudaError_t few_launch(const FewParams& P, cudaStream_t st) {
     const DenseArgs& a = P.a;
+    auto kern = dense_few_kernel<T, D, MT, kCap, kBias>;
     static thread_local unsigned long long raised = 0;  // devices (below 64) whose shared-memory limit this thread has raised for this kernel
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev > 63 || !((raised >> dev) & 1)) {
-        e = cudaFuncSetAttribute(dense_few_kernel<T, D, kCap, kBias>, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem<D>());
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem<D, MT>());
         if (e != cudaSuccess) return e;
         if (dev <= 63) raised |= 1ull << dev;
     }
     const long long ctas = (long long)a.B * a.Hk * P.tiles * P.splits;
     if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-    dense_few_kernel<T, D, kCap, kBias><<<(unsigned)ctas, kFewWarps * 32, few_smem<D>(), st>>>(P);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kFewWarps * 32);
+    cfg.dynamicSmemBytes = few_smem<D, MT>();
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = P.chunk == 0 ? P.splits : 1;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = P.chunk == 0 && P.splits > 1 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kern, P);
     if (e != cudaSuccess || P.part_o == nullptr) return e;
     const long long rows = (long long)a.B * a.Hk * P.rows;
     dense_combine_kernel<T, D><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(P);
     return cudaGetLastError();
 }
 
-template <typename T, int D>
+template <typename T, int D, int MT>
 cudaError_t few_shape(const FewParams& P, cudaStream_t st) {
     const bool cap = P.a.cap > 0.f, bias = P.a.slopes != nullptr;
-    if (cap) return bias ? few_launch<T, D, true, true>(P, st) : few_launch<T, D, true, false>(P, st);
-    return bias ? few_launch<T, D, false, true>(P, st) : few_launch<T, D, false, false>(P, st);
+    if (cap) return bias ? few_launch<T, D, MT, true, true>(P, st) : few_launch<T, D, MT, true, false>(P, st);
+    return bias ? few_launch<T, D, MT, false, true>(P, st) : few_launch<T, D, MT, false, false>(P, st);
 }
+template <typename T, int D>
+cudaError_t few_rows(const FewParams& P, cudaStream_t st) { return P.mt == 1 ? few_shape<T, D, 1>(P, st) : few_shape<T, D, 2>(P, st); }
 
 }  // namespace
 
@@ -439,7 +514,7 @@ size_t dense_fwd_workspace_bytes(const DenseArgs& a) {
     FewParams P;
     few_plan(a, P);
     const size_t plan = few_queries(a) ? 0 : dense_plan_bytes(a, false);
-    if (P.splits == 1) return plan;
+    if (P.chunk == 0) return plan;
     const size_t few = (size_t)a.B * a.Hk * P.rows * P.splits * (a.D + 2) * 4;
     return few > plan ? few : plan;
 }
@@ -457,13 +532,13 @@ cudaError_t launch_dense_fwd(DenseArgs a, void* workspace, cudaStream_t st, cons
     few_plan(a, P);
     P.part_o = nullptr;
     P.part_ml = nullptr;
-    if (P.splits > 1) {
+    if (P.chunk > 0) {
         P.part_o = static_cast<float*>(workspace);
         P.part_ml = reinterpret_cast<float2*>(P.part_o + (long long)a.B * a.Hk * P.rows * P.splits * a.D);
     }
     const cudaError_t e = a.dtype == LCBSA_BF16
-                              ? (a.D == 128 ? few_shape<__nv_bfloat16, 128>(P, st) : few_shape<__nv_bfloat16, 64>(P, st))
-                              : (a.D == 128 ? few_shape<__half, 128>(P, st) : few_shape<__half, 64>(P, st));
+                              ? (a.D == 128 ? few_rows<__nv_bfloat16, 128>(P, st) : few_rows<__nv_bfloat16, 64>(P, st))
+                              : (a.D == 128 ? few_rows<__half, 128>(P, st) : few_rows<__half, 64>(P, st));
     if (e == cudaErrorInvalidConfiguration) *why = "more CTAs than a launch takes";
     return e;
 }
