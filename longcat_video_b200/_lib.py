@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.util
 import os
 import struct
 from typing import Sequence
@@ -101,11 +102,12 @@ SIGNATURES = {
     "lcbsa_rope_table_floats": (ctypes.c_size_t, [_P(LcbsaGrid), ctypes.c_int]),
     "lcbsa_norm_rope": (ctypes.c_int, [_P(LcbsaTensor), ctypes.c_void_p, _P(LcbsaGrid), ctypes.c_void_p, ctypes.c_float,
                                        _P(LcbsaTensor), ctypes.c_void_p]),
-    # tensors and scores as plain pointers: packed_rows() hands over bytes, which ctypes passes without a copy
-    "lcbsa_dense_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int]),
-    "lcbsa_dense_attn_fwd": (ctypes.c_int, [ctypes.c_void_p] * 8 + [ctypes.c_size_t, ctypes.c_void_p]),
-    "lcbsa_dense_attn_bwd": (ctypes.c_int, [ctypes.c_void_p] * 12 + [ctypes.c_size_t, ctypes.c_void_p]),
-    "lcbsa_rotary": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, _P(ctypes.c_uint64), ctypes.c_int, ctypes.c_int, ctypes.c_int,
+    "lcbsa_dense_attn_workspace_bytes": (ctypes.c_size_t, [_P(LcbsaTensor), _P(LcbsaTensor), ctypes.c_int]),
+    "lcbsa_dense_attn_fwd": (ctypes.c_int, [_P(LcbsaTensor)] * 3 + [_P(LcbsaScores), _P(LcbsaTensor)] + [ctypes.c_void_p] * 3
+                             + [ctypes.c_size_t, ctypes.c_void_p]),
+    "lcbsa_dense_attn_bwd": (ctypes.c_int, [_P(LcbsaTensor)] * 5 + [_P(LcbsaScores), ctypes.c_void_p, ctypes.c_void_p]
+                             + [_P(LcbsaTensor)] * 3 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "lcbsa_rotary": (ctypes.c_int, [_P(LcbsaTensor), _P(LcbsaTensor), ctypes.c_int, _P(ctypes.c_uint64), ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                     ctypes.c_float, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]),
     "lcbsa_copy_slabs": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p]),
     "lcbsa_check_device_status": (ctypes.c_int, []),
@@ -126,6 +128,23 @@ def lib() -> ctypes.CDLL:
             fn.restype, fn.argtypes = res, args
         _lib = handle
     return _lib
+
+
+_binding = None
+
+
+def binding():
+    """The Python functions of ``csrc/binding.cpp``, over the liblcbsa.so next to them; raises if it has not been built."""
+    global _binding
+    if _binding is None:
+        path = os.path.join(_HERE, "csrc", "_binding.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python -m longcat_video_b200.build`")
+        lib()
+        spec = importlib.util.spec_from_file_location("_binding", path)
+        _binding = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_binding)
+    return _binding
 
 
 def check(code: int) -> None:
@@ -152,17 +171,6 @@ def tensor_desc(t: torch.Tensor) -> LcbsaTensor:
         raise RuntimeError("lcbsa runs on CUDA tensors only (there is no CPU path)")
     # one packed write instead of ten attribute stores (6 us a descriptor, six descriptors a call)
     return LcbsaTensor.from_buffer_copy(_PACK_TENSOR(t.data_ptr(), dtype_code(t.dtype), 0, *t.shape, *t.stride()))
-
-
-def packed_rows(t: torch.Tensor):
-    """A bf16 / fp16 ``[B,H,S,D]`` CUDA tensor for the entry points whose tensors are typed as plain pointers: (the tensor, made contiguous
-    where the 16-byte rules or a missing stride along S ask for it; the bytes of its LcbsaTensor).  One call where abi_ok and
-    tensor_desc are two: the smallest calls spend their time here."""
-    s0, s1, s2, s3 = t.stride()
-    if s3 != 1 or (s0 | s1 | s2) & 7 or t.data_ptr() & 15 or (s2 == 0 and t.shape[2] > 1):
-        t = t.contiguous()
-        s0, s1, s2, s3 = t.stride()
-    return t, _PACK_TENSOR(t.data_ptr(), dtype_code(t.dtype), 0, *t.shape, s0, s1, s2, s3)
 
 
 def grid_desc(latent_shape: Sequence[int], chunk: Sequence[int]) -> LcbsaGrid:

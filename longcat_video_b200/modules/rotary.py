@@ -30,6 +30,7 @@ class RotaryFrequencies:
         if not all(math.isfinite(f) for f in self.radians) or not math.isfinite(self.factor):
             raise ValueError("frequencies and factor must be finite")
         self.turns = (ctypes.c_uint64 * self.pairs)(*(round(Fraction(f) / (2 * _PI) * 2 ** 64) % 2 ** 64 for f in self.radians))
+        self.address = ctypes.addressof(self.turns)
 
 
 _KINDS = {"linear": {"factor"}, "base": {"factor"}, "by_parts": {"factor", "original_length", "fast", "slow", "attention_factor"},
@@ -91,44 +92,6 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     return _frequencies(int(rotary_dim), float(base), tuple(sorted((scaling or {}).items())))
 
 
-def _launch(xs, freqs: RotaryFrequencies, positions, offset: int, interleaved: bool, inverse: bool):
-    dev = xs[0].device
-    outs = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in xs]
-    packed = [L.packed_rows(x) for x in xs]  # the tensors stay alive with it
-    xd, od, n = b"".join(p[1] for p in packed), b"".join(L.packed_rows(x)[1] for x in outs), len(xs)
-    ptr, bits, sb, ss = None, 32, 0, 0
-    if positions is not None:
-        ptr, bits = positions.data_ptr(), 64 if positions.dtype == torch.int64 else 32
-        ss = positions.stride(-1)
-        sb = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-    with L.on_device(dev):
-        L.check(L.lib().lcbsa_rotary(xd, od, n, freqs.turns, freqs.pairs, int(interleaved), int(inverse), freqs.factor, ptr, bits, sb, ss,
-                                     int(offset), L.current_stream(dev)))
-    return outs
-
-
-class _Rotary(torch.autograd.Function):
-    """The embedding is linear: the gradient is the rotation back, times the same factor."""
-
-    @staticmethod
-    def forward(ctx, freqs, positions, offset, interleaved, *xs):
-        ctx.freqs, ctx.offset, ctx.interleaved = freqs, offset, interleaved
-        ctx.like = [(x.shape, x.dtype, x.device) for x in xs]
-        ctx.save_for_backward(*(() if positions is None else (positions,)))
-        return tuple(_launch(xs, freqs, positions, offset, interleaved, False))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, *grads):
-        positions = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        there = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[4 + i]]
-        out = [None] * len(grads)
-        if there:
-            for i, g in zip(there, _launch([grads[i] for i in there], ctx.freqs, positions, ctx.offset, ctx.interleaved, True)):
-                out[i] = g
-        return (None, None, None, None, *out)
-
-
 def _embed(xs, freqs, positions, offset, interleaved):
     x0 = xs[0]
     for x in xs:
@@ -138,6 +101,7 @@ def _embed(xs, freqs, positions, offset, interleaved):
             raise ValueError("expected [B, H, S, D] tensors")
         if x.device != x0.device:
             raise ValueError(f"tensors on {x0.device} and {x.device}")
+        L.dtype_code(x.dtype)
         if 2 * freqs.pairs > x.shape[3]:
             raise ValueError(f"{2 * freqs.pairs} turning dimensions of a head of {x.shape[3]}")
     B, _, S, _ = x0.shape
@@ -150,9 +114,7 @@ def _embed(xs, freqs, positions, offset, interleaved):
             raise ValueError(f"positions of shape {tuple(positions.shape)} for {B} entries of {S} tokens")
         if offset:
             raise ValueError("positions and offset exclude each other")
-    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-        return _Rotary.apply(freqs, positions, offset, interleaved, *xs)
-    return tuple(_launch(xs, freqs, positions, offset, interleaved, False))
+    return L.binding().rotary(xs, freqs.address, freqs.pairs, freqs.factor, positions, int(offset), interleaved)
 
 
 @torch.compiler.disable

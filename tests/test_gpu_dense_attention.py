@@ -324,12 +324,37 @@ def test_refusals_on_the_gpu():
     dense = _dense()
     from longcat_video_b200._lib import LcbsaError
     for bad in (lambda: dense(q[..., :32], k[..., :32], v[..., :32]), lambda: dense(q[:, :3], k, v), lambda: dense(q, k, v[:, :, :4]),
-                lambda: dense(q.float(), k.float(), v.float()), lambda: dense(q, k.half(), v.half())):
+                lambda: dense(q.float(), k.float(), v.float())):
         with pytest.raises(LcbsaError):
             bad()
+    with pytest.raises(ValueError):
+        dense(q, k.half(), v.half())
+    with pytest.raises(TypeError):
+        dense(q.double(), k.double(), v.double())
     with pytest.raises(TypeError):
         dense(q, k, v, k_lens=torch.ones(1, device="cuda"))
     with pytest.raises(ValueError):
         dense(q, k, v, k_lens=torch.ones(1, dtype=torch.int32))
     with pytest.raises(ValueError):
         dense(q, k, v, slopes=torch.ones(4, device="cuda", requires_grad=True))
+
+
+def test_no_second_derivative():
+    """A gradient that is itself differentiated says so instead of coming out as zero."""
+    from longcat_video_b200.modules import embed_rotary, rotary_frequencies
+    q, k, v, dout = _inputs(1, 2, 2, 70, 70, 64, torch.bfloat16)
+    q.requires_grad_()
+    for out in (_dense()(q, k, v), embed_rotary(q, rotary_frequencies(64))):
+        (dq,) = torch.autograd.grad(out, q, dout.requires_grad_(), create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            dq.sum().backward()
+
+
+def test_versions_of_saved_tensors_are_checked():
+    q, k, v, dout = _inputs(1, 2, 2, 70, 70, 64, torch.bfloat16)
+    leaf = q.clone().requires_grad_()
+    k = k.clone()
+    out = _dense()(leaf, k, v)
+    k.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.backward(dout)
