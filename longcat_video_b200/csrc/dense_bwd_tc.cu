@@ -232,9 +232,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
         const int k = it.first + kBlk * e;
         return k < it.all_lo || k + kBlk > it.all_hi;
     };
-    auto mixed_queries = [](const Item& it, const int4& unit) {
+    auto mixed_queries = [&P](const Item& it, const int4& unit) {
         const int k = it.own * kM;
-        return k < unit.z || k + kM > unit.w;
+        return k < unit.z || min(k + kM, P.rows) > unit.w;  // rows behind the last key are not stored
     };
     auto seen_of_slot = [&](int slot) { return reinterpret_cast<const int4*>(smem + Ly::offExtra + slot * Ly::extra + kStatsBytes); };
 

@@ -445,7 +445,8 @@ void few_plan(const DenseArgs& a, FewParams& P) {
     const long long units = (long long)a.B * a.Hk * P.tiles;
     P.chunk = 0;
     P.splits = 1;
-    while (P.splits < kMaxCluster && units * P.splits < 148 * 8 && P.splits * kStep < a.Sk) P.splits *= 2;
+    while (P.splits < kMaxCluster && units * P.splits < 148 && P.splits * kStep < a.Sk) P.splits *= 2;
+    while (P.splits < kMaxCluster && units * P.splits < 148 * 8 && P.splits * kStep * 64 <= a.Sk) P.splits *= 2;
     if (units * P.splits >= 148 || a.Sk <= kMaxCluster * 16 * kStep) return;
     // clusters leave SMs idle, with more than 16 rounds to a CTA: chunks, some four for every SM
     long long splits = (148 * 4 + units - 1) / (units > 0 ? units : 1);
@@ -507,8 +508,19 @@ bool dense_supported(const DenseArgs& a, const char** why) {
     return true;
 }
 
-// Which kernel: the tcgen05 kernel computes 128 rows of one head at a time, this one 16 rows of a group of heads.  (To be measured.)
-static bool few_queries(const DenseArgs& a) { return (long long)a.group * a.Sq <= 64; }
+// Which kernel, from what the two cost in us: this one 5, for every key of a tile of 16 (32) rows 0.0100 (0.0145) over the
+// SMs at head_dim 128 and half of it at 64, and 4 for every further wave of CTAs; the tcgen05 kernel 8 (a plan before it, tensor maps) and 0.55 for every
+// unit of 64 keys of 128 rows of ONE head.  Measured (few / tcgen05, us): 8 sequences x 16 heads, head_dim 128: 4 x 512 10.1 / 13.9, 16 x 4096
+// 50.2 / 51.0, 32 x 4096 53.4 / 50.5, 64 x 512 19.7 / 14.2; 2 x 16 heads sharing 4: 64 x 4096 31.7 / 39.6, 200 x 1000 29.0 / 17.8;
+// head_dim 64, 8 heads: 200 x 200 8.4 / 11.0, 64 x 4096 13.6 / 37.9; 8 x 16: 128 x 128 15.1 / 10.9.
+static bool few_queries(const DenseArgs& a) {
+    FewParams P;
+    few_plan(a, P);
+    const double units = (double)a.B * a.Hk * P.tiles, items = (double)a.B * a.Hq * ((a.Sq + 127) / 128);
+    const double few = 5 + units * a.Sk * (a.D / 128.0) * (P.mt == 1 ? 0.0100 : 0.0145) / 148 + 4 * (units > 296 ? units / 296 - 1 : 0);
+    const double tc = 8 + 0.55 * (items <= 148 ? 1 : items / 148) * a.Sk / 64;
+    return few <= tc;
+}
 
 size_t dense_fwd_workspace_bytes(const DenseArgs& a) {
     FewParams P;

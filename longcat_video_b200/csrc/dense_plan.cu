@@ -21,16 +21,18 @@ __device__ __forceinline__ void plan_cta(const DenseArgs& a, int cta, int b, int
         for (int e = 0; e < 2; ++e) {
             const int i = u * kDenseUnit + e * 32 + lane;
             Seen s{0, 0, 0};
-            if (i < a.Sq) s = dense_seen(a.mask, b, i, a.Sq, a.Sk);
-            a.seen[((long long)b * n_u + u) * kSeenPitch + e * 32 + lane] = make_int4(s.lo, s.hi, s.pos, 0);
-            if (s.lo < s.hi) {
-                u_lo = min(u_lo, s.lo);
-                u_hi = max(u_hi, s.hi);
-                all_lo = max(all_lo, s.lo);
-                all_hi = min(all_hi, s.hi);
-            } else {
-                all_hi = 0;
+            if (i < a.Sq) {  // rows behind the last query see nothing and count for nothing: whatever they come to is not stored
+                s = dense_seen(a.mask, b, i, a.Sq, a.Sk);
+                if (s.lo < s.hi) {
+                    u_lo = min(u_lo, s.lo);
+                    u_hi = max(u_hi, s.hi);
+                    all_lo = max(all_lo, s.lo);
+                    all_hi = min(all_hi, s.hi);
+                } else {
+                    all_hi = 0;
+                }
             }
+            a.seen[((long long)b * n_u + u) * kSeenPitch + e * 32 + lane] = make_int4(s.lo, s.hi, s.pos, 0);
         }
         u_lo = __reduce_min_sync(0xffffffffu, u_lo);
         u_hi = __reduce_max_sync(0xffffffffu, u_hi);
