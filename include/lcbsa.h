@@ -332,8 +332,10 @@ typedef struct LcbsaScores {
     const int32_t *cu_q, *cu_k, *k_len, *prefix;
     int64_t cu_stride, prefix_stride;
     int32_t docs, causal;
+    int32_t impl;            /* forward: LCBSA_ATTN_AUTO, _TC (tcgen05, 128 rows of a head at a time), _MMA (warp level, 16 or 32 rows of a group) */
+    int32_t reserved;
 } LcbsaScores;
-size_t lcbsa_dense_attn_workspace_bytes(const LcbsaTensor* q, const LcbsaTensor* k, int backward);
+size_t lcbsa_dense_attn_workspace_bytes(const LcbsaTensor* q, const LcbsaTensor* k, int impl, int backward);
 int lcbsa_dense_attn_fwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaScores* scores, const LcbsaTensor* out,
                          float* lse, void* rest, void* workspace, size_t workspace_bytes, void* stream);
 int lcbsa_dense_attn_bwd(const LcbsaTensor* q, const LcbsaTensor* k, const LcbsaTensor* v, const LcbsaTensor* out, const LcbsaTensor* dout,

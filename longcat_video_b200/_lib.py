@@ -52,7 +52,7 @@ class LcbsaRowJob(ctypes.Structure):
 class LcbsaScores(ctypes.Structure):
     _fields_ = [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p),
                 ("k_len", ctypes.c_void_p), ("prefix", ctypes.c_void_p), ("cu_stride", ctypes.c_int64), ("prefix_stride", ctypes.c_int64),
-                ("docs", ctypes.c_int32), ("causal", ctypes.c_int32)]
+                ("docs", ctypes.c_int32), ("causal", ctypes.c_int32), ("impl", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 # every symbol include/lcbsa.h declares, with its C signature
@@ -102,7 +102,7 @@ SIGNATURES = {
     "lcbsa_rope_table_floats": (ctypes.c_size_t, [_P(LcbsaGrid), ctypes.c_int]),
     "lcbsa_norm_rope": (ctypes.c_int, [_P(LcbsaTensor), ctypes.c_void_p, _P(LcbsaGrid), ctypes.c_void_p, ctypes.c_float,
                                        _P(LcbsaTensor), ctypes.c_void_p]),
-    "lcbsa_dense_attn_workspace_bytes": (ctypes.c_size_t, [_P(LcbsaTensor), _P(LcbsaTensor), ctypes.c_int]),
+    "lcbsa_dense_attn_workspace_bytes": (ctypes.c_size_t, [_P(LcbsaTensor), _P(LcbsaTensor), ctypes.c_int, ctypes.c_int]),
     "lcbsa_dense_attn_fwd": (ctypes.c_int, [_P(LcbsaTensor)] * 3 + [_P(LcbsaScores), _P(LcbsaTensor)] + [ctypes.c_void_p] * 3
                              + [ctypes.c_size_t, ctypes.c_void_p]),
     "lcbsa_dense_attn_bwd": (ctypes.c_int, [_P(LcbsaTensor)] * 5 + [_P(LcbsaScores), ctypes.c_void_p, ctypes.c_void_p]

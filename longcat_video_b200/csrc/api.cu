@@ -581,7 +581,8 @@ static int dense_args(const char* what, const LcbsaTensor* q, const LcbsaTensor*
     a->Sq = (int)q->size[2]; a->Sk = (int)k->size[2];
     a->q = view_of(q); a->k = view_of(k); a->v = view_of(v);
     a->mask = lcbsa::DenseMask{sc->cu_q, sc->cu_k, sc->k_len, sc->prefix, sc->docs, sc->causal != 0, sc->cu_stride, sc->prefix_stride};
-    a->scale = sc->scale; a->cap = sc->cap; a->slopes = sc->slopes;
+    if (sc->impl < LCBSA_ATTN_AUTO || sc->impl > LCBSA_ATTN_MMA) return fail(LCBSA_EINVAL, "%s: unknown impl %d", what, sc->impl);
+    a->scale = sc->scale; a->cap = sc->cap; a->slopes = sc->slopes; a->impl = sc->impl;
     const char* why = "";
     if (!lcbsa::dense_supported(*a, &why)) return fail(LCBSA_EUNSUPPORTED, "%s: %s", what, why);
     return LCBSA_OK;
@@ -611,9 +612,10 @@ static int same_shape(const char* what, const char* name, const LcbsaTensor* t, 
     return LCBSA_OK;
 }
 
-size_t lcbsa_dense_attn_workspace_bytes(const LcbsaTensor* q, const LcbsaTensor* k, int backward) {
-    if (!q || !k) return 0;
-    const lcbsa::DenseArgs a = dense_sizes(q, k);
+size_t lcbsa_dense_attn_workspace_bytes(const LcbsaTensor* q, const LcbsaTensor* k, int impl, int backward) {
+    if (!q || !k || q->size[1] < 1 || k->size[1] < 1) return 0;
+    lcbsa::DenseArgs a = dense_sizes(q, k);
+    a.impl = impl;
     return backward ? lcbsa::dense_bwd_workspace_bytes(a) : lcbsa::dense_fwd_workspace_bytes(a);
 }
 

@@ -7,8 +7,10 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -49,6 +51,7 @@ void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.
 struct Scores {
     double scale, cap;
     bool causal;
+    int64_t impl;
     at::Tensor slopes, cu_q, cu_k, k_lens, prefix;  // undefined: none
 
     LcbsaScores desc() const {
@@ -57,6 +60,7 @@ struct Scores {
         s.scale = (float)scale;
         s.cap = (float)cap;
         s.causal = causal;
+        s.impl = (int32_t)impl;
         s.slopes = slopes.defined() ? static_cast<const float*>(slopes.data_ptr()) : nullptr;
         s.cu_q = ints(cu_q);
         s.cu_k = ints(cu_k);
@@ -82,7 +86,7 @@ Result dense_forward(const at::Tensor& q_in, const at::Tensor& k_in, const at::T
     if (need_rest) r.rest = at::empty(q_in.sizes(), q_in.options());
     const Rows q = rows(q_in), k = rows(k_in), v = rows(v_in), o = rows(r.out);
     const LcbsaScores s = scores.desc();
-    const size_t need = lcbsa_dense_attn_workspace_bytes(&q.d, &k.d, 0);
+    const size_t need = lcbsa_dense_attn_workspace_bytes(&q.d, &k.d, s.impl, 0);
     const at::Tensor ws = need ? at::empty({(int64_t)need}, q_in.options().dtype(at::kByte)) : at::Tensor();
     check(lcbsa_dense_attn_fwd(&q.d, &k.d, &v.d, &s, &o.d, need_lse ? static_cast<float*>(r.lse.data_ptr()) : nullptr,
                                need_rest ? r.rest.data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, need, stream_of(q_in)));
@@ -128,11 +132,11 @@ struct DenseAttention : torch::autograd::Function<DenseAttention> {
             const at::NoGradGuard no_grad;
             const c10::cuda::CUDAGuard guard(saved[0].device());
             const Scores scores{ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["causal"].toBool(),
-                                saved[6], saved[7], saved[8], saved[9], saved[10]};
+                                LCBSA_ATTN_AUTO, saved[6], saved[7], saved[8], saved[9], saved[10]};
             const Rows q = rows(saved[0]), k = rows(saved[1]), v = rows(saved[2]), o = rows(saved[3]), g = rows(grads[0]);
             const Rows dq = rows(dense_like(q.t)), dk = rows(dense_like(k.t)), dv = rows(dense_like(v.t));
             const LcbsaScores s = scores.desc();
-            const size_t need = lcbsa_dense_attn_workspace_bytes(&q.d, &k.d, 1);
+            const size_t need = lcbsa_dense_attn_workspace_bytes(&q.d, &k.d, s.impl, 1);
             const at::Tensor ws = at::empty({(int64_t)need}, q.t.options().dtype(at::kByte));
             in_backward([&] {
                 check(lcbsa_dense_attn_bwd(&q.d, &k.d, &v.d, &o.d, &g.d, &s, static_cast<const float*>(saved[4].data_ptr()), saved[5].data_ptr(),
@@ -239,20 +243,33 @@ PyObject* tuple_of(const torch::autograd::variable_list& ts) {
     return r;
 }
 
+// Whether the call is recorded for a backward.  Under stream capture a leaf that also belongs to a live graph made on another stream is
+// refused: the backward would wait for that stream, which no capture can, and the error would come up in the engine.
 bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
     if (!at::GradMode::is_enabled()) return false;
-    for (const at::Tensor* t : ts)
-        if (t->requires_grad()) return true;
-    return false;
+    bool wants = false;
+    for (const at::Tensor* t : ts) wants |= t->requires_grad();
+    if (wants && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+        for (const at::Tensor* t : ts) {
+            if (!t->requires_grad() || t->grad_fn() != nullptr) continue;
+            const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+            if (node == nullptr) continue;
+            const auto stream = node->stream();
+            TORCH_CHECK(!stream || *stream == c10::cuda::getCurrentCUDAStream(t->get_device()).unwrap(),
+                        "a leaf of this captured call also belongs to a live graph made on another stream: release that graph before the capture");
+        }
+    }
+    return wants;
 }
 
-// dense_attention(q, k, v, scale, cap, causal, slopes, cu_q, cu_k, k_lens, prefix, return_lse) -> out or (out, lse)
+// dense_attention(q, k, v, scale, cap, causal, slopes, cu_q, cu_k, k_lens, prefix, return_lse, impl) -> out or (out, lse)
 PyObject* py_dense_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     try {
-        if (n != 12) return PyErr_Format(PyExc_TypeError, "12 arguments");
+        if (n != 13) return PyErr_Format(PyExc_TypeError, "13 arguments");
         const at::Tensor q = THPVariable_Unpack(a[0]), k = THPVariable_Unpack(a[1]), v = THPVariable_Unpack(a[2]);
-        const Scores s{PyFloat_AsDouble(a[3]), PyFloat_AsDouble(a[4]), PyObject_IsTrue(a[5]) == 1, maybe(a[6]), maybe(a[7]), maybe(a[8]), maybe(a[9]), maybe(a[10])};
+        const Scores s{PyFloat_AsDouble(a[3]), PyFloat_AsDouble(a[4]), PyObject_IsTrue(a[5]) == 1, PyLong_AsLongLong(a[12]), maybe(a[6]), maybe(a[7]), maybe(a[8]), maybe(a[9]), maybe(a[10])};
+        if (PyErr_Occurred()) return nullptr;
         const bool return_lse = PyObject_IsTrue(a[11]) == 1;
         at::Tensor out, lse;
         if (wants_grad({&q, &k, &v})) {

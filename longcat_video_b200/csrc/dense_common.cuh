@@ -39,6 +39,7 @@ struct DenseArgs {
     View q, k, v, o, dout, dq, dk, dv;
     DenseMask mask;
     float scale, cap;
+    int impl;              // LCBSA_ATTN_*
     const float* slopes;   // [Hq] or null
     float* lse;            // [B*Hq, Sq], natural log; nullable in the forward
     void* rest;            // nullable, dense [B, Hq, Sq, D] in the input type: what rounding the output left, for delta

@@ -514,6 +514,7 @@ bool dense_supported(const DenseArgs& a, const char** why) {
 // 50.2 / 51.0, 32 x 4096 53.4 / 50.5, 64 x 512 19.7 / 14.2; 2 x 16 heads sharing 4: 64 x 4096 31.7 / 39.6, 200 x 1000 29.0 / 17.8;
 // head_dim 64, 8 heads: 200 x 200 8.4 / 11.0, 64 x 4096 13.6 / 37.9; 8 x 16: 128 x 128 15.1 / 10.9.
 static bool few_queries(const DenseArgs& a) {
+    if (a.impl != LCBSA_ATTN_AUTO) return a.impl == LCBSA_ATTN_MMA;
     FewParams P;
     few_plan(a, P);
     const double units = (double)a.B * a.Hk * P.tiles, items = (double)a.B * a.Hq * ((a.Sq + 127) / 128);
@@ -533,6 +534,10 @@ size_t dense_fwd_workspace_bytes(const DenseArgs& a) {
 
 cudaError_t launch_dense_fwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why) {
     if (a.B * a.Hq == 0 || a.Sq == 0) return cudaSuccess;
+    if (!few_queries(a) && a.impl == LCBSA_ATTN_TC && !dense_tc_supported(a)) {
+        *why = "the tcgen05 kernel takes at least one query and one key, and tokens a stride apart";
+        return cudaErrorInvalidValue;
+    }
     if (!few_queries(a) && dense_tc_supported(a)) {
         dense_plan_carve(a, workspace, false);
         const cudaError_t e = launch_dense_plan(a, st);

@@ -71,7 +71,7 @@ def _shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, sc
 def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False, softcap: float = 0.0,
                     slopes: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None, cu_k: Optional[torch.Tensor] = None,
                     k_lens: Optional[torch.Tensor] = None, prefix_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-                    return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+                    return_lse: bool = False, impl: int = L.ATTN_AUTO) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """softmax(x) v over the keys that a query sees, x_ij = cap tanh(scale q_i k_j / cap) - slope |pos_i - j|.
 
     ``q [B, Hq, Sq, D]``, ``k``, ``v`` ``[B, Hk, Sk, D]``, bf16 or fp16, D 64 or 128, Hq a multiple of Hk (query head h reads key head
@@ -85,6 +85,8 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
     ``cu_q``) of the document.  These numbers stay on the GPU: nothing is read back, and a captured call replays with what they then
     hold.  A query that sees nothing gets 0 (``lse`` -inf).  What is hidden may hold anything, infinities and NaN included.
 
+    ``impl`` names the forward kernel (``ATTN_TC``: tcgen05, ``ATTN_MMA``: the one for few queries) where the choice by size is not wanted.
+
     Returns ``out [B, Hq, Sq, D]``, with ``return_lse`` also the fp32 ``lse [B, Hq, Sq]`` (no gradient runs through it)."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise RuntimeError("dense_attention needs CUDA tensors; there is no CPU path")
@@ -95,4 +97,4 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
     if q.dtype != k.dtype or q.dtype != v.dtype:
         raise ValueError(f"q, k, v have the types {q.dtype}, {k.dtype}, {v.dtype}")
     L.dtype_code(q.dtype)
-    return L.binding().dense_attention(q, k, v, *_shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, scale), return_lse)
+    return L.binding().dense_attention(q, k, v, *_shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, scale), return_lse, impl)

@@ -61,7 +61,7 @@ def test_the_library_refuses_before_a_launch():
                        ((q, _desc(1, 2, 100, 128), _desc(1, 2, 100, 128), ok, q), "disagree"), ((q, k, k, ok, k), "another shape"),
                        ((q, k, k, _scores(cap=-1.0), q), "cap"), ((q, k, k, _scores(scale=math.inf), q), "finite"),
                        ((q, k, k, _scores(cu_q=4096), q), "go together"), ((q, k, k, _scores(cu_q=4096, cu_k=4096), q), "at least 1"),
-                       ((q, k, k, _scores(cu_q=4096, cu_k=4096, docs=1, k_len=4096), q), "exclude"), ((q, k, k, _scores(prefix=4096), q), "causal"),
+                       ((q, k, k, _scores(cu_q=4096, cu_k=4096, docs=1, k_len=4096), q), "exclude"), ((q, k, k, _scores(prefix=4096), q), "causal"), ((q, k, k, _scores(impl=3), q), "impl"),
                        ((_desc(2, 4, 64, 128, data=4100), k, k, ok, q), "16-byte"), ((_desc(2, 4, 64, 128, L.LCBSA_FP16), k, k, ok, q), "dtypes")):
         rc, msg = _fwd(*args)
         assert rc == -1 and word in msg, msg

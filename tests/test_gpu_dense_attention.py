@@ -76,21 +76,25 @@ def _options(case, dtype, D):
     return lo, hi, pos, kw, o.get("scale") or 1 / math.sqrt(D), o.get("spread", 1.0)
 
 
+TC, MMA = 1, 2  # the forward kernels: tcgen05, and the one for few queries
+
+
+@pytest.mark.parametrize("impl", [TC, MMA])
 @pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16), (64, torch.bfloat16), (128, torch.float16)])
 @pytest.mark.parametrize("name", CASES)
-def test_forward_and_gradients(name, D, dtype):
+def test_forward_and_gradients(name, D, dtype, impl):
     B, Hq, Hk, Sq, Sk = CASES[name][0]
     lo, hi, pos, kw, scale, spread = _options(CASES[name], dtype, D)
     q, k, v, dout = _inputs(B, Hq, Hk, Sq, Sk, D, dtype, spread=spread)
     want = R.attend(q, k, v, lo, hi, pos, scale, kw["softcap"], kw.get("slopes"), dout)
     with torch.no_grad():
-        plain, lse = _dense()(q, k, v, return_lse=True, **kw)
+        plain, lse = _dense()(q, k, v, return_lse=True, impl=impl, **kw)
     assert R.worst(plain, want["o"]) <= 1
     blind = torch.isinf(want["lse"])
     assert torch.equal(torch.isinf(lse), blind) and torch.equal(plain[blind], torch.zeros_like(plain[blind]))
     assert float((lse.double() - want["lse"])[~blind].abs().max()) <= R.SCORE + 1e-5
     leaves = [x.clone().requires_grad_() for x in (q, k, v)]
-    out = _dense()(*leaves, **kw)
+    out = _dense()(*leaves, impl=impl, **kw)
     grads = torch.autograd.grad(out, leaves, dout)
     assert torch.equal(out, plain)
     for got, x in zip(grads, ("dq", "dk", "dv")):
@@ -132,13 +136,13 @@ def _in_64(qkv, lo, hi, pos, scale, cap, slopes):
 
 
 @pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
-@pytest.mark.parametrize("Sq", [1, 6, 200])
-def test_hidden_keys_may_hold_anything(poison, Sq):
+@pytest.mark.parametrize("Sq,impl", [(1, MMA), (6, MMA), (200, MMA), (200, TC), (3, TC)])
+def test_hidden_keys_may_hold_anything(poison, Sq, impl):
     """Keys behind the length, keys of another document, queries of no document: not a bit of the result changes."""
     B, Hq, Hk, Sk, D = 2, 4, 2, 300, 128
     q, k, v, dout = _inputs(B, Hq, Hk, Sq, Sk, D, torch.bfloat16, seed=1)
     lens = torch.tensor([200 + Sq % 7, 61], dtype=torch.int32, device="cuda")
-    kw = dict(causal=True, k_lens=lens)
+    kw = dict(causal=True, k_lens=lens, impl=impl)
 
     def all_of(q, k, v):
         leaves = [x.clone().requires_grad_() for x in (q, k, v)]
@@ -153,8 +157,8 @@ def test_hidden_keys_may_hold_anything(poison, Sq):
         assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)])
-def test_documents_and_order_keep_values_apart(D, dtype):
+@pytest.mark.parametrize("D,dtype,impl", [(128, torch.bfloat16, TC), (64, torch.float16, TC), (128, torch.bfloat16, MMA)])
+def test_documents_and_order_keep_values_apart(D, dtype, impl):
     """One document, and the later half of another, hold NaN and infinities in q, k, v and dout: the results of the rows that do not see
     them, and the gradients of the keys that are not seen by such queries, are finite and within their bounds."""
     S, H = 400, 2
@@ -167,7 +171,7 @@ def test_documents_and_order_keep_values_apart(D, dtype):
         for n, i in enumerate(sorted(bad)):
             x[0, :, i, (7 * n) % D] = (math.nan, math.inf, -math.inf)[n % 3]
     leaves = [x.clone().requires_grad_() for x in (q, k, v)]
-    out = _dense()(*leaves, causal=True, cu_q=torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    out = _dense()(*leaves, causal=True, cu_q=torch.tensor(cu, dtype=torch.int32, device="cuda"), impl=impl)
     dq, dk, dv = torch.autograd.grad(out, leaves, dout)
     rows = list(range(0, 150)) + list(range(290, 350))  # see no bad key
     keys = list(range(0, 150))                            # seen by no bad query
@@ -177,23 +181,25 @@ def test_documents_and_order_keep_values_apart(D, dtype):
     assert torch.isnan(out[:, :, 150:290]).any(-1).all() and torch.isnan(dq[:, :, 150:290]).any(-1).all()
 
 
-def test_a_seen_infinity_stays_where_it_is():
+@pytest.mark.parametrize("impl", [TC, MMA])
+def test_a_seen_infinity_stays_where_it_is(impl):
     """v = inf in one dimension of a key that some rows of a tile see: those rows are inf there and finite elsewhere."""
     q, k, v, _ = _inputs(1, 2, 2, 100, 100, 64, torch.bfloat16, seed=4)
     v[0, 1, 40, 5] = math.inf
-    out = _dense()(q, k, v, causal=True)
+    out = _dense()(q, k, v, causal=True, impl=impl)
     assert torch.isposinf(out[0, 1, 40:, 5]).all()
     out[0, 1, 40:, 5] = 0
     assert torch.isfinite(out).all()
     q1 = q[:, :, :1]
-    out = _dense()(q1, k, v, k_lens=torch.tensor([41], dtype=torch.int32, device="cuda"))
+    out = _dense()(q1, k, v, k_lens=torch.tensor([41], dtype=torch.int32, device="cuda"), impl=impl)
     assert torch.isposinf(out[0, 1, 0, 5]) and int(torch.isfinite(out).sum()) == out.numel() - 1
 
 
-def test_a_nan_score_makes_its_rows_nan():
+@pytest.mark.parametrize("impl", [TC, MMA])
+def test_a_nan_score_makes_its_rows_nan(impl):
     q, k, v, _ = _inputs(1, 2, 2, 130, 130, 64, torch.bfloat16, seed=4)
     k[0, 0, 70, 3] = math.nan
-    out, lse = _dense()(q, k, v, causal=True, return_lse=True)
+    out, lse = _dense()(q, k, v, causal=True, return_lse=True, impl=impl)
     assert torch.isnan(out[0, 0, 70:]).all() and torch.isfinite(out[0, 0, :70]).all() and torch.isfinite(out[0, 1]).all()
     assert torch.isnan(lse[0, 0, 70:]).all() and torch.isfinite(lse[0, 0, :70]).all()
 
@@ -223,12 +229,13 @@ def test_strides_and_broadcast():
         assert torch.equal(a, b)
 
 
-def test_two_calls_give_the_same_bits():
+@pytest.mark.parametrize("impl", [TC, MMA])
+def test_two_calls_give_the_same_bits(impl):
     q, k, v, dout = _inputs(2, 8, 2, 500, 500, 128, torch.bfloat16)
     res = []
     for _ in range(2):
         leaves = [x.clone().requires_grad_() for x in (q, k, v)]
-        out = _dense()(*leaves, causal=True, softcap=20.0, slopes=_slopes(8))
+        out = _dense()(*leaves, causal=True, softcap=20.0, slopes=_slopes(8), impl=impl)
         res.append([out.detach(), *torch.autograd.grad(out, leaves, dout)])
     assert all(torch.equal(a, b) for a, b in zip(*res))
 
@@ -256,14 +263,14 @@ def test_empty_tensors():
     assert torch.equal(grads[0], torch.zeros_like(q)) and grads[1].shape == (1, 2, 0, 64)
 
 
-@pytest.mark.parametrize("Sq,Sk", [(3, 700), (300, 300)])
-def test_captured_calls_follow_their_numbers(Sq, Sk):
+@pytest.mark.parametrize("Sq,Sk,impl", [(3, 700, MMA), (1, 30000, MMA), (300, 300, TC)])
+def test_captured_calls_follow_their_numbers(Sq, Sk, impl):
     """Two graphs of the same call on their own streams: replayed with other lengths, values and slopes."""
     q, k, v, _ = _inputs(2, 4, 2, Sq, Sk, 128, torch.bfloat16)
     lens = torch.tensor([Sk, Sk // 2], dtype=torch.int32, device="cuda")
     slopes = _slopes(4)
     graphs, outs = [], []
-    call = lambda: _dense()(q, k, v, causal=True, k_lens=lens, slopes=slopes, softcap=10.0)  # noqa: E731
+    call = lambda: _dense()(q, k, v, causal=True, k_lens=lens, slopes=slopes, softcap=10.0, impl=impl)  # noqa: E731
     call()
     for _ in range(2):
         g = torch.cuda.CUDAGraph()
@@ -286,11 +293,11 @@ def test_captured_calls_follow_their_numbers(Sq, Sk):
 
 def test_other_streams():
     """Calls on two streams at once, forward and backward: each has its own workspace."""
-    args = [_inputs(1, 4, 2, 400, 400, 64, torch.float16, seed=s) for s in range(2)]
+    args = [_inputs(1, 16, 8, 700, 700, 64, torch.float16, seed=s) for s in range(2)]
 
     def step(q, k, v, dout):
         leaves = [x.clone().requires_grad_() for x in (q, k, v)]
-        out = _dense()(*leaves, causal=True)
+        out = _dense()(*leaves, causal=True, impl=TC)
         return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
     want = [step(*a) for a in args]
     torch.cuda.synchronize()
@@ -358,3 +365,109 @@ def test_versions_of_saved_tensors_are_checked():
     k.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         out.backward(dout)
+
+
+@pytest.mark.parametrize("D,dtype,kw", [(128, torch.bfloat16, dict(causal=True)), (64, torch.float16, dict(softcap=8.0, slopes=True)),
+                                        (64, torch.bfloat16, dict(causal=True, docs=True))])
+def test_many_items_per_cta(D, dtype, kw):
+    """More tiles than SMs, several to a CTA, of very different lengths: every head gives the bits it gives alone, and a few of
+    them are held to the formulas."""
+    B, Hq, Hk, S = 3, 40, 40, 700
+    kw = dict(kw)
+    if kw.pop("docs", False):
+        kw["cu_q"] = torch.tensor([[0, 90, 91, 600, 700], [0, 0, 300, 300, 700], [5, 100, 200, 500, 650]], dtype=torch.int32, device="cuda")
+    slopes = _slopes(Hq) if kw.pop("slopes", False) else None
+    q, k, v, dout = _inputs(B, Hq, Hk, S, S, D, dtype, seed=7)
+
+    def step(q, k, v, dout, slopes):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = _dense()(*leaves, slopes=slopes, impl=TC, **kw)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+    full = step(q, k, v, dout, slopes)
+    for h in (0, 17, 39):
+        one = step(*(x[:, h:h + 1] for x in (q, k, v, dout)), None if slopes is None else slopes[h:h + 1])
+        for a, b in zip(full, one):
+            assert torch.equal(a[:, h:h + 1], b)
+    docs = None if "cu_q" not in kw else [(c, c) for c in kw["cu_q"].tolist()]
+    lo, hi, pos = R.runs(B, S, S, kw.get("causal", False), docs, None, None)
+    want = R.attend(*(x[:, 17:19] for x in (q, k, v)), lo, hi, pos, 1 / math.sqrt(D), kw.get("softcap", 0.0), None if slopes is None else slopes[17:19],
+                    dout[:, 17:19])
+    for got, x in zip(full, ("o", "dq", "dk", "dv")):
+        assert R.worst(got[:, 17:19], want[x]) <= 1, x
+
+
+def test_waves_of_heads():
+    """K and V of all heads together exceed what the items' order keeps in the L2: heads in waves, each with the bits it has alone."""
+    H, S, D = 37, 4096, 128
+    q, k, v, dout = _inputs(1, H, H, S, S, D, torch.bfloat16)
+
+    def step(q, k, v, dout):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = _dense()(*leaves, causal=True, impl=TC)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+    full = step(q, k, v, dout)
+    for h in (0, 18, 19, 36):
+        for a, b in zip(full, step(*(x[:, h:h + 1] for x in (q, k, v, dout)))):
+            assert torch.equal(a[:, h:h + 1], b)
+
+
+@pytest.mark.parametrize("B,Hq,Hk,Sq,Sk,D", [(1, 4, 1, 1, 20000, 128), (1, 2, 1, 3, 12345, 64), (40, 8, 4, 1, 2100, 128), (2, 16, 2, 3, 900, 64),
+                                             (1, 1, 1, 1, 65, 128), (70, 4, 4, 2, 130, 64), (1, 64, 2, 1, 515, 128)])
+def test_ways_of_sharing_out_the_keys(B, Hq, Hk, Sq, Sk, D):
+    """Chunks with a second kernel, clusters of every size, one CTA; one tile of rows and several of two."""
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, Sk + 1, (B,), generator=g).tolist()
+    lens[0] = Sk
+    q, k, v, _ = _inputs(B, Hq, Hk, Sq, Sk, D, torch.bfloat16)
+    lo, hi, pos = R.runs(B, Sq, Sk, True, None, lens, None)
+    want = R.attend(q, k, v, lo, hi, pos, 1 / math.sqrt(D), 25.0, _slopes(Hq))
+    out, lse = _dense()(q, k, v, causal=True, softcap=25.0, slopes=_slopes(Hq), k_lens=torch.tensor(lens, device="cuda"), return_lse=True, impl=MMA)
+    assert R.worst(out, want["o"]) <= 1
+    blind = torch.isinf(want["lse"])
+    assert torch.equal(torch.isinf(lse), blind) and float((lse.double() - want["lse"])[~blind].abs().max()) <= R.SCORE + 1e-5
+
+
+def test_scores_of_any_size_under_a_cap():
+    """Scores far beyond the cap, where the polynomial does not reach, next to small ones."""
+    for impl in (TC, MMA):
+        q, k, v, dout = _inputs(1, 2, 2, 200, 200, 64, torch.bfloat16, seed=9)
+        q[:, :, 30:40] *= 40
+        lo, hi, pos = R.runs(1, 200, 200, True, None, None, None)
+        want = R.attend(q, k, v, lo, hi, pos, 0.02, 2.0, None, dout)
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = _dense()(*leaves, causal=True, softcap=2.0, scale=0.02, impl=impl)
+        assert R.worst(out.detach(), want["o"]) <= 1
+        for got, x in zip(torch.autograd.grad(out, leaves, dout), ("dq", "dk", "dv")):
+            assert R.worst(got, want[x]) <= 1, x
+
+
+def test_a_scale_of_zero():
+    q, k, v, dout = _inputs(1, 2, 2, 150, 150, 64, torch.bfloat16)
+    for impl in (TC, MMA):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = _dense()(*leaves, scale=0.0, softcap=3.0, impl=impl)
+        mean = v.double().mean(2, keepdim=True)
+        assert float((out.detach().double() - mean).abs().max()) <= 2.0 ** -8 * 2 * float(v.detach().abs().max())
+        dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+        assert not dq.any() and not dk.any() and torch.isfinite(dv).all()
+
+
+def test_a_step_in_a_graph_beside_an_eager_one():
+    """Forward and gradients captured while an eager graph of the same leaves lives: refused at the call, before the capture breaks
+    in the engine.  With the eager graph released the same capture goes through and gives the same."""
+    q, k, v, dout = _inputs(1, 4, 2, 300, 300, 64, torch.bfloat16)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    call = lambda: _dense()(*leaves, causal=True, softcap=9.0)  # noqa: E731
+    eager = call()
+    with pytest.raises(RuntimeError, match="live graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            call()
+    want = [eager.detach(), *torch.autograd.grad(eager, leaves, dout)]
+    del eager
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+        grads = torch.autograd.grad(out, leaves, dout)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((out, *grads), want))
