@@ -11,7 +11,7 @@
 // of the launch, so a call reads nothing but its rows and its positions.
 //
 // A thread owns one 16-byte vector of a token (half layout: the two vectors that its eight pairs lie in) and walks over a group
-// of heads, so the angles are worked out once for all of them; the next head's vectors are in flight under the arithmetic.
+// of heads, four at a time, so the angles are worked out once for all of them.
 // A call takes q and k together: one launch.
 #include "common.cuh"
 
@@ -20,6 +20,7 @@ namespace lcbsa {
 namespace {
 
 constexpr int kRotThreads = 256;
+constexpr int kBatch = 4;  // heads whose vectors a thread has in flight
 
 template <typename T> struct Two;
 template <> struct Two<__nv_bfloat16> {
@@ -71,6 +72,22 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
     const int turning = kInter ? P.pairs / 4 : P.pairs / 8;
     const bool turns = slot < turning;
     const int at = turns ? slot * 8 : 2 * P.pairs + (slot - turning) * 8;
+    const T* src = static_cast<const T*>(J.x.data) + b * J.x.sb + s * J.x.ss + h0 * J.x.sh + at;
+    T* dst = static_cast<T*>(const_cast<void*>(J.out.data)) + b * J.out.sb + s * J.out.ss + h0 * J.out.sh + at;
+    const bool both = !kInter && turns;
+    // kBatch heads at a time, all of their vectors in flight together; those of the first batch under the angles
+    uint4 v[kBatch], w[kBatch];
+    auto fetch = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (h + i < h1) {
+                v[i] = *reinterpret_cast<const uint4*>(src);
+                if (both) w[i] = *reinterpret_cast<const uint4*>(src + P.pairs);
+                src += J.x.sh;
+            }
+        }
+    };
+    fetch(h0);
     float cs[kAngles], sn[kAngles];
     if (turns) {
         long long pos = P.offset + s;
@@ -87,25 +104,18 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
             sn[i] *= P.inverse ? -P.factor : P.factor;
         }
     }
-    const T* src = static_cast<const T*>(J.x.data) + b * J.x.sb + s * J.x.ss + h0 * J.x.sh + at;
-    T* dst = static_cast<T*>(const_cast<void*>(J.out.data)) + b * J.out.sb + s * J.out.ss + h0 * J.out.sh + at;
-    const bool both = !kInter && turns;
-    uint4 a = *reinterpret_cast<const uint4*>(src), c = make_uint4(0u, 0u, 0u, 0u);
-    if (both) c = *reinterpret_cast<const uint4*>(src + P.pairs);
 #pragma unroll 1
-    for (int h = h0; h < h1; ++h) {
-        uint4 na = make_uint4(0u, 0u, 0u, 0u), nc = na;
-        src += J.x.sh;
-        if (h + 1 < h1) {
-            na = *reinterpret_cast<const uint4*>(src);
-            if (both) nc = *reinterpret_cast<const uint4*>(src + P.pairs);
+    for (int h = h0; h < h1; h += kBatch) {
+        if (h > h0) fetch(h);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (h + i < h1) {
+                if (turns) turn<T, kInter>(v[i], w[i], cs, sn);
+                *reinterpret_cast<uint4*>(dst) = v[i];
+                if (both) *reinterpret_cast<uint4*>(dst + P.pairs) = w[i];
+                dst += J.out.sh;
+            }
         }
-        if (turns) turn<T, kInter>(a, c, cs, sn);
-        *reinterpret_cast<uint4*>(dst) = a;
-        if (both) *reinterpret_cast<uint4*>(dst + P.pairs) = c;
-        dst += J.out.sh;
-        a = na;
-        c = nc;
     }
 }
 
@@ -129,7 +139,7 @@ cudaError_t launch_rotary(int dtype, RotaryArgs& P, int B, int D, cudaStream_t s
         for (int i = 0; i < P.n; ++i) n += P.job[i].groups = (P.job[i].H + P.hpc - 1) / P.hpc;
         return n;
     };
-    while (P.hpc > 1 && ctas * groups() < 148 * 8) P.hpc /= 2;
+    while (P.hpc > 1 && ctas * groups() < 148 * 4) P.hpc /= 2;
     const int n = groups();
     if (n > 65535) {
         *why = "more heads than a launch takes";

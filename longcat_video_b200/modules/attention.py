@@ -15,6 +15,7 @@ import torch
 
 from .. import _lib as L
 from ..block_sparse_attention.bsa_interface import flash_attn_bsa_3d, flash_attn_bsa_3d_cond
+from .dense_attention import dense_attention
 from .rope_3d import RowJob, kv_cache_row_jobs, run_row_jobs
 
 
@@ -27,14 +28,26 @@ def _rows_can_be_copied(src: torch.Tensor, dst: torch.Tensor) -> bool:
             and torch.autograd.forward_ad._current_level < 0)
 
 
+def _dense_cond(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, shape: Sequence[int], num_cond_latents: Optional[int]) -> torch.Tensor:
+    """The layer's attention with block sparsity off: every token to every token, the conditioning frames among themselves."""
+    nc = int(num_cond_latents or 0)
+    if nc <= 0:
+        return dense_attention(q, k, v)
+    T, Hh, W = shape
+    if nc >= T:
+        raise ValueError(f"num_cond_latents {nc} outside (0, {T})")
+    sc = nc * Hh * W
+    return torch.cat([dense_attention(q[:, :, :sc], k[:, :, :sc], v[:, :, :sc]), dense_attention(q[:, :, sc:], k, v)], dim=2)
+
+
 def self_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
-                   shape: Sequence[int], bsa_params: dict, num_cond_latents: Optional[int] = None, return_kv: bool = False,
+                   shape: Sequence[int], bsa_params: Optional[dict], num_cond_latents: Optional[int] = None, return_kv: bool = False,
                    eps: float = 1e-6):
     """``Attention.forward`` between the projections (attention.py:116-137): q/k RMSNorm, 3-D rotary embedding over
     ``shape`` = (T, H, W), then the block-sparse attention -- with ``num_cond_latents`` the first that many frames attend
     among themselves and the rest to everything (attention.py:124-135), as one op on views.  ``return_kv`` also returns
     what the layer caches for video continuation: the normalised, not yet embedded k and a copy of v
-    (attention.py:118-119).  Returns ``x [B, H, N, D]`` or ``(x, (k_cache, v_cache))``."""
+    (attention.py:118-119).  ``bsa_params`` None: a layer without block sparsity, on ``dense_attention``.  Returns ``x [B, H, N, D]`` or ``(x, (k_cache, v_cache))``."""
     shape = tuple(int(s) for s in shape)
     kv = None
     q_e, k_e = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
@@ -50,7 +63,9 @@ def self_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: 
     else:
         jobs.append(RowJob(k, k_e, k_weight, shape))
     run_row_jobs(jobs, eps)
-    if num_cond_latents is not None and num_cond_latents > 0:
+    if bsa_params is None:
+        x = _dense_cond(q_e, k_e, v, shape, num_cond_latents)
+    elif num_cond_latents is not None and num_cond_latents > 0:
         x = flash_attn_bsa_3d_cond(q_e, k_e, v, shape, num_cond_latents, **bsa_params)
     else:
         x = flash_attn_bsa_3d(q_e, k_e, v, shape, shape, **bsa_params)
@@ -58,7 +73,7 @@ def self_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: 
 
 
 def self_attention_with_kv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
-                                 shape: Sequence[int], kv_cache: Tuple[torch.Tensor, torch.Tensor], bsa_params: dict,
+                                 shape: Sequence[int], kv_cache: Tuple[torch.Tensor, torch.Tensor], bsa_params: Optional[dict],
                                  num_cond_latents: int, eps: float = 1e-6) -> torch.Tensor:
     """``Attention.forward_with_kv_cache`` between the projections (attention.py:156-173): the ``T`` new frames of
     ``shape`` = (T, H, W) attend to the ``num_cond_latents`` cached frames and to themselves.  The cached keys (stored
@@ -67,7 +82,7 @@ def self_attention_with_kv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     reference puts in front of it (attention.py:166-169), and the attention runs with ``Tq = T`` query frames against
     ``Tk = T + NC`` key frames.  A cache of batch 1 serves every batch entry (attention.py:159-162).  The reference
     defines the concatenated k, v only when ``num_cond_latents > 0`` (attention.py:164-169); any other value is refused
-    here.  Returns ``x [B, H, N, D]``."""
+    here.  ``bsa_params`` None: a layer without block sparsity.  Returns ``x [B, H, N, D]``."""
     T, Hh, W = (int(s) for s in shape)
     nc = int(num_cond_latents or 0)
     if nc <= 0:
@@ -88,4 +103,6 @@ def self_attention_with_kv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
         else:
             dst.copy_(src)
     run_row_jobs(jobs, eps)
+    if bsa_params is None:
+        return dense_attention(q_e, k_full, v_full)
     return flash_attn_bsa_3d(q_e, k_full, v_full, (T, Hh, W), (T + nc, Hh, W), **bsa_params)

@@ -56,3 +56,27 @@ def test_tokens_one_at_a_time():
     out = torch.cat(rows, 2)
     lo, hi, p = R.runs(B, total, total, True, None, None, None)
     assert R.worst(out, R.attend(qe, ke, v, lo, hi, p, 1 / math.sqrt(D))["o"]) <= 1
+
+
+@pytest.mark.parametrize("nc", [0, 2])
+def test_layer_without_block_sparsity(nc):
+    """self_attention with bsa_params None: RMSNorm and 3-D rotary, then every token to every token, the conditioning frames among
+    themselves; the same layer with those frames cached gives the rows behind them."""
+    from longcat_video_b200.modules import qk_norm_rope, self_attention, self_attention_with_kv_cache
+    B, H, D, shape = 2, 3, 128, (5, 6, 7)
+    N, sc = 5 * 6 * 7, nc * 6 * 7
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qkv = torch.randn(B, N, 3, H, D, generator=g, device="cuda").bfloat16()
+    q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
+    wq, wk = torch.rand(2, D, generator=g, device="cuda") + 0.5
+    x, (k_cache, v_cache) = self_attention(q, k, v, wq, wk, shape, None, nc, return_kv=True)
+    qe, ke = qk_norm_rope(q, k, wq, wk, shape)
+    zero = torch.zeros(B, N, dtype=torch.int64)
+    hi = torch.full((B, N), N)
+    hi[:, :sc] = sc
+    assert R.worst(x, R.attend(qe, ke, v, zero, hi, zero, 1 / math.sqrt(D))["o"]) <= 1
+    if nc:
+        new = self_attention_with_kv_cache(q[:, :, sc:], k[:, :, sc:], v[:, :, sc:], wq, wk, (5 - nc, 6, 7), (k_cache[:, :, :sc], v_cache[:, :, :sc]), None, nc)
+        assert R.worst(new, tuple(t[:, :, sc:] for t in R.attend(qe, ke, v, zero, hi, zero, 1 / math.sqrt(D))["o"])) <= 1
+        with pytest.raises(ValueError):
+            self_attention(q, k, v, wq, wk, shape, None, 5)
