@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
             __syncwarp();
             return true;
         };
-        Item cur, nx;
+        Item cur;
         if (is_k) {
             ok = announce(0, blockIdx.x, cur);
             if (ok && cur.n >= 0) request_q(cur);
@@ -423,14 +423,6 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
             ok = take_item(0, cur);
         }
         while (ok && cur.n >= 0) {
-            if (is_k) {
-                int idx = 0;
-                if (lane == 0) idx = (int)gridDim.x + atomicAdd(P.next_item, 1);
-                ok = announce(wk + 1, __shfl_sync(0xffffffffu, idx, 0), nx);
-            } else {
-                ok = take_item(wk + 1, nx);
-            }
-            if (!ok) break;
             const int b = cur.bh / P.Hq, h = (cur.bh - b * P.Hq) / P.group;
             const int ch = (fold & 1) ? 0 : h, cb = (fold & 2) ? 0 : b;
             const int n_iter = rounds(cur);
@@ -456,23 +448,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                 mbar_arrive_elect(bar_v_ok(vs));
                 return true;
             };
-            bool q_due = is_k && nx.n >= 0;  // Q of the next item has not been requested yet
 #pragma unroll 1
             for (int j = 0; j < n_iter; ++j) {
-                // Q of the next item as soon as the buffer is free again (see the epilogue warps), which is early in this
-                // item; behind the last chance for it comes the item's last K.
-                if (q_due) {
-                    const uint32_t bar = wk == 0 ? bar_qt_full : bar_q_free, ph = wk == 0 ? 0 : (wk - 1) & 1;
-                    bool go = __all_sync(0xffffffffu, mbar_test(bar, ph));
-                    if (!go && j == n_iter - 1) {
-                        ok = go = mbar_wait_warp(bar, ph, ctl, 10, wk);
-                        if (!ok) break;
-                    }
-                    if (go) {
-                        request_q(nx);
-                        q_due = false;
-                    }
-                }
                 ok = mbar_wait_warp(empty0 + 8u * slot, parity, ctl, is_k ? 20 : 22, gk);
                 if (!ok) break;
                 const uint32_t bar = full0 + 8u * slot, dst = ring + slot * Ly::tile;
@@ -492,9 +469,21 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                     if (!ok) break;
                 }
             }
-            if (!is_k)
+            if (!ok) break;
+            if (is_k) {
+                // The next item, behind this one's last copies: six units of work are in the ring then.  Asked earlier, a CTA commits itself to
+                // an item that it will not come to for long.
+                int idx = 0;
+                if (lane == 0) idx = (int)gridDim.x + atomicAdd(P.next_item, 1);
+                ok = announce(wk + 1, __shfl_sync(0xffffffffu, idx, 0), cur);
+                if (ok && cur.n >= 0) {  // its Q as soon as the buffer is free (see the epilogue warps)
+                    ok = wk == 0 ? mbar_wait_warp(bar_qt_full, 0, ctl, 10, wk) : mbar_wait_warp(bar_q_free, (wk - 1) & 1, ctl, 11, wk);
+                    if (ok) request_q(cur);
+                }
+            } else {
                 for (int j = max(n_iter - 3, 0); j < n_iter && ok; ++j) ok = look_at(j);
-            cur = nx;
+                if (ok) ok = take_item(wk + 1, cur);
+            }
             ++wk;
         }
         if (!ok && lane == 0) {
