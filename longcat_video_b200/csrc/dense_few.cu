@@ -5,8 +5,8 @@
 // four of them and the cache is still read once.  The keys that the rows see are split evenly over the CTAs of a cluster, which join
 // their partial results (fp32, relative to their maxima) through each other's shared memory: one launch, no workspace, one order.
 // Where clusters of eight leave the chip idle and the keys are many, chunks of a fixed number of keys go to CTAs of their own
-// instead, and a second kernel joins partial results from the workspace.  Inside a CTA four warps take every fourth tile of 16
-// (head_dim 64: 32) keys: a warp has a ring of its own in shared memory and nothing in the loop waits for another warp.  S, P and O
+// instead, and a second kernel joins partial results from the workspace.  Inside a CTA four warps (eight at head_dim 64) take
+// tiles of 16 keys in turn: a warp has a ring of its own in shared memory and nothing in the loop waits for another warp.  S, P and O
 // stay in registers (mma.sync m16n8k16, fp32 accumulators; P is rounded to the input type for the product with V, as in the
 // other attention kernels, the row sum is taken before the rounding); running maximum and sum per row in fp32.
 //
@@ -20,12 +20,12 @@ namespace lcbsa {
 
 namespace {
 
-constexpr int kFewWarps = 4;
+template <int D> constexpr int kFewWarps = D == 64 ? 8 : 4;
 constexpr int kFewStages = 3;   // tiles of a warp's ring, of K and V each
-template <int D> constexpr int kKeys = D == 64 ? 32 : 16;  // keys of a warp's tile: 4 KB of K and of V
+constexpr int kKeys = 16;       // keys of a warp's tile
 constexpr int kMaxCluster = 8;  // CTAs of a cluster (16, which have to be asked for, start one after another: 20 us became 32)
 constexpr int kMaxSplits = 256;
-constexpr int few_step(int D) { return kFewWarps * (D == 64 ? 32 : 16); }  // keys of a CTA's round
+constexpr int few_step(int D) { return (D == 64 ? 8 : 4) * kKeys; }  // keys of a CTA's round
 
 struct FewParams {
     DenseArgs a;
@@ -40,18 +40,20 @@ struct FewParams {
 
 template <int D, int MT>
 constexpr int few_smem() {
-    return 16 * MT * D * 2 + kFewWarps * kFewStages * 2 * kKeys<D> * D * 2 + 16 * MT * 16;
+    return 16 * MT * D * 2 + kFewWarps<D> * kFewStages * 2 * kKeys * D * 2 + 16 * MT * 16;
 }
 
-// rows from `first` on into a swizzled tile; rows at `end` or behind are zero
+// A warp's rows `first` .. of K or V into a swizzled tile; rows at `end` or behind are zero.  src: where this lane's 16 bytes of row
+// first + lane / (chunks of a row) are, if there is such a row; head: an address that there is.
 template <typename T, int D>
-__device__ __forceinline__ void load_keys(uint32_t tile, const T* head, long long ss, int first, int end, int lane) {
-    constexpr int CPR = D * 2 / 16;
+__device__ __forceinline__ void load_keys(uint32_t tile, const T* src, const T* head, long long ss, int first, int end, int lane) {
+    constexpr int CPR = D * 2 / 16, kRowsAtOnce = 32 / CPR;
+    const int r0 = lane / CPR, c = lane % CPR;
 #pragma unroll
-    for (int v = lane; v < kKeys<D> * CPR; v += 32) {
-        const int row = v / CPR, c = v % CPR;
+    for (int i = 0; i < kKeys / kRowsAtOnce; ++i, src += kRowsAtOnce * ss) {
+        const int row = r0 + i * kRowsAtOnce;
         const bool there = first + row < end;
-        mm::cp_async16(tile + row * (D * 2) + ((c ^ (row & 7)) << 4), head + (there ? (long long)(first + row) * ss : 0) + c * 8, there);
+        mm::cp_async16(tile + row * (D * 2) + ((c ^ (row & 7)) << 4), there ? src : head, there);
     }
 }
 
@@ -86,11 +88,11 @@ __device__ __forceinline__ void write_row(const DenseArgs& a, int b, int hk, int
 }
 
 template <typename T, int D, int MT, bool kCap, bool kBias>
-__global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_constant__ FewParams P) {
-    constexpr int kN = kKeys<D>, kTileBytes = kN * D * 2, kRows = 16 * MT, kStages = kFewStages, kStep = few_step(D);
+__global__ void __launch_bounds__(kFewWarps<D> * 32, 2) dense_few_kernel(const __grid_constant__ FewParams P) {
+    constexpr int kN = kKeys, kTileBytes = kN * D * 2, kRows = 16 * MT, kStages = kFewStages, kStep = few_step(D), kW = kFewWarps<D>;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* const ring0 = smem + kRows * D * 2;
-    int4* const seen_s = reinterpret_cast<int4*>(ring0 + kFewWarps * kStages * 2 * kTileBytes);  // [rows] lo, hi, pos
+    int4* const seen_s = reinterpret_cast<int4*>(ring0 + kW * kStages * 2 * kTileBytes);  // [rows] lo, hi, pos
     const DenseArgs& a = P.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int split = blockIdx.x % P.splits;  // in a cluster: the CTA's rank
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
     {   // the rows' queries into a swizzled tile, and what they see
         constexpr int CPR = D * 2 / 16;
         const uint32_t q_tile = mm::smem_u32(smem);
-        for (int v = tid; v < kRows * CPR; v += kFewWarps * 32) {
+        for (int v = tid; v < kRows * CPR; v += kW * 32) {
             const int r = v / CPR, c = v % CPR, rr = row0 + r;
             const bool there = rr < P.rows;
             const int i = there ? rr / a.group : 0, h = hk * a.group + (there ? rr % a.group : 0);
@@ -143,16 +145,22 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
     const T* const kh = static_cast<const T*>(a.k.data) + (long long)b * a.k.sb + (long long)hk * a.k.sh;
     const T* const vh = static_cast<const T*>(a.v.data) + (long long)b * a.v.sb + (long long)hk * a.v.sh;
     unsigned char* const ring = ring0 + warp * kStages * 2 * kTileBytes;
+    // this lane's place in the warp's first tile; the tiles of a warp are kStep keys apart and asked for one after another
+    constexpr int kCpr = D * 2 / 16;
+    const T* k_src = kh + (long long)(first + warp * kN + lane / kCpr) * a.k.ss + lane % kCpr * 8;
+    const T* v_src = vh + (long long)(first + warp * kN + lane / kCpr) * a.v.ss + lane % kCpr * 8;
     auto request = [&](int t, int slot) {
         if (t < n_tiles) {
             const uint32_t dst = mm::smem_u32(ring) + slot * 2 * kTileBytes;
-            load_keys<T, D>(dst, kh, a.k.ss, first + t * kN, end, lane);
-            load_keys<T, D>(dst + kTileBytes, vh, a.v.ss, first + t * kN, end, lane);
+            load_keys<T, D>(dst, k_src, kh, a.k.ss, first + t * kN, end, lane);
+            load_keys<T, D>(dst + kTileBytes, v_src, vh, a.v.ss, first + t * kN, end, lane);
+            k_src += (long long)kStep * a.k.ss;
+            v_src += (long long)kStep * a.v.ss;
         }
         mm::cp_async_commit();
     };
 #pragma unroll
-    for (int i = 0; i + 1 < kStages; ++i) request(warp + i * kFewWarps, i);
+    for (int i = 0; i + 1 < kStages; ++i) request(warp + i * kW, i);
     mm::cp_async_wait<kStages - 1>();  // the queries
     __syncthreads();
 
@@ -185,8 +193,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
     }
 
     int slot = 0;
-    for (int t = warp; t < n_tiles; t += kFewWarps) {
-        request(t + (kStages - 1) * kFewWarps, slot >= 1 ? slot - 1 : kStages - 1);
+    for (int t = warp; t < n_tiles; t += kW) {
+        request(t + (kStages - 1) * kW, slot >= 1 ? slot - 1 : kStages - 1);
         mm::cp_async_wait<kStages - 1>();
         __syncwarp();
         unsigned char* const v_ptr = ring + slot * 2 * kTileBytes + kTileBytes;
@@ -329,12 +337,12 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
         l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
     }
 
-    // ---- join of the four warps: their accumulators in the ring, [warp][rows][D + 4] fp32, and (m, l) behind them
+    // ---- join of the warps: their accumulators in the ring, [warp][rows][D + 4] fp32, and (m, l) behind them
     __syncthreads();
     constexpr int kPitch = D + 4;
     float* const acc_s = reinterpret_cast<float*>(ring0);
-    float2* const ml_s = reinterpret_cast<float2*>(ring0 + kFewWarps * kRows * kPitch * 4);
-    static_assert(kFewWarps * kRows * kPitch * 4 + kFewWarps * kRows * 8 <= kFewWarps * kStages * 2 * kTileBytes, "the join fits the ring");
+    float2* const ml_s = reinterpret_cast<float2*>(ring0 + kW * kRows * kPitch * 4);
+    static_assert(kW * kRows * kPitch * 4 + kW * kRows * 8 <= kW * kStages * 2 * kTileBytes, "the join fits the ring");
     {
         float* const mine = acc_s + warp * kRows * kPitch;
 #pragma unroll
@@ -347,18 +355,18 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
         }
     }
     __syncthreads();
-    constexpr int kPer = D / 32;  // values of a lane, a warp takes rows warp, warp + 4, ...
+    constexpr int kPer = D / 32;  // values of a lane, a warp takes rows warp, warp + kW, ...
     const bool cluster = P.chunk == 0 && P.splits > 1;
-    for (int r = warp; r < kRows && row0 + r < P.rows; r += kFewWarps) {
+    for (int r = warp; r < kRows && row0 + r < P.rows; r += kW) {
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, ml_s[w * kRows + r].x);
+        for (int w = 0; w < kW; ++w) top = fmaxf(top, ml_s[w * kRows + r].x);
         const float base = top == -INFINITY ? 0.f : top;
         float sum = 0.f, x[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) x[e] = 0.f;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) {
+        for (int w = 0; w < kW; ++w) {
             const float2 ml = ml_s[w * kRows + r];
             const float f = dense_ex2(ml.x - base);
             sum += ml.y * f;
@@ -385,7 +393,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) dense_few_kernel(const __grid_
     if (!cluster) return;
     // ---- join of the cluster: CTA c takes rows c, c + splits, ..., D / 4 lanes a row
     cluster_sync();
-    constexpr int kLanes = D / 4, kAtOnce = kFewWarps * 32 / kLanes;
+    constexpr int kLanes = D / 4, kAtOnce = kW * 32 / kLanes;
     const int c4 = tid % kLanes;
     for (int r = split + P.splits * (tid / kLanes); r < kRows && row0 + r < P.rows; r += P.splits * kAtOnce) {
         float top = -INFINITY;
@@ -474,7 +482,7 @@ cudaError_t few_launch(const FewParams& P, cudaStream_t st) {
     if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kFewWarps * 32);
+    cfg.blockDim = dim3(kFewWarps<D> * 32);
     cfg.dynamicSmemBytes = few_smem<D, MT>();
     cfg.stream = st;
     cudaLaunchAttribute at{};
