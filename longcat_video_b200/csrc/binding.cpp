@@ -26,21 +26,22 @@ void check(int rc) {
     if (rc != LCBSA_OK) throw LibraryError{rc, lcbsa_last_error()};
 }
 
-// A [B, H, S, D] operand and its description; made contiguous where the 16-byte rules or a missing stride along S ask for it.
+// A [B, H, S, D] operand and its description; copied where the 16-byte rules or a missing stride along S ask for it.  The stride of an axis
+// of one is nobody's: it may be anything and counts for nothing.
 struct Rows {
     at::Tensor t;
     LcbsaTensor d;
 };
 Rows rows(at::Tensor t) {
-    auto st = t.strides();
-    if (st[3] != 1 || ((st[0] | st[1] | st[2]) & 7) || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) || (st[2] == 0 && t.size(2) > 1))
-        t = t.contiguous();
+    auto stride = [&t](int i) { return t.size(i) > 1 ? t.stride(i) : i < 3 ? t.size(3) : 1; };
+    if (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) t = t.clone(at::MemoryFormat::Contiguous);
+    else if (stride(3) != 1 || ((stride(0) | stride(1) | stride(2)) & 7) || (stride(2) == 0)) t = t.contiguous();
     LcbsaTensor d{};
     d.data = t.data_ptr();
     d.dtype = t.scalar_type() == at::kBFloat16 ? LCBSA_BF16 : t.scalar_type() == at::kHalf ? LCBSA_FP16 : LCBSA_FP32;
     for (int i = 0; i < 4; ++i) {
         d.size[i] = t.size(i);
-        d.stride[i] = t.stride(i);
+        d.stride[i] = stride(i);
     }
     return Rows{std::move(t), d};
 }

@@ -82,7 +82,7 @@ __device__ __forceinline__ Seen dense_seen(const DenseMask& m, int b, int i, int
     const int pos = k1 - (q1 - i);  // the last query of a document stands at its last key
     int hi = k1;
     if (m.causal) {
-        const int pre = m.prefix != nullptr ? min(max(__ldg(m.prefix + b * m.prefix_stride + d), 0), Sk) : 0;
+        const int pre = m.prefix != nullptr ? min(max(__ldg(m.prefix + b * m.prefix_stride + d), 0), Sk - k0) : 0;
         hi = min(max(max(pos + 1, k0 + pre), k0), k1);
     }
     return Seen{k0, hi, pos};
@@ -90,11 +90,12 @@ __device__ __forceinline__ Seen dense_seen(const DenseMask& m, int b, int i, int
 
 // A score in units of log2, as the exponent of its probability: x2 = scale log2(e) s, with a cap cap log2(e) tanh(y), y = scale s / cap.
 //
-//   Any y: tanh(y) = 1 - t, t = 2 / (1 + exp(2 y)): two special functions, right at both ends (exp = inf: 1; exp = 0: -1), off by a few
+//   |y| > 1/2: tanh(y) = 1 - t, t = 2 / (1 + exp(2 y)): two special functions, right at both ends (exp = inf: 1; exp = 0: -1), off by a few
 //   2^-24 in between.  (The machine's own tanh is off by 2^-11, which a cap of 50 would make 2 % of a probability.)
-//   |y| <= 1/2: tanh(y) = y p(y^2), p of degree 3 through the Chebyshev nodes of [0, 1/4], off by 4.6 * 2^-23 of the value; with the powers of
-//   scale / cap in its coefficients x2 = s (c0 + t (c1 + t (c2 + t c3))), t = s^2: five operations of the arithmetic units, where the special
-//   functions (16 a clock and SM, one per score already) would take twice as long as the rest of a tile.
+//   |y| <= 1/2, where that difference would cost a large cap its small scores: tanh(y) = y p(y^2), p of degree 3 through the Chebyshev nodes
+//   of [0, 1/4], off by 4.6 * 2^-23 of the value; with the powers of scale / cap (kept between 2^-20 and 2^20 by the entry) in its coefficients
+//   x2 = s (c0 + t (c1 + t (c2 + t c3))), t = s^2: five operations of the arithmetic units, where the special functions (16 a clock and
+//   SM, one per score already) would take twice as long as the rest of a tile.  Most tiles have no other scores and skip the first form.
 struct ScoreShape {
     float mul;     // scale * log2(e)
     float mul_ex;  // 2 * scale / cap * log2(e)
@@ -126,14 +127,7 @@ __device__ __forceinline__ float dense_rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two scores -> cap log2(e) tanh(y), and 1 - tanh(y)^2 (used by the backward)
-__device__ __forceinline__ float2 capped_any(const ScoreShape& f, float2 s, float2& slack) {
-    const float2 t = make_float2(2.f * dense_rcp(1.f + dense_ex2(s.x * f.mul_ex)), 2.f * dense_rcp(1.f + dense_ex2(s.y * f.mul_ex)));
-    const float2 c = make_float2(f.cap2, f.cap2), m = make_float2(-f.cap2, -f.cap2);
-    slack = __fmul2_rn(t, __fadd2_rn(make_float2(2.f, 2.f), make_float2(-t.x, -t.y)));
-    return __ffma2_rn(t, m, c);
-}
-// the same for small scores, plus c
+// Two scores of at most s_small -> cap log2(e) tanh(y) + c, and the same without c and with 1 - tanh(y)^2 (used by the backward)
 __device__ __forceinline__ float2 capped_small_plus(const ScoreShape& f, float2 s, float2 c) {
     auto both = [](float x) { return make_float2(x, x); };
     const float2 t = __fmul2_rn(s, s);
@@ -148,6 +142,15 @@ __device__ __forceinline__ float2 capped_small(const ScoreShape& f, float2 s, fl
     const float2 t = __fmul2_rn(x, make_float2(i, i));
     slack = __ffma2_rn(t, make_float2(-t.x, -t.y), make_float2(1.f, 1.f));
     return x;
+}
+
+// Two scores of any size
+__device__ __forceinline__ float2 capped_any(const ScoreShape& f, float2 s, float2& slack) {
+    const float2 t = make_float2(2.f * dense_rcp(1.f + dense_ex2(s.x * f.mul_ex)), 2.f * dense_rcp(1.f + dense_ex2(s.y * f.mul_ex)));
+    const float2 c = make_float2(f.cap2, f.cap2), m = make_float2(-f.cap2, -f.cap2), small = capped_small_plus(f, s, make_float2(0.f, 0.f));
+    slack = __fmul2_rn(t, __fadd2_rn(make_float2(2.f, 2.f), make_float2(-t.x, -t.y)));
+    const float2 x = __ffma2_rn(t, m, c);
+    return make_float2(fabsf(s.x) <= f.s_small ? small.x : x.x, fabsf(s.y) <= f.s_small ? small.y : x.y);
 }
 
 // The bias of n columns whose keys lie on one side of the query, plus a constant: plus - slope |at - j| is a line in the column's number j.

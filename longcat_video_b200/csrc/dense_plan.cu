@@ -64,7 +64,7 @@ __device__ __forceinline__ void plan_cta(const DenseArgs& a, int cta, int b, int
         if (k_first >= k1) q_end = 0;
     }
     if (m.causal) {
-        const int pre = m.prefix != nullptr ? min(max(__ldg(m.prefix + b * m.prefix_stride + d), 0), a.Sk) : 0;
+        const int pre = m.prefix != nullptr ? min(max(__ldg(m.prefix + b * m.prefix_stride + d), 0), a.Sk - k0) : 0;
         const int key = max(k_first, k0);
         if (key >= k0 + pre) q0 = max(q0, q1 - (k1 - key));
     }

@@ -37,6 +37,8 @@ def _shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, sc
         raise ValueError(f"softcap {softcap}: 0 (none) or a positive number")
     if not math.isfinite(scale):
         raise ValueError(f"scale {scale} is not finite")
+    if softcap and scale and not 2.0 ** -20 <= abs(scale) / softcap <= 2.0 ** 20:
+        raise ValueError(f"softcap {softcap}: further than a factor of 2^20 from scale {scale}")
     docs = 1
     if cu_q is not None or cu_k is not None:
         if cu_q is None:
@@ -75,7 +77,8 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
     """softmax(x) v over the keys that a query sees, x_ij = cap tanh(scale q_i k_j / cap) - slope |pos_i - j|.
 
     ``q [B, Hq, Sq, D]``, ``k``, ``v`` ``[B, Hk, Sk, D]``, bf16 or fp16, D 64 or 128, Hq a multiple of Hk (query head h reads key head
-    ``h // (Hq // Hk)``), any strides with D contiguous.  ``scale`` defaults to ``D ** -0.5``; ``softcap`` 0 caps nothing;
+    ``h // (Hq // Hk)``), any strides with D contiguous.  ``scale`` defaults to ``D ** -0.5``; ``softcap`` 0 caps nothing,
+    others lie within a factor of 2^20 of ``scale``;
     ``slopes [Hq]`` (constants) weigh the distance between the query's place among the keys and the key.
 
     Which keys a query sees: all of its batch entry's; with ``k_lens [B]`` the first that many (a padded cache); with ``cu_q``

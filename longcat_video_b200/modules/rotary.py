@@ -44,8 +44,10 @@ def _frequencies(rotary_dim: int, base: float, scaling) -> RotaryFrequencies:
     if kind is not None:
         if kind not in _KINDS or set(s) - _KINDS[kind] - {"kind"}:
             raise ValueError(f"scaling {s}: one of {sorted(_KINDS)} with its own parameters")
-        if not factor >= 1.0:
+        if not (math.isfinite(factor) and factor >= 1.0):
             raise ValueError(f"scaling factor {factor}: at least 1")
+        if "original_length" in _KINDS[kind] and not s.get("original_length", 0) > 0:
+            raise ValueError(f"scaling {s}: needs the original_length, a positive number")
     if kind == "base":
         if rotary_dim == 2:
             raise ValueError("scaling by the base needs more than one pair")

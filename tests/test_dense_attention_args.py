@@ -54,6 +54,26 @@ def test_shapes_are_checked(kw):
         _shape_of(q, q, **{**base, "k_lens": torch.ones(2)})
 
 
+def test_a_cap_far_from_the_scale_is_refused():
+    q = torch.zeros(2, 2, 4, 64, dtype=torch.bfloat16)
+    for cap, scale, ok in ((131072.0, None, True), (131073.0, None, False), (1e-7, None, False), (1.0, -2.0 ** 20, True), (1.0, 2.0 ** -21, False), (5.0, 0.0, True)):
+        if ok:
+            assert _shape_of(q, q, False, cap, None, None, None, None, None, scale)[1] == cap
+        else:
+            with pytest.raises(ValueError, match="2\\^20"):
+                _shape_of(q, q, False, cap, None, None, None, None, None, scale)
+    d = _desc(2, 4, 64, 128)
+    rc, msg = _fwd(d, d, d, _scores(scale=1.0, cap=2e6), d)
+    assert rc == -1 and "2^20" in msg
+
+
+def test_scalings_name_what_is_missing():
+    from longcat_video_b200.modules import rotary_frequencies
+    for scaling in ({"kind": "by_parts", "factor": 4.0}, {"kind": "by_wavelength", "factor": 4.0, "original_length": 0}, {"kind": "linear", "factor": math.inf}):
+        with pytest.raises(ValueError):
+            rotary_frequencies(64, 10000.0, scaling)
+
+
 def test_the_library_refuses_before_a_launch():
     q, k = _desc(2, 4, 64, 128), _desc(2, 2, 100, 128)
     ok = _scores()

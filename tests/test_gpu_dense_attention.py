@@ -229,6 +229,48 @@ def test_strides_and_broadcast():
         assert torch.equal(a, b)
 
 
+def _unaligned(t):
+    """The same values behind eight bytes of something else, in a storage whose batch stride is odd where there is one batch entry."""
+    flat = torch.zeros(2, t.numel() + 9, dtype=t.dtype, device=t.device)
+    view = flat[1, 4:4 + t.numel()].view(t.shape)
+    if t.shape[0] == 1:
+        view = flat.as_strided(t.shape, (t.numel() + 9, *t.stride()[1:]), 8)
+    return view.copy_(t)
+
+
+def test_unaligned_and_single_entry_views():
+    for B in (1, 2):
+        q, k, v, dout = _inputs(B, 4, 2, 100, 100, 64, torch.float16, seed=8)
+        leaves = [x.requires_grad_() for x in (q, k, v)]
+        out = _dense()(*leaves, causal=True)
+        want = [out, *torch.autograd.grad(out, leaves, dout)]
+        odd = [_unaligned(x.detach()).requires_grad_() for x in (q, k, v)]
+        assert all(x.is_contiguous() for x in odd)
+        out = _dense()(*odd, causal=True)
+        assert all(torch.equal(a, b) for a, b in zip(want, [out, *torch.autograd.grad(out, odd, _unaligned(dout))]))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("impl", [TC, MMA])
+def test_a_large_cap_keeps_small_scores(impl, D):
+    """A cap far above the scores changes nothing, in tiles with scores on its own scale too: the rows whose scores are small keep the bounds
+    of every other case (the others' scores are off by 2^-24 of 10^5 and more; their dout is zero)."""
+    B, Hq, Hk, S = 1, 4, 2, 150
+    q, k, v, dout = _inputs(B, Hq, Hk, S, S, D, torch.bfloat16, seed=9)
+    small = torch.arange(S, device="cuda") % 50 != 7
+    q = torch.where(small[:, None], q, q * 3e5)
+    dout = dout * small[:, None]
+    lo, hi, pos = R.runs(B, S, S, True, None, None, None)
+    for cap in (80000.0, 2000.0):
+        want = R.attend(q, k, v, lo, hi, pos, D ** -0.5, cap, None, dout)
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = _dense()(*leaves, causal=True, softcap=cap, impl=impl)
+        assert R.worst(out[:, :, small], [x[:, :, small] for x in want["o"]]) <= 1
+        grads = torch.autograd.grad(out, leaves, dout)
+        assert R.worst(grads[0][:, :, small], [x[:, :, small] for x in want["dq"]]) <= 1
+        assert R.worst(grads[1], want["dk"]) <= 1 and R.worst(grads[2], want["dv"]) <= 1
+
+
 @pytest.mark.parametrize("impl", [TC, MMA])
 def test_two_calls_give_the_same_bits(impl):
     q, k, v, dout = _inputs(2, 8, 2, 500, 500, 128, torch.bfloat16)
