@@ -664,41 +664,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                     const float2 base = make_float2(-m_eff, -m_eff);
                     const float at = kBias ? (float)(see.z - key0) : 0.f;
                     const bool both_sides = kBias && __any_sync(0xffffffffu, at > 0.f && at < (float)(kBlk - 1));
-                    auto exponents = [&](auto shaped, bool two_sides) {
-                        BiasLine line;
-                        if (kBias && !two_sides) line = bias_line(at, f.slope2, -m_eff);
-#pragma unroll
-                        for (int j = 0; j < 64; j += 2) {
-                            float2 c = base;
-                            if (kBias) {
-                                if (two_sides) c = __ffma2_rn(make_float2(fabsf(at - (float)j), fabsf(at - (float)(j + 1))), make_float2(-f.slope2, -f.slope2), base);
-                                else c = bias_next(line, j / 2);
-                            }
-                            put2(sr, j, shaped(get2(sr, j), c));
-                        }
-                    };
-                    if constexpr (kCap) {
-                        const bool large = __any_sync(0xffffffffu, !(row_size(sr) <= f.s_small));
-                        auto any = [&](float2 s, float2 c) { float2 slack; return __fadd2_rn(capped_any(f, s, slack), c); };
-                        auto small = [&](float2 s, float2 c) { return capped_small_plus(f, s, c); };
-                        if (LCBSA_UNLIKELY(large)) exponents(any, true);
-                        else if (kBias && both_sides) exponents(small, true);
-                        else exponents(small, false);
-                    } else {
-                        auto plain = [&](float2 s, float2 c) { return __ffma2_rn(s, make_float2(f.mul, f.mul), c); };
-                        if (kBias && both_sides) exponents(plain, true);
-                        else exponents(plain, false);
-                    }
-                    if (mixed_unit(cur, i)) {
-                        const int lo = min(max(see.x - key0, 0), kBlk), hi = min(max(see.y - key0, 0), kBlk);  // a run of bits
-                        const uint64_t sees = hi > lo ? (~0ull >> (kBlk - (hi - lo))) << lo : 0ull;
-                        const uint32_t s_lo = (uint32_t)sees, s_hi = (uint32_t)(sees >> 32);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            if (!((s_lo >> j) & 1u)) sr[j] = 0xff800000u;  // -inf
-                            if (!((s_hi >> j) & 1u)) sr[32 + j] = 0xff800000u;
-                        }
-                    }
+                    auto plain = [&](float2 s, float2 c) { return __ffma2_rn(s, make_float2(f.mul, f.mul), c); };
+                    auto small = [&](float2 s, float2 c) { return capped_small_plus(f, s, c); };
+                    auto any = [&](float2 s, float2 c) { float2 slack; return __fadd2_rn(capped_any(f, s, slack), c); };
                     auto row_max = [&]() {
                         float mx8[8];  // eight chains of eight values, three at a time
 #pragma unroll
@@ -713,25 +681,15 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
 #pragma unroll
                         for (int j = 0; j < 64; j += 2) put2(sr, j, __fadd2_rn(get2(sr, j), b2));
                     };
-                    // The first unit in which the row sees a key takes its own maximum as the reference.
-                    if (LCBSA_UNLIKELY(first)) {
-                        const float m = row_max();
-                        if (m != -INFINITY) {
-                            m_ref = m;
-                            first = false;
-                            shift(m);
-                        }
-                    }
-                    // The probabilities are computed against the current reference while the row maximum is tracked beside them;
-                    // only if it has moved by more than 2^8 is the pass repeated with the new reference.
-                    auto probs = [&](float& rsum) {
+                    // Probabilities against the current reference, the row sum before their rounding.  exponent(pair number) gives two exponents.
+                    auto probs = [&](float& rsum, auto exponent) {
                         float2 r01 = make_float2(0.f, 0.f), r23 = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int cch = 0; cch < 8; ++cch) {
                             float2 e[4];
 #pragma unroll
                             for (int jp = 0; jp < 4; ++jp) {
-                                const float2 x = get2(sr, cch * 8 + 2 * jp);
+                                const float2 x = exponent(cch * 4 + jp);
                                 e[jp] = make_float2(ex2(x.x), ex2(x.y));
                             }
                             r01 = __fadd2_rn(r01, e[0]);
@@ -745,15 +703,74 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                         }
                         rsum = (r01.x + r01.y) + (r23.x + r23.y);
                     };
+                    auto ready_made = [&](int pair) { return get2(sr, 2 * pair); };
+                    bool large = false;
+                    if constexpr (kCap) large = __any_sync(0xffffffffu, !(row_size(sr) <= f.s_small));
+                    const bool mixed = mixed_unit(cur, i);
                     float rs = 0.f;
-                    probs(rs);
+                    // With a cap the exponents of the usual unit are made in the same pass as its probabilities, so that the arithmetic of one pair runs
+                    // under the special functions of another (16 heads, 8192 tokens: 642 us in two passes, 549 in one).  Without one there
+                    // is too little of it (453 and 467 us): the other units' way, exponents first, is every unit's.
+                    constexpr bool kOnePass = kCap;
+                    if (!kOnePass || LCBSA_UNLIKELY(mixed || large || both_sides || __any_sync(0xffffffffu, first))) {
+                        auto exponents = [&](auto shaped, bool two_sides) {
+                            BiasLine line;
+                            if (kBias && !two_sides) line = bias_line(at, f.slope2, -m_eff);
+#pragma unroll
+                            for (int j = 0; j < 64; j += 2) {
+                                float2 c = base;
+                                if (kBias) {
+                                    if (two_sides) c = __ffma2_rn(make_float2(fabsf(at - (float)j), fabsf(at - (float)(j + 1))), make_float2(-f.slope2, -f.slope2), base);
+                                    else c = bias_next(line, j / 2);
+                                }
+                                put2(sr, j, shaped(get2(sr, j), c));
+                            }
+                        };
+                        if constexpr (kCap) {
+                            if (LCBSA_UNLIKELY(large)) exponents(any, true);
+                            else exponents(small, true);
+                        } else {
+                            if (kBias && both_sides) exponents(plain, true);
+                            else exponents(plain, false);
+                        }
+                        if (mixed) {
+                            const int lo = min(max(see.x - key0, 0), kBlk), hi = min(max(see.y - key0, 0), kBlk);  // a run of bits
+                            const uint64_t sees = hi > lo ? (~0ull >> (kBlk - (hi - lo))) << lo : 0ull;
+                            const uint32_t s_lo = (uint32_t)sees, s_hi = (uint32_t)(sees >> 32);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                if (!((s_lo >> j) & 1u)) sr[j] = 0xff800000u;  // -inf
+                                if (!((s_hi >> j) & 1u)) sr[32 + j] = 0xff800000u;
+                            }
+                        }
+                        // The first unit in which the row sees a key takes its own maximum as the reference.
+                        if (LCBSA_UNLIKELY(first)) {
+                            const float m = row_max();
+                            if (m != -INFINITY) {
+                                m_ref = m;
+                                first = false;
+                                shift(m);
+                            }
+                        }
+                        probs(rs, ready_made);
+                    } else {
+                        BiasLine line;
+                        if (kBias) line = bias_line(at, f.slope2, -m_eff);
+                        probs(rs, [&](int pair) {
+                            const float2 s = get2(sr, 2 * pair), c = kBias ? bias_next(line, pair) : base;
+                            const float2 x = small(s, c);
+                            put2(sr, 2 * pair, x);
+                            return x;
+                        });
+                    }
+                    // The row maximum was tracked beside them; only if it has moved by more than 2^8 is the pass repeated with the new reference.
                     const float m_top = row_max();
                     if (LCBSA_UNLIKELY(m_top > 8.f)) {
                         need = true;
                         alpha = ex2(-m_top);
                         m_ref += m_top;
                         shift(m_top);
-                        probs(rs);
+                        probs(rs, ready_made);
                     }
                     l_sum = l_sum * alpha + rs;  // alpha is 1 unless this row's reference maximum moved
                 }
