@@ -16,8 +16,10 @@
 // (five operations per pair of scores for a cap, one for a bias: see ScoreShape and BiasLine).
 //
 // Bound by the softmax warps: 8192 exponentials of a unit take 512 of the 1024 cycles that its two products take, and the
-// warps that compute them wait for each other's S and PV.  37 heads of 4096 tokens, head_dim 128: 540 ns a unit (1.1 PFLOP/s), 730 with a cap, 720
-// with a bias, 920 with both; at 37 x 2048 under the profiler the tensor pipe is 48 % busy, 34 % with a cap, issue slots 43 %.
+// warps that compute them wait for each other's S and PV.  37 heads of 4096 tokens, head_dim 128: 540 ns a unit (1.1 PFLOP/s), 690 with a cap, 630
+// with a bias, 760 with both; at 37 x 2048 under the profiler the tensor pipe is 47 % busy, 35 % with a cap, issue slots 43 and 45 %.  Every eighth
+// pair of exponentials on the arithmetic pipes instead (a polynomial of degree 4): 455 us in the place of 447 at head_dim 128, 412 of 434 at 64;
+// every fourth 471 and 413: not worth a second kind.
 //
 // Hidden values may be anything.  A score that is not finite stays in its column and is replaced there.  V enters the product of every row
 // of the tile, so in mixed units its producer looks through the tile first: values that are not finite are set to zero, and the epilogue adds
