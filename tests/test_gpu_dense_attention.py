@@ -229,6 +229,48 @@ def test_strides_and_broadcast():
         assert torch.equal(a, b)
 
 
+WALKS = {  # with a distance the units of keys come in another order than the keys
+    "all_seen": ((1, 3, 1, 700, 700), dict(slopes=True)),
+    "more_keys": ((2, 2, 2, 200, 900), dict(slopes=True, cap=30.0)),
+    "more_queries": ((1, 2, 1, 900, 200), dict(slopes=True)),  # the first queries stand before the first key
+    "prefix_far_ahead": ((1, 2, 2, 600, 600), dict(slopes=True, causal=True, prefix=[[500]])),
+    "documents_of_other_lengths": ((1, 2, 2, 500, 640), dict(slopes=True, docs=[([0, 60, 61, 400, 480], [0, 300, 300, 420, 640])])),
+    "lengths": ((3, 2, 1, 150, 520), dict(slopes=True, k_lens=[520, 1, 333])),
+}
+
+
+@pytest.mark.parametrize("impl", [TC, MMA])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("name", WALKS)
+def test_walks_with_a_distance(name, D, impl):
+    B, Hq, Hk, Sq, Sk = WALKS[name][0]
+    lo, hi, pos, kw, scale, _ = _options(WALKS[name], torch.bfloat16, D)
+    q, k, v, _ = _inputs(B, Hq, Hk, Sq, Sk, D, torch.bfloat16, seed=11)
+    want = R.attend(q, k, v, lo, hi, pos, scale, kw["softcap"], kw["slopes"])
+    out, lse = _dense()(q, k, v, return_lse=True, impl=impl, **kw)
+    assert R.worst(out, want["o"]) <= 1
+    blind = torch.isinf(want["lse"])
+    assert torch.equal(torch.isinf(lse), blind) and float((lse.double() - want["lse"])[~blind].abs().max()) <= R.SCORE + 1e-5
+    v[:, :, 300 % Sk, 5] = math.inf  # seen by some rows of mixed tiles, by all of whole ones
+    lo, hi = (x.to("cuda")[:, None] for x in (lo, hi))
+    sees = ((lo <= 300 % Sk) & (hi > 300 % Sk)).expand(B, Hq, Sq)
+    out = _dense()(q, k, v, impl=impl, **kw)
+    assert torch.isfinite(out[..., :5]).all() and torch.isfinite(out[..., 5][~sees]).all() and not torch.isfinite(out[..., 5][sees]).any()
+
+
+@pytest.mark.parametrize("impl", [TC, MMA])
+@pytest.mark.parametrize("cap", [0.0, 400.0])
+def test_a_reference_that_moves(impl, cap):
+    """Keys from 640 on have scores of four times the size, so that the maximum of most rows jumps there, in whole units and in mixed ones.
+    Sums of |q_d k_d| scale stay below 128 * 6 * 4 * 0.64 * 0.02 = 39 on average."""
+    q, k, v, _ = _inputs(1, 4, 2, 1100, 1100, 128, torch.bfloat16, seed=12, spread=6.0)
+    k[:, :, 640:] *= 4
+    lo, hi, pos = R.runs(1, 1100, 1100, True, None, None, None)
+    want = R.attend(q, k, v, lo, hi, pos, 0.02, cap)
+    out, lse = _dense()(q, k, v, causal=True, scale=0.02, softcap=cap, return_lse=True, impl=impl)
+    assert R.worst(out, want["o"]) <= 1 and float((lse.double() - want["lse"]).abs().max()) <= R.SCORE + 1e-5
+
+
 def _unaligned(t):
     """The same values behind eight bytes of something else, in a storage whose batch stride is odd where there is one batch entry."""
     flat = torch.zeros(2, t.numel() + 9, dtype=t.dtype, device=t.device)
