@@ -688,17 +688,17 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                                 if (two_sides) c = __ffma2_rn(far, make_float2(-slope2, -slope2), c);
                                 else c = __fadd2_rn(c, bias_next(line, k));
                             }
-                            p[k] = probs(two(x[2 * k], x[2 * k + 1]), c, lg, slack);
+                            float2 w = probs(two(x[2 * k], x[2 * k + 1]), c, lg, slack);
+                            p[k] = __fmul2_rn(w, make_float2(P.scale, P.scale));
+                            if (kCap) p[k] = __fmul2_rn(p[k], slack);
                             if (mx) {
                                 const float4 d4 = st4[16 + (k >> 1)];
-                                if (!isfinite(k & 1 ? d4.z : d4.x)) p[k].x = __int_as_float(0x7fc00000);  // dO is not finite
-                                if (!isfinite(k & 1 ? d4.w : d4.y)) p[k].y = __int_as_float(0x7fc00000);
-                                if (key < a.x || key >= a.y) p[k].x = 0.f;
-                                if (key < d.x || key >= d.y) p[k].y = 0.f;
+                                if (!isfinite(k & 1 ? d4.z : d4.x)) w.x = p[k].x = __int_as_float(0x7fc00000);  // dO is not finite
+                                if (!isfinite(k & 1 ? d4.w : d4.y)) w.y = p[k].y = __int_as_float(0x7fc00000);
+                                if (key < a.x || key >= a.y) w.x = p[k].x = 0.f;  // last: the slack of a hidden score may be NaN
+                                if (key < d.x || key >= d.y) w.y = p[k].y = 0.f;
                             }
-                            out[k] = pack2(kBf16, p[k].x, p[k].y);
-                            p[k] = __fmul2_rn(p[k], make_float2(P.scale, P.scale));
-                            if (kCap) p[k] = __fmul2_rn(p[k], slack);
+                            out[k] = pack2(kBf16, w.x, w.y);
                         }
                     };
                     if (kCap && LCBSA_UNLIKELY(large)) all(true, true, true);
