@@ -48,7 +48,7 @@ struct DenseArgs {
     int4* seen;            // [B, units, 65]: lo, hi, pos, 0 of a unit's 64 queries (those behind the last see nothing), then
                            // min lo, max hi over the queries that see a key, max lo, min hi over all of them
     int2* hulls;           // [B, key units]: first and one past the last query that can see a key of the unit (backward)
-    float* stats;          // [B*Hq, units, 2, 64]: -lse * log2(e) and -rowsum(dout * out) of a unit's queries, 0 behind the last (backward)
+    float* stats;          // [B*Hq, units, 2, 64]: -lse * log2(e) and -rowsum(dout * out) of a unit's queries, -inf and 0 behind the last (backward)
     float* part;           // sums of dk and dv of parts of a group of heads (backward)
     int* next_item;        // items taken by the persistent kernels, zero when they start
 };

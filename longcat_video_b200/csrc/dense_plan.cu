@@ -75,7 +75,8 @@ __device__ __forceinline__ void plan_cta(const DenseArgs& a, int cta, int b, int
 
 // Backward: rowsum(dout * out) in fp32, out with what its rounding left: a half step of out moves dS by as much as rounding dS does (dq
 // of a causal row of 600 keys, bf16, is off by 1.53 times its own rounding without the rest, 1.46 with it).  D / 8 lanes a row; rows
-// behind the last query of their unit get zeros.
+// behind the last query get a probability of zero (-lse of -inf) whatever their distance to a key counts for: their entries are not
+// masked in a unit that is whole.
 template <typename T, int D>
 __device__ __forceinline__ void stats_cta(const DenseArgs& a, long long cta) {
     constexpr int kLanes = D / 8;
@@ -98,7 +99,7 @@ __device__ __forceinline__ void stats_cta(const DenseArgs& a, long long cta) {
     for (int x = kLanes / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
     if (sub == 0) {
         float* dst = a.stats + r / kDenseUnit * kDenseStats + r % kDenseUnit;
-        dst[0] = i < a.Sq ? -(a.lse[bh * a.Sq + i] * kLog2e) : 0.f;
+        dst[0] = i < a.Sq ? -(a.lse[bh * a.Sq + i] * kLog2e) : -INFINITY;
         dst[kDenseUnit] = i < a.Sq ? -s : 0.f;
     }
 }

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import dense_reference as R
-from tests.test_gpu_dense_attention import _dense, _inputs
+from tests.test_gpu_dense_attention import MMA, TC, _dense, _inputs, _slopes
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,41 @@ def test_documents_keep_their_gradients_apart(cap, poison, D, dtype):
         val, bound = want[x]
         assert R.worst(got[:, :, rows], (val[:, :, rows], bound[:, :, rows])) <= 1, x
         assert not got[:, :, outside].any(), x
+
+
+# ---- slopes below zero -------------------------------------------------------------------------------------------------------------
+
+NEGATIVE = {  # the last unit of 64 queries is not full, and keys far from it are seen by all of its queries
+    "all_seen": ((1, 4, 2, 330, 330), dict()),
+    "all_seen_short": ((2, 2, 2, 100, 100), dict()),
+    "causal": ((1, 4, 2, 330, 330), dict(causal=True)),
+    "causal_prefix": ((1, 2, 1, 290, 290), dict(causal=True, prefix=[[200]])),
+    "one_query": ((2, 4, 2, 1, 300), dict()),
+    "documents": ((1, 2, 2, 415, 415), dict(docs=[([0, 60, 415], [0, 60, 415])])),
+}
+
+
+@pytest.mark.parametrize("impl", [TC, MMA])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+@pytest.mark.parametrize("name", NEGATIVE)
+def test_slopes_below_zero(name, D, dtype, cap, impl):
+    """A distance that counts for a key: far keys weigh most.  x is at most 40 + 0.5 * 415 in size, so the distance in fp32 is off by 2^-24 of 250,
+    1.5e-5, which SCORE has room for."""
+    (B, Hq, Hk, Sq, Sk), o = NEGATIVE[name]
+    docs, prefix, causal = o.get("docs"), o.get("prefix"), o.get("causal", False)
+    lo, hi, pos = R.runs(B, Sq, Sk, causal, docs, None, prefix)
+    slopes = -_slopes(Hq)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    kw = dict(causal=causal, softcap=cap, slopes=slopes, impl=impl)
+    if docs:
+        kw["cu_q"], kw["cu_k"] = ints(docs[0][0]), ints(docs[0][1])
+    if prefix:
+        kw["prefix_lens"] = ints(prefix[0])
+    q, k, v, dout = _inputs(B, Hq, Hk, Sq, Sk, D, dtype, seed=21)
+    want = R.attend(q, k, v, lo, hi, pos, 1 / math.sqrt(D), cap, slopes, dout)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = _dense()(*leaves, **kw)
+    grads = torch.autograd.grad(out, leaves, dout)
+    for got, x in zip((out.detach(), *grads), ("o", "dq", "dk", "dv")):
+        assert R.worst(got, want[x]) <= 1, x
