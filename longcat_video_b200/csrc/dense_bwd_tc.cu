@@ -129,7 +129,7 @@ __device__ __forceinline__ void store_row32(unsigned char* row_ptr, int col0, co
 }
 
 // whether one of the scores is too large for the polynomial of the cap (a NaN is passed over: it stays one through it)
-__device__ __forceinline__ bool any_large(const uint32_t (&r)[32], float s_small) {
+__device__ __forceinline__ bool any_large(const uint32_t (&r)[32], float s_fast) {
     float m[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -137,7 +137,7 @@ __device__ __forceinline__ bool any_large(const uint32_t (&r)[32], float s_small
 #pragma unroll
         for (int j = 0; j < 8; j += 2) m[k] = max3(m[k], fabsf(__uint_as_float(r[8 * k + j])), fabsf(__uint_as_float(r[8 * k + j + 1])));
     }
-    return __any_sync(0xffffffffu, !(fmaxf(max3(m[0], m[1], m[2]), m[3]) <= s_small));
+    return __any_sync(0xffffffffu, !(fmaxf(max3(m[0], m[1], m[2]), m[3]) <= s_fast));
 }
 
 // kMode 0: dQ pass, 1: dK/dV pass.  Persistent, one CTA per SM.
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                     tc_fence_before();
                     mbar_arrive_elect(bar_s_free(wg));
                 }
-                const bool large = kCap && any_large(x, P.shape.s_small);
+                const bool large = kCap && any_large(x, P.shape.s_fast);
                 bool mixed;
                 const float4* const st4 = reinterpret_cast<const float4*>(smem + Ly::offExtra + slot * Ly::extra) + 8 * half;  // dK/dV pass
                 if constexpr (kMode == 0) {

@@ -9,6 +9,7 @@
 #pragma once
 #include <cuda.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "common.cuh"
@@ -96,12 +97,17 @@ __device__ __forceinline__ Seen dense_seen(const DenseMask& m, int b, int i, int
 //   of [0, 1/4], off by 4.6 * 2^-23 of the value; with the powers of scale / cap (kept between 2^-20 and 2^20 by the entry) in its coefficients
 //   x2 = s (c0 + t (c1 + t (c2 + t c3))), t = s^2: five operations of the arithmetic units, where the special functions (16 a clock and
 //   SM, one per score already) would take twice as long as the rest of a tile.  Most tiles have no other scores and skip the first form.
+//   At the low end of the range c3 is rounded to the grid of 2^-149, which moves x2 by 2^-150 s^7 <= 2^-17.  At the high end scale (scale / cap)^6
+//   passes 2^128 for scales of 2^8 and more: there y = s scale / cap is formed first, the coefficients are those of y, and every tile takes
+//   the way of the large scores.
 struct ScoreShape {
     float mul;     // scale * log2(e)
     float mul_ex;  // 2 * scale / cap * log2(e)
     float cap2;    // cap * log2(e)
-    float c[4];
+    float unit;    // 1, or scale / cap where the powers of that are not in the coefficients
+    float c[4];    // of (unit s)
     float s_small; // scores up to this magnitude go through the polynomial
+    float s_fast;  // s_small if the polynomial of s itself serves them, else -1: no score does without the factor `unit`
     float slope2;  // slope of the head * log2(e)
 };
 inline ScoreShape score_shape(float scale, float cap) {
@@ -111,9 +117,12 @@ inline ScoreShape score_shape(float scale, float cap) {
     s.mul = (float)(scale * e);
     s.mul_ex = (float)(2.0 * y * e);
     s.cap2 = (float)(cap * e);
-    double f = scale * e;
-    for (int i = 0; i < 4; ++i, f *= y * y) s.c[i] = (float)(f * p[i]);
+    const bool fits = std::fabs(scale * e * p[3] * y * y * y * y * y * y) < 0x1p127;  // the others are finite then, too
+    s.unit = fits ? 1.f : (float)y;
+    double f = fits ? scale * e : cap * e;
+    for (int i = 0; i < 4; ++i, f *= fits ? y * y : 1.0) s.c[i] = (float)(f * p[i]);
     s.s_small = y != 0.0 ? (float)(0.5 / (y < 0 ? -y : y)) : 0.f;
+    s.s_fast = fits ? s.s_small : -1.f;
     s.slope2 = 0.f;
     return s;
 }
@@ -127,7 +136,7 @@ __device__ __forceinline__ float dense_rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two scores of at most s_small -> cap log2(e) tanh(y) + c, and the same without c and with 1 - tanh(y)^2 (used by the backward)
+// Two scores of at most s_fast, times the unit, -> cap log2(e) tanh(y) + c, and the same without c and with 1 - tanh(y)^2 (used by the backward)
 __device__ __forceinline__ float2 capped_small_plus(const ScoreShape& f, float2 s, float2 c) {
     auto both = [](float x) { return make_float2(x, x); };
     const float2 t = __fmul2_rn(s, s);
@@ -147,7 +156,8 @@ __device__ __forceinline__ float2 capped_small(const ScoreShape& f, float2 s, fl
 // Two scores of any size
 __device__ __forceinline__ float2 capped_any(const ScoreShape& f, float2 s, float2& slack) {
     const float2 t = make_float2(2.f * dense_rcp(1.f + dense_ex2(s.x * f.mul_ex)), 2.f * dense_rcp(1.f + dense_ex2(s.y * f.mul_ex)));
-    const float2 c = make_float2(f.cap2, f.cap2), m = make_float2(-f.cap2, -f.cap2), small = capped_small_plus(f, s, make_float2(0.f, 0.f));
+    const float2 c = make_float2(f.cap2, f.cap2), m = make_float2(-f.cap2, -f.cap2);
+    const float2 small = capped_small_plus(f, __fmul2_rn(s, make_float2(f.unit, f.unit)), make_float2(0.f, 0.f));
     slack = __fmul2_rn(t, __fadd2_rn(make_float2(2.f, 2.f), make_float2(-t.x, -t.y)));
     const float2 x = __ffma2_rn(t, m, c);
     return make_float2(fabsf(s.x) <= f.s_small ? small.x : x.x, fabsf(s.y) <= f.s_small ? small.y : x.y);

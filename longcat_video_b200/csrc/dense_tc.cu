@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                     };
                     auto ready_made = [&](int pair) { return get2(sr, 2 * pair); };
                     bool large = false;
-                    if constexpr (kCap) large = __any_sync(0xffffffffu, !(row_size(sr) <= f.s_small));
+                    if constexpr (kCap) large = __any_sync(0xffffffffu, !(row_size(sr) <= f.s_fast));
                     const bool mixed = mixed_unit(cur, i);
                     float rs = 0.f;
                     // With a cap the exponents of the usual unit are made in the same pass as its probabilities, so that the arithmetic of one pair runs

@@ -72,3 +72,29 @@ def test_slopes_below_zero(name, D, dtype, cap, impl):
     grads = torch.autograd.grad(out, leaves, dout)
     for got, x in zip((out.detach(), *grads), ("o", "dq", "dk", "dv")):
         assert R.worst(got, want[x]) <= 1, x
+
+
+# ---- scales and caps at both ends of what is accepted ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("impl", [TC, MMA])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scale,cap", [(2.0 ** 20, 1.0), (-2.0 ** 20, 1.0), (4096.0, 2.0 ** -8), (2.0 ** 40, 2.0 ** 22), (2.0 ** 90, 4.0 * 2.0 ** 70),
+                                       (1.0, 2.0 ** 20), (2.0 ** -4, 2.0 ** 16), (2.0 ** -40, 2.0 ** -20)])
+def test_scales_far_from_their_cap(scale, cap, D, impl):
+    """Scores of some units of the cap or of one, whichever is less, among them rows and keys of zeros: the formulas' bounds, whatever powers of
+    scale and cap come to in 32 bits.  The inputs keep sums of |q_d k_d| scale below 40: q is 2^e / scale times a normal number."""
+    B, Hq, Hk, S = 1, 4, 2, 150
+    q, k, v, dout = _inputs(B, Hq, Hk, S, S, D, torch.bfloat16, seed=22)
+    size = min(1.0, 4 * cap) * (0.5 if D == 64 else 0.25)
+    q = (q.float() * (size / abs(scale))).bfloat16()
+    q[:, :, 10:20] = 0
+    k[:, :, 30:35] = 0
+    q[:, :, 140] *= 2.0 ** -6
+    lo, hi, pos = R.runs(B, S, S, True, None, None, None)
+    want = R.attend(q, k, v, lo, hi, pos, scale, cap, None, dout)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out, lse = _dense()(*leaves, causal=True, scale=scale, softcap=cap, return_lse=True, impl=impl)
+    assert R.worst(out.detach(), want["o"]) <= 1
+    assert float((lse.double() - want["lse"]).abs().max()) <= R.SCORE + 1e-5
+    for got, x in zip(torch.autograd.grad(out, leaves, dout), ("dq", "dk", "dv")):
+        assert R.worst(got, want[x]) <= 1, x
