@@ -319,6 +319,7 @@ int lcbsa_norm_rope_jobs(const LcbsaRowJob* jobs, int n_jobs, float eps, void* s
  * entries prefix_stride apart; null: none).  Bounds outside the tensors are clamped, never followed.
  * Keys and values that no query of a call sees, and those hidden from a query, may hold anything, infinities and NaN included.
  *
+ * scale, cap: finite, up to 2^126 in size, cap 0 or within a factor of 2^20 of the size of scale (scale 0: any cap).
  * lse: fp32 dense [B, Hq, Sq], natural log, nullable in the forward.  A row with a NaN or +inf score is NaN, its lse too.
  * rest: nullable, dense [B, Hq, Sq, D] in the type of q: what rounding out to its type left.  A backward that is given it takes
  * rowsum(dout * out) from both, which halves what that sum adds to the error of dq and dk.

@@ -572,6 +572,8 @@ static int dense_args(const char* what, const LcbsaTensor* q, const LcbsaTensor*
     if (k->size[1] < 1 || q->size[1] < 1 || q->size[1] % k->size[1] != 0)
         return fail(LCBSA_EINVAL, "%s: %lld query heads do not share %lld key heads evenly", what, (long long)q->size[1], (long long)k->size[1]);
     if (!std::isfinite(sc->scale) || !std::isfinite(sc->cap) || sc->cap < 0.f) return fail(LCBSA_EINVAL, "%s: scale must be finite, cap finite and not negative", what);
+    if (std::fabs(sc->scale) > 0x1p126f || sc->cap > 0x1p126f)  // times log2(e) they are kept in 32 bits
+        return fail(LCBSA_EINVAL, "%s: scale and cap up to 2^126", what);
     if (sc->cap > 0.f && sc->scale != 0.f && !(std::fabs(sc->scale) <= 0x1p20 * sc->cap && sc->cap <= 0x1p20 * std::fabs(sc->scale)))
         return fail(LCBSA_EINVAL, "%s: cap further than a factor of 2^20 from scale", what);
     if ((sc->cu_q == nullptr) != (sc->cu_k == nullptr)) return fail(LCBSA_EINVAL, "%s: the documents of the queries and of the keys go together", what);

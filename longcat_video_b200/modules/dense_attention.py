@@ -37,6 +37,8 @@ def _shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, sc
         raise ValueError(f"softcap {softcap}: 0 (none) or a positive number")
     if not math.isfinite(scale):
         raise ValueError(f"scale {scale} is not finite")
+    if abs(scale) > 2.0 ** 126 or softcap > 2.0 ** 126:
+        raise ValueError(f"scale {scale}, softcap {softcap}: up to 2^126")
     if softcap and scale and not 2.0 ** -20 <= abs(scale) / softcap <= 2.0 ** 20:
         raise ValueError(f"softcap {softcap}: further than a factor of 2^20 from scale {scale}")
     docs = 1
@@ -78,7 +80,7 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
 
     ``q [B, Hq, Sq, D]``, ``k``, ``v`` ``[B, Hk, Sk, D]``, bf16 or fp16, D 64 or 128, Hq a multiple of Hk (query head h reads key head
     ``h // (Hq // Hk)``), any strides with D contiguous.  ``scale`` defaults to ``D ** -0.5``; ``softcap`` 0 caps nothing,
-    others lie within a factor of 2^20 of ``scale``;
+    others lie within a factor of 2^20 of ``scale``, both up to 2^126;
     ``slopes [Hq]`` (constants) weigh the distance between the query's place among the keys and the key.
 
     Which keys a query sees: all of its batch entry's; with ``k_lens [B]`` the first that many (a padded cache); with ``cu_q``
