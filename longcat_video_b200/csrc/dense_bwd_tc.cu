@@ -17,7 +17,8 @@
 //
 // Hidden values may be anything.  A hidden pair's P and dS are set to zero; in mixed entries a producer looks through the tiles that are
 // summed over, and once S and dP have read them the issuer of the gradient MMAs sets values that are not finite to zero (0 * inf is not 0).  A pair
-// that is seen has its NaN from S and dP; for dV it is the query's delta that says that dO is not finite.
+// that is seen has its NaN from S and dP; for dV a mark in the place of the query's delta (kBadRow) says that dO is not finite.  (delta itself
+// does not: it is the same where dO is finite and a value that the row sees is not, of which dV knows nothing.)
 //
 // Bound by the chain S -> P -> dP -> dS -> product and the operands' way from shared memory; two buffers of S and dP keep two entries in it.  37
 // heads of 4096 tokens, head_dim 128 (ns for 128 x 64 pairs): dQ 650, with a cap 780; dK/dV 880 (1.4 PFLOP/s), with a cap 1040; tensor pipe 59
@@ -693,8 +694,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                             if (kCap) p[k] = __fmul2_rn(p[k], slack);
                             if (mx) {
                                 const float4 d4 = st4[16 + (k >> 1)];
-                                if (!isfinite(k & 1 ? d4.z : d4.x)) w.x = p[k].x = __int_as_float(0x7fc00000);  // dO is not finite
-                                if (!isfinite(k & 1 ? d4.w : d4.y)) w.y = p[k].y = __int_as_float(0x7fc00000);
+                                if (__float_as_uint(k & 1 ? d4.z : d4.x) == kBadRow) w.x = p[k].x = __int_as_float(0x7fc00000);  // dO is not finite
+                                if (__float_as_uint(k & 1 ? d4.w : d4.y) == kBadRow) w.y = p[k].y = __int_as_float(0x7fc00000);
                                 if (key < a.x || key >= a.y) w.x = p[k].x = 0.f;  // last: the slack of a hidden score may be NaN
                                 if (key < d.x || key >= d.y) w.y = p[k].y = 0.f;
                             }

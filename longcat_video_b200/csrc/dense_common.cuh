@@ -20,6 +20,7 @@ constexpr int kDenseCounters = 2;
 constexpr int kDenseUnit = 64;              // rows of a query unit, keys of a key unit
 constexpr int kDenseStats = 2 * kDenseUnit;  // floats of a query unit in the plan of the backward: -lse * log2(e) [64], -delta [64]
 constexpr int kSeenPitch = kDenseUnit + 1;  // int4 of a query unit in the plan
+constexpr uint32_t kBadRow = 0x7fc0dadau;    // a NaN in the place of -delta: the row's dout holds a value that is not finite
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // What a query sees: keys [lo, hi); pos is its position among the keys.
@@ -49,7 +50,8 @@ struct DenseArgs {
     int4* seen;            // [B, units, 65]: lo, hi, pos, 0 of a unit's 64 queries (those behind the last see nothing), then
                            // min lo, max hi over the queries that see a key, max lo, min hi over all of them
     int2* hulls;           // [B, key units]: first and one past the last query that can see a key of the unit (backward)
-    float* stats;          // [B*Hq, units, 2, 64]: -lse * log2(e) and -rowsum(dout * out) of a unit's queries, -inf and 0 behind the last (backward)
+    float* stats;          // [B*Hq, units, 2, 64]: -lse * log2(e) and -rowsum(dout * out) of a unit's queries, -inf and 0 behind the last;
+                           // kBadRow in the place of -delta where dout is not finite (backward)
     float* part;           // sums of dk and dv of parts of a group of heads (backward)
     int* next_item;        // items taken by the persistent kernels, zero when they start
 };

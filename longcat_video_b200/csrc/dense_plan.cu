@@ -84,6 +84,7 @@ __device__ __forceinline__ void stats_cta(const DenseArgs& a, long long cta) {
     const long long r = cta * (128 / kLanes) + threadIdx.x / kLanes;  // (b * Hq + h) * units * 64 + row of the unit: whole CTAs of them
     const int n_u = dense_units(a.Sq);
     float s = 0.f;
+    bool bad = false;
     const long long bh = r / ((long long)n_u * kDenseUnit);
     const int i = (int)(r % ((long long)n_u * kDenseUnit)), b = (int)(bh / a.Hq), h = (int)(bh % a.Hq);
     if (i < a.Sq) {
@@ -91,16 +92,18 @@ __device__ __forceinline__ void stats_cta(const DenseArgs& a, long long cta) {
         const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout.data) + b * a.dout.sb + h * a.dout.sh + i * a.dout.ss + sub * 8);
         uint4 left = make_uint4(0u, 0u, 0u, 0u);
         if (a.rest != nullptr) left = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.rest) + (bh * a.Sq + i) * D + sub * 8);
+        bad = chunk_nonfinite<T>(g);
         const T *op = reinterpret_cast<const T*>(&o), *gp = reinterpret_cast<const T*>(&g), *lp = reinterpret_cast<const T*>(&left);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s = fmaf(DType<T>::to_f32(op[e]) + DType<T>::to_f32(lp[e]), DType<T>::to_f32(gp[e]), s);
     }
 #pragma unroll
     for (int x = kLanes / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    bad = (__ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 31 & ~(kLanes - 1)) & ((1u << kLanes) - 1u)) != 0u;
     if (sub == 0) {
         float* dst = a.stats + r / kDenseUnit * kDenseStats + r % kDenseUnit;
         dst[0] = i < a.Sq ? -(a.lse[bh * a.Sq + i] * kLog2e) : -INFINITY;
-        dst[kDenseUnit] = i < a.Sq ? -s : 0.f;
+        dst[kDenseUnit] = bad ? __uint_as_float(kBadRow) : i < a.Sq ? -s : 0.f;
     }
 }
 

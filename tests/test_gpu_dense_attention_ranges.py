@@ -98,3 +98,40 @@ def test_scales_far_from_their_cap(scale, cap, D, impl):
     assert float((lse.double() - want["lse"]).abs().max()) <= R.SCORE + 1e-5
     for got, x in zip(torch.autograd.grad(out, leaves, dout), ("dq", "dk", "dv")):
         assert R.worst(got, want[x]) <= 1, x
+
+
+# ---- values that are not finite in one operand alone -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+@pytest.mark.parametrize("poison", [math.inf, math.nan])
+def test_values_do_not_reach_their_own_gradient(poison, D, dtype):
+    """dv is P^T dout: infinities and NaN in v, which make outputs and dq of the rows that see them what they are, leave dv alone, in tiles that all
+    rows see and in those that some see."""
+    S = 400
+    q, k, v, dout = _inputs(1, 4, 2, S, S, D, dtype, seed=23)
+    lo, hi, pos = R.runs(1, S, S, True, None, None, None)
+    want = R.attend(q, k, v, lo, hi, pos, 1 / math.sqrt(D), 0.0, None, dout)["dv"]
+    v[0, 1, 40, 5] = v[0, 0, 333, 7] = poison
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = _dense()(*leaves, causal=True)
+    assert not torch.isfinite(out[0, 2, 40:, 5]).any()
+    assert R.worst(torch.autograd.grad(out, leaves, dout)[2], want) <= 1
+
+
+@pytest.mark.parametrize("poison", [math.inf, -math.inf, math.nan])
+def test_a_gradient_that_is_not_finite_stays_with_its_row(poison):
+    """dout of one query of one head, in one dimension: dv of the keys that it sees is not finite there, of all others it is within its bound; dq of
+    the other rows too."""
+    S, D, i, c = 400, 128, 211, 9
+    q, k, v, dout = _inputs(1, 2, 2, S, S, D, torch.bfloat16, seed=24)
+    lo, hi, pos = R.runs(1, S, S, True, None, None, None)
+    want = R.attend(q, k, v, lo, hi, pos, 1 / math.sqrt(D), 0.0, None, dout)
+    dout[0, 1, i, c] = poison
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    dq, _, dv = torch.autograd.grad(_dense()(*leaves, causal=True), leaves, dout)
+    assert not torch.isfinite(dv[0, 1, :i + 1, c]).any()
+    part = lambda x, idx: tuple(t[idx] for t in x)  # noqa: E731
+    assert R.worst(dv[0, 0], part(want["dv"], (0, 0))) <= 1 and R.worst(dv[0, 1, i + 1:], part(want["dv"], (0, 1, slice(i + 1, None)))) <= 1
+    rows = [r for r in range(S) if r != i]
+    assert R.worst(dq[0, 1, rows], part(want["dq"], (0, 1, rows))) <= 1
+    assert not torch.isfinite(dq[0, 1, i]).any()
