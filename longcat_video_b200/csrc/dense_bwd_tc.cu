@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                         }
                     };
                     if (kCap && LCBSA_UNLIKELY(large)) all(true, true);
-                    else if (kBias && both_sides) all(false, true);
+                    else if (kBias && (both_sides || (kCap && mixed))) all(false, true);  // mixed: the way of a tile that a hidden score makes large
                     else all(false, false);
                     if (mixed) {
                         const int lo = min(max(me.see.x - first, 0), 32), hi = min(max(me.see.y - first, 0), 32);  // a run of bits

@@ -155,14 +155,25 @@ __device__ __forceinline__ float2 capped_small(const ScoreShape& f, float2 s, fl
     return x;
 }
 
-// Two scores of any size
+// Two scores of any size.  What a score comes to is a matter of the score alone, to the bit: a small one comes out as from the forms above, so a
+// tile may take this way because of a score that is hidden from a row and change nothing of the row.
+__device__ __forceinline__ float2 capped_large(const ScoreShape& f, float2 s, float2& t) {
+    t = make_float2(2.f * dense_rcp(1.f + dense_ex2(s.x * f.mul_ex)), 2.f * dense_rcp(1.f + dense_ex2(s.y * f.mul_ex)));
+    return __ffma2_rn(t, make_float2(-f.cap2, -f.cap2), make_float2(f.cap2, f.cap2));
+}
+__device__ __forceinline__ float2 capped_pick(const ScoreShape& f, float2 s, float2 small, float2 large) {
+    return make_float2(fabsf(s.x) <= f.s_small ? small.x : large.x, fabsf(s.y) <= f.s_small ? small.y : large.y);
+}
+__device__ __forceinline__ float2 capped_any_plus(const ScoreShape& f, float2 s, float2 c) {
+    float2 t;
+    const float2 large = __fadd2_rn(capped_large(f, s, t), c);
+    return capped_pick(f, s, capped_small_plus(f, __fmul2_rn(s, make_float2(f.unit, f.unit)), c), large);
+}
 __device__ __forceinline__ float2 capped_any(const ScoreShape& f, float2 s, float2& slack) {
-    const float2 t = make_float2(2.f * dense_rcp(1.f + dense_ex2(s.x * f.mul_ex)), 2.f * dense_rcp(1.f + dense_ex2(s.y * f.mul_ex)));
-    const float2 c = make_float2(f.cap2, f.cap2), m = make_float2(-f.cap2, -f.cap2);
-    const float2 small = capped_small_plus(f, __fmul2_rn(s, make_float2(f.unit, f.unit)), make_float2(0.f, 0.f));
-    slack = __fmul2_rn(t, __fadd2_rn(make_float2(2.f, 2.f), make_float2(-t.x, -t.y)));
-    const float2 x = __ffma2_rn(t, m, c);
-    return make_float2(fabsf(s.x) <= f.s_small ? small.x : x.x, fabsf(s.y) <= f.s_small ? small.y : x.y);
+    float2 t, small_slack;
+    const float2 large = capped_large(f, s, t), small = capped_small(f, __fmul2_rn(s, make_float2(f.unit, f.unit)), small_slack);
+    slack = capped_pick(f, s, small_slack, __fmul2_rn(t, __fadd2_rn(make_float2(2.f, 2.f), make_float2(-t.x, -t.y))));
+    return capped_pick(f, s, small, large);
 }
 
 // The bias of n columns whose keys lie on one side of the query, plus a constant: plus - slope |at - j| is a line in the column's number j.

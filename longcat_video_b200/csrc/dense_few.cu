@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(kFewWarps<D> * 32, 2) dense_few_kernel(const _
 #pragma unroll
             for (int nt = 0; nt < kN / 8; ++nt) {
                 const int j = key0 + nt * 8 + 2 * (lane & 3);
-                float2 x = make_float2(s[q][nt][e0], s[q][nt][e0 + 1]), slack;
-                if (kCap) x = capped_any(P.shape, x, slack);
+                float2 x = make_float2(s[q][nt][e0], s[q][nt][e0 + 1]);
+                if (kCap) x = capped_any_plus(P.shape, x, make_float2(0.f, 0.f));
                 else x = make_float2(x.x * P.shape.mul, x.y * P.shape.mul);
                 if (kBias) {
                     x.x = fmaf(-slope[k], fabsf((float)(see[k].z - j)), x.x);

@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
                     const bool both_sides = kBias && __any_sync(0xffffffffu, at > 0.f && at < (float)(kBlk - 1));
                     auto plain = [&](float2 s, float2 c) { return __ffma2_rn(s, make_float2(f.mul, f.mul), c); };
                     auto small = [&](float2 s, float2 c) { return capped_small_plus(f, s, c); };
-                    auto any = [&](float2 s, float2 c) { float2 slack; return __fadd2_rn(capped_any(f, s, slack), c); };
+                    auto any = [&](float2 s, float2 c) { return capped_any_plus(f, s, c); };
                     auto row_max = [&]() {
                         float mx8[8];  // eight chains of eight values, three at a time
 #pragma unroll

@@ -135,3 +135,40 @@ def test_a_gradient_that_is_not_finite_stays_with_its_row(poison):
     rows = [r for r in range(S) if r != i]
     assert R.worst(dq[0, 1, rows], part(want["dq"], (0, 1, rows))) <= 1
     assert not torch.isfinite(dq[0, 1, i]).any()
+
+
+# ---- hidden values under a cap -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("poison", [math.inf, -math.inf, math.nan, 3e4])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("D,Sq,impl", [(128, 6, MMA), (128, 200, MMA), (128, 200, TC), (64, 200, TC)])
+def test_hidden_keys_under_a_cap(D, Sq, impl, slopes, poison):
+    """What keys behind the length hold, numbers far beyond the cap among them, changes not a bit of outputs and gradients."""
+    B, Hq, Hk, Sk = 2, 4, 2, 300
+    q, k, v, dout = _inputs(B, Hq, Hk, Sq, Sk, D, torch.float16, seed=25)
+    lens = torch.tensor([200 + Sq % 7, 61], dtype=torch.int32, device="cuda")
+    kw = dict(causal=True, k_lens=lens, softcap=30.0, slopes=_slopes(Hq) if slopes else None, impl=impl)
+
+    def all_of(k, v):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = _dense()(*leaves, **kw)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+    kp, vp = k.clone(), v.clone()
+    for b in range(B):
+        kp[b, :, int(lens[b]):] = poison
+        vp[b, :, int(lens[b]):] = poison
+    assert all(torch.equal(a, b) for a, b in zip(all_of(kp, vp), all_of(k, v)))
+
+
+@pytest.mark.parametrize("poison", [math.nan, 3e4])
+def test_later_keys_under_a_cap(poison):
+    """What comes behind a query in the order changes not a bit of its output: its neighbours, which see it, may be NaN or at the cap."""
+    S = 300
+    q, k, v, _ = _inputs(1, 4, 2, S, S, 128, torch.float16, seed=26)
+    for slopes in (None, _slopes(4)):
+        call = lambda k, v: _dense()(q, k, v, causal=True, softcap=30.0, slopes=slopes, impl=TC)  # noqa: E731
+        want = call(k, v)
+        kp, vp = k.clone(), v.clone()
+        kp[:, :, 150:152] = poison
+        vp[:, :, 150:152] = poison
+        assert torch.equal(call(kp, vp)[:, :, :150], want[:, :, :150])
