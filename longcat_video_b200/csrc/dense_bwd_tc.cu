@@ -11,6 +11,11 @@
 //   the query units that may see the keys, query head after query head of the group
 //       S = A1 B1^T    dP = A2 B2^T    P, dS in registers, to TMEM in the input type    dQ += dS B1,  or  dV += P^T B2, dK += dS^T B1
 //
+// dS goes into its products without the factor scale, which the fp32 sums get when they are stored: a scale of 1 / sqrt(D) would move it three
+// bits further into the subnormal numbers of fp16 (2048 keys, head_dim 64: dq off by 2.1 % for a dout of 10^-3 with it inside, 0.27 % outside; 0.21 and
+// 0.038 % for 10^-2, 0.030 % for 1 either way).
+// At the other end dS passes 65504 three bits earlier: at values of dout - which have the same limit - of some 10^4.
+//
 // The roles of the warps, the rings and the TMEM columns are those of the block-sparse backward for 128-token blocks (attn_bwd_tc.cu), where
 // they are explained.  What differs: the walks are runs, so no lists are read; an entry is whole (all of its pairs are seen) or mixed, and
 // only mixed ones are masked pair by pair; a query unit brings what its rows see along with its lse and delta.
@@ -100,8 +105,7 @@ struct BwdParams {
     int splits, walk;
     float* part;
     int n_items, wave;
-    float scale, scale_lg;  // log2 of its magnitude
-    float sign;             // of the scale (dQ pass)
+    float scale;
     ScoreShape shape;
 };
 
@@ -568,8 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
             mbar_arrive_elect(bar_a_empty);
             return true;
         };
-        // Two scores -> P, and 1 - tanh^2 with a cap.  c: -lse * log2(e) (dQ pass: and log2 of the scale's magnitude, so that P times
-        // dP - delta is dS), with a bias less the distance times the slope.
+        // Two scores -> P, and 1 - tanh^2 with a cap.  c: -lse * log2(e), with a bias less the distance times the slope.
         auto probs = [&](float2 s, float2 c, bool large, float2& slack) {
             float2 x;
             if (kCap) x = __fadd2_rn(large ? capped_any(P.shape, s, slack) : capped_small(P.shape, s, slack), c);
@@ -589,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                 if (u < P.n_u) {
                     r.see = P.seen[((long long)b * P.n_u + u) * kSeenPitch + i % kBlk];
                     const float* st = P.stats + ((long long)it.bh * P.n_u + u) * kDenseStats + i % kBlk;
-                    r.nl = st[0] + P.scale_lg;
+                    r.nl = st[0];
                     r.nd = st[kBlk];
                 }
                 if (kBias) r.slope2 = __ldg(P.slopes + h) * kLog2e;
@@ -624,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t x[32], out[16];  // S, then dP
-                float2 p[16];      // what dP - delta is multiplied by: P times 1 - tanh^2 and, dK/dV pass, the scale
+                float2 p[16];      // what dP - delta is multiplied by: P times 1 - tanh^2
                 tc_ld32(tmem + C::s(wg) + 32u * half + t_lane, x);
                 tc_wait_ld();
                 if (kMode == 0) {
@@ -690,8 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
                                 else c = __fadd2_rn(c, bias_next(line, k));
                             }
                             float2 w = probs(two(x[2 * k], x[2 * k + 1]), c, lg, slack);
-                            p[k] = __fmul2_rn(w, make_float2(P.scale, P.scale));
-                            if (kCap) p[k] = __fmul2_rn(p[k], slack);
+                            p[k] = kCap ? __fmul2_rn(w, slack) : w;
                             if (mx) {
                                 const float4 d4 = st4[16 + (k >> 1)];
                                 if (__float_as_uint(k & 1 ? d4.z : d4.x) == kBadRow) w.x = p[k].x = __int_as_float(0x7fc00000);  // dO is not finite
@@ -772,9 +774,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_bwd_tc_kernel(const __grid_
 #pragma unroll
                     for (int j = 0; j < 32; ++j) acc[j] = 0u;  // nobody sees these rows, or they see nothing
                 }
-                if (kMode == 0 && P.sign < 0.f) {
+                if (!second) {  // the scale that dS is without
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[j] ^= 0x80000000u;
+                    for (int j = 0; j < 32; ++j) acc[j] = __float_as_uint(__uint_as_float(acc[j]) * P.scale);
                 }
                 if (i >= P.rows || col >= D) continue;
                 if (kMode == 1 && P.splits > 1) {
@@ -895,8 +897,6 @@ cudaError_t passes(const DenseArgs& a, cudaStream_t st, const char** why) {
     P.seen = a.seen; P.hulls = a.hulls; P.stats = a.stats; P.slopes = a.slopes; P.status = a.status;
     P.B = a.B; P.Hq = a.Hq; P.Hk = a.Hk; P.group = a.group; P.n_u = dense_units(a.Sq); P.n_k = dense_units(a.Sk);
     P.scale = a.scale;
-    P.scale_lg = log2f(fabsf(a.scale));  // -inf for 0: dQ is 0
-    P.sign = a.scale < 0.f ? -1.f : 1.f;
     P.shape = score_shape(a.scale, a.cap);
     auto map = [&](CUtensorMap* tm, const View& v, int H, int S, int box, int* fold) {
         if (S == 0 || dense_rows_map(tm, a.dtype, v, a.B, H, S, D, box, fold)) return true;

@@ -172,3 +172,50 @@ def test_later_keys_under_a_cap(poison):
         kp[:, :, 150:152] = poison
         vp[:, :, 150:152] = poison
         assert torch.equal(call(kp, vp)[:, :, :150], want[:, :, :150])
+
+
+# ---- fp16 gradients of small size --------------------------------------------------------------------------------------------------
+
+def test_small_fp16_gradients_are_kept():
+    """256 keys of equal weight (q or k zero), values of +-1, dout 2^-16 in one dimension: dS is +-2^-24 before the factor scale = 1/8, the smallest
+    number that fp16 has, and nothing behind it.  dq and dk are 256 * 2^-27 = 2^-19.  P and dS are off by a few 2^-24 of their size (lse, ex2), so dS
+    rounds to +-2^-24, and the sums are exact but for that: the result is 2^-19, on the grid of fp16."""
+    n, D = 256, 64
+    sign = 1.0 - 2.0 * (torch.arange(n, device="cuda") % 2)
+    zero = lambda: torch.zeros(1, 1, n, D, device="cuda", dtype=torch.float16)  # noqa: E731
+    for side in ("dq", "dk"):
+        q, k, v, dout = zero(), zero(), zero(), zero()
+        v[0, 0, :, 0] = sign.half()
+        dout[..., 0] = 2.0 ** -16
+        (k if side == "dq" else q)[0, 0, :, 3] = sign.half() if side == "dq" else 1.0
+        leaves = [x.requires_grad_() for x in (q, k, v)]
+        dq, dk, _ = torch.autograd.grad(_dense()(*leaves), leaves, dout)
+        want = zero()
+        want[0, 0, :, 3] = 2.0 ** -19 if side == "dq" else (sign * 2.0 ** -19).half()
+        assert torch.equal(dq if side == "dq" else dk, want), side
+
+
+@pytest.mark.parametrize("scale", [None, -0.05])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3])
+@pytest.mark.parametrize("D,heads", [(64, (2, 2)), (128, (8, 2))])
+def test_roundings_of_small_fp16_gradients(D, heads, size, scale):
+    """The root mean square error of dq and dk against that of independent roundings: each dS / scale off by a uniform error of one step of fp16 at its
+    size (step / sqrt(12), 2^-24 at least), times scale and the other operand; the result off by half of its own step.  delta and P, whose errors are
+    2^-20 and less of a dS, have the rest of the factor 1.25 (the two groups of errors, at sizes 1 to 1e-3, are 10^4 numbers and more)."""
+    B, S, (Hq, Hk) = 1, 1500, heads
+    q, k, v, dout = _inputs(B, Hq, Hk, S, S, D, torch.float16, seed=27)
+    dout = (dout.float() * size).half()
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    dq, dk, _ = torch.autograd.grad(_dense()(*leaves, scale=scale), leaves, dout)
+    scale = D ** -0.5 if scale is None else scale
+    step = lambda x: torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -14))) - 10)  # noqa: E731
+    G = Hq // Hk
+    kk, vv = k.double().repeat_interleave(G, 1), v.double().repeat_interleave(G, 1)
+    p = torch.softmax(q.double() @ kk.transpose(-1, -2) * scale, -1)
+    dp = dout.double() @ vv.transpose(-1, -2)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    var = (step(ds) * scale) ** 2 / 12
+    fold = lambda x: x.view(B, Hk, G, S, D).sum(2)  # noqa: E731
+    for got, want, v2 in ((dq, ds @ kk * scale, var @ kk ** 2), (dk, fold(ds.transpose(-1, -2) @ q.double()) * scale, fold(var.transpose(-1, -2) @ q.double() ** 2))):
+        room = 1.25 * (v2 + step(want) ** 2 / 12).mean().sqrt()
+        assert float((got.double() - want).square().mean().sqrt()) <= float(room)
