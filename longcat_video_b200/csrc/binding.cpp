@@ -263,6 +263,12 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
     return wants;
 }
 
+// There is no rule that carries a tangent on: an input that has one is an error, not a result without it.
+void no_tangents(std::initializer_list<const at::Tensor*> ts) {
+    for (const at::Tensor* t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "no forward-mode derivative: an input carries a tangent");
+}
+
 // dense_attention(q, k, v, scale, cap, causal, slopes, cu_q, cu_k, k_lens, prefix, return_lse, impl) -> out or (out, lse)
 PyObject* py_dense_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -272,6 +278,7 @@ PyObject* py_dense_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Scores s{PyFloat_AsDouble(a[3]), PyFloat_AsDouble(a[4]), PyObject_IsTrue(a[5]) == 1, PyLong_AsLongLong(a[12]), maybe(a[6]), maybe(a[7]), maybe(a[8]), maybe(a[9]), maybe(a[10])};
         if (PyErr_Occurred()) return nullptr;
         const bool return_lse = PyObject_IsTrue(a[11]) == 1;
+        no_tangents({&q, &k, &v});
         at::Tensor out, lse;
         if (wants_grad({&q, &k, &v})) {
             const auto r = DenseAttention::apply(q, k, v, s);
@@ -299,6 +306,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const RotaryCall c{static_cast<const uint64_t*>(PyLong_AsVoidPtr(a[1])), (int)PyLong_AsLong(a[2]), PyFloat_AsDouble(a[3]), maybe(a[4]),
                            PyLong_AsLongLong(a[5]), PyObject_IsTrue(a[6]) == 1};
         if (PyErr_Occurred()) return nullptr;
+        for (const at::Tensor& x : xs) no_tangents({&x});
         const bool grad = xs.size() == 2 ? wants_grad({&xs[0], &xs[1]}) : wants_grad({&xs[0]});
         return tuple_of(grad ? Rotary::apply(c, xs[0], xs.size() == 2 ? std::optional<at::Tensor>(xs[1]) : std::nullopt) : rotary_launch(xs, c, false));
     } catch (const LibraryError& e) {

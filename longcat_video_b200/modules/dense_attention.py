@@ -67,6 +67,8 @@ def _shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, sc
             raise ValueError(f"slopes is on {slopes.device}, q on {dev}")
         if slopes.requires_grad and torch.is_grad_enabled():
             raise ValueError("slopes are constants: they have no gradient")
+        if torch.autograd.forward_ad._current_level >= 0 and torch.autograd.forward_ad.unpack_dual(slopes).tangent is not None:
+            raise ValueError("slopes are constants: they carry no tangent")
         slopes = slopes.detach().to(torch.float32).contiguous()
     return scale, softcap, bool(causal), slopes, cu_q, cu_k, k_lens, prefix_lens
 

@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+from longcat_video_b200 import _lib as L
+from longcat_video_b200.modules import rotary_frequencies
 from longcat_video_b200.modules.dense_attention import _shape_of
 from tests.test_dense_attention_args import _desc, _fwd, _scores
 
@@ -24,3 +26,22 @@ def test_scales_that_32_bits_do_not_hold():
         assert rc == -1 and "2^126" in msg
     assert _shape(scale=-2.0 ** 126, softcap=2.0 ** 126)[:2] == (-2.0 ** 126, 2.0 ** 126)
     assert math.isfinite(torch.tensor(2.0 ** 126 * 1.4426950408889634, dtype=torch.float32))
+
+
+def test_tangents_are_refused():
+    """Before a launch, so tensors of the CPU do."""
+    x = torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16)
+    f = rotary_frequencies(64)
+    forward = torch.autograd.forward_ad
+    with forward.dual_level():
+        dual = forward.make_dual(x, torch.ones_like(x))
+        for i in range(3):
+            qkv = [dual if j == i else x for j in range(3)]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                L.binding().dense_attention(*qkv, 0.125, 0.0, False, None, None, None, None, None, False, 0)
+        for xs in ((dual,), (dual, x), (x, dual)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                L.binding().rotary(xs, f.address, f.pairs, f.factor, None, 0, False)
+        with pytest.raises(ValueError, match="tangent"):
+            _shape(slopes=forward.make_dual(torch.ones(2), torch.ones(2)))
+        assert _shape(slopes=torch.ones(2))[3].shape == (2,)

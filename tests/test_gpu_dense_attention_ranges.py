@@ -219,3 +219,22 @@ def test_roundings_of_small_fp16_gradients(D, heads, size, scale):
     for got, want, v2 in ((dq, ds @ kk * scale, var @ kk ** 2), (dk, fold(ds.transpose(-1, -2) @ q.double()) * scale, fold(var.transpose(-1, -2) @ q.double() ** 2))):
         room = 1.25 * (v2 + step(want) ** 2 / 12).mean().sqrt()
         assert float((got.double() - want).square().mean().sqrt()) <= float(room)
+
+
+# ---- forward-mode derivatives ------------------------------------------------------------------------------------------------------
+
+def test_tangents_are_refused():
+    """A tangent that no rule carries on is an error, with and without a backward recorded; outside of its level the call goes through."""
+    from longcat_video_b200.modules import embed_rotary, embed_rotary_qk, rotary_frequencies
+    q, k, v, _ = _inputs(1, 2, 2, 20, 20, 64, torch.bfloat16)
+    f = rotary_frequencies(64)
+    with torch.autograd.forward_ad.dual_level():
+        for grad in (False, True):
+            dual = torch.autograd.forward_ad.make_dual(q.clone().requires_grad_(grad), torch.ones_like(q))
+            for call in (lambda: _dense()(dual, k, v), lambda: _dense()(q, dual, v), lambda: _dense()(q, k, dual), lambda: embed_rotary(dual, f),
+                         lambda: embed_rotary_qk(q, dual, f)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        assert torch.equal(_dense()(q, k, v), _dense()(q, k, v))
