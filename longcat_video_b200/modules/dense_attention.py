@@ -17,14 +17,17 @@ from .. import _lib as L
 
 
 def _numbers(name: str, t: torch.Tensor, device, shapes) -> torch.Tensor:
-    """An int32 tensor of one of the shapes on the call's device, contiguous."""
+    """An int32 tensor of one of the shapes on the call's device, contiguous.  What 32 bits do not hold lies outside of every tensor and becomes the
+    nearest number that they hold."""
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, q on {device}")
     if tuple(t.shape) not in shapes:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {' or '.join(map(str, shapes))}")
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
 
 
 def _shape_of(q, k, causal, softcap, slopes, cu_q, cu_k, k_lens, prefix_lens, scale) -> tuple:

@@ -45,3 +45,17 @@ def test_tangents_are_refused():
         with pytest.raises(ValueError, match="tangent"):
             _shape(slopes=forward.make_dual(torch.ones(2), torch.ones(2)))
         assert _shape(slopes=torch.ones(2))[3].shape == (2,)
+
+
+def test_numbers_that_32_bits_do_not_hold():
+    """Lengths, bounds and prefixes in 64 bits are cut to what 32 hold: far behind the keys stays far behind, far before stays far before."""
+    far = [-2 ** 40, -2 ** 32 + 3, 5, 2 ** 31, 2 ** 32 + 5, 2 ** 62]
+    cut = [-2 ** 31, -2 ** 31, 5, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1]
+    cu_q, cu_k = _shape(cu_q=torch.tensor(far))[4:6]
+    assert cu_q.dtype == torch.int32 and cu_q.tolist() == cut and cu_k.tolist() == cut
+    assert _shape(k_lens=torch.tensor([2 ** 32 + 1, -2 ** 33 + 7]))[6].tolist() == [2 ** 31 - 1, -2 ** 31]
+    assert _shape(causal=True, prefix_lens=torch.tensor([[2 ** 40], [9]]))[7].tolist() == [[2 ** 31 - 1], [9]]
+    same = torch.tensor([0, 4], dtype=torch.int32)
+    assert _shape(cu_q=same)[4] is same
+    strided = torch.arange(6, dtype=torch.int32)[::3]
+    assert _shape(cu_q=strided)[4].tolist() == [0, 3] and _shape(cu_q=strided)[4].is_contiguous()

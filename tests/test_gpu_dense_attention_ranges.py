@@ -238,3 +238,14 @@ def test_tangents_are_refused():
                 with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                     call()
         assert torch.equal(_dense()(q, k, v), _dense()(q, k, v))
+
+
+# ---- numbers that 32 bits do not hold ----------------------------------------------------------------------------------------------
+
+def test_lengths_beyond_32_bits():
+    q, k, v, _ = _inputs(1, 2, 2, 30, 90, 64, torch.bfloat16)
+    far = lambda *x: torch.tensor(x, device="cuda")  # noqa: E731
+    for impl in (TC, MMA):
+        assert torch.equal(_dense()(q, k, v, k_lens=far(2 ** 32 + 5), impl=impl), _dense()(q, k, v, impl=impl))
+        assert torch.equal(_dense()(q, k, v, k_lens=far(-2 ** 33 + 50), impl=impl), torch.zeros_like(q))
+        assert torch.equal(_dense()(q, k, v, causal=True, prefix_lens=far(2 ** 40), impl=impl), _dense()(q, k, v, impl=impl))
