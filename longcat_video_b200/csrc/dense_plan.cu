@@ -67,7 +67,7 @@ __device__ __forceinline__ void plan_cta(const DenseArgs& a, int cta, int b, int
     if (m.causal) {
         const int pre = m.prefix != nullptr ? min(max(__ldg(m.prefix + b * m.prefix_stride + d), 0), a.Sk - k0) : 0;
         const int key = max(k_first, k0);
-        if (key >= k0 + pre) q0 = max(q0, q1 - (k1 - key));
+        if (key >= k0 + pre) q0 = (int)max((long long)q0, (long long)q1 - (k1 - key));  // a bound far before the tensor stays before it
     }
     q0 = min(max(q0, 0), a.Sq);
     a.hulls[(long long)b * n_k + u] = make_int2(q0, min(max(q_end, q0), a.Sq));

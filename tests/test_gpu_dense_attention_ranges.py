@@ -249,3 +249,16 @@ def test_lengths_beyond_32_bits():
         assert torch.equal(_dense()(q, k, v, k_lens=far(2 ** 32 + 5), impl=impl), _dense()(q, k, v, impl=impl))
         assert torch.equal(_dense()(q, k, v, k_lens=far(-2 ** 33 + 50), impl=impl), torch.zeros_like(q))
         assert torch.equal(_dense()(q, k, v, causal=True, prefix_lens=far(2 ** 40), impl=impl), _dense()(q, k, v, impl=impl))
+
+
+def test_a_document_far_before_the_queries():
+    """Its end is the lowest number of 32 bits: nothing of it is in the tensor, and the keys of the document behind it, in the same unit of 64 as its own,
+    have their gradients."""
+    q, k, v, dout = _inputs(1, 2, 2, 600, 400, 64, torch.bfloat16)  # query 210 is the first to see key 10, 264 key 64: units 3 and 4
+    cu_k = torch.tensor([0, 10, 400], dtype=torch.int32, device="cuda")
+
+    def grads(first):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        cu_q = torch.tensor([first, first, 600], dtype=torch.int32, device="cuda")
+        return torch.autograd.grad(_dense()(*leaves, causal=True, cu_q=cu_q, cu_k=cu_k), leaves, dout)
+    assert all(torch.equal(a, b) for a, b in zip(grads(-2 ** 31), grads(0)))
