@@ -652,7 +652,7 @@ int lcbsa_dense_attn_bwd(const LcbsaTensor* q, const LcbsaTensor* k, const Lcbsa
     if (int rc = same_shape("dense_attn_bwd", "dk", dk, k)) return rc;
     if (int rc = same_shape("dense_attn_bwd", "dv", dv, k)) return rc;
     if (reinterpret_cast<uintptr_t>(rest) % 16 != 0) return fail(LCBSA_EINVAL, "dense_attn_bwd: rest not 16-byte aligned");
-    if (!lse && a.B * a.Hq * a.Sq > 0) return fail(LCBSA_EINVAL, "dense_attn_bwd: null lse");
+    if (!lse && a.B > 0 && a.Hq > 0 && a.Sq > 0) return fail(LCBSA_EINVAL, "dense_attn_bwd: null lse");
     if (int rc = dense_workspace("dense_attn_bwd", workspace, workspace_bytes, lcbsa::dense_bwd_workspace_bytes(a))) return rc;
     a.o = view_of(out); a.dout = view_of(dout); a.dq = view_of(dq); a.dk = view_of(dk); a.dv = view_of(dv);
     const char* why = "";

@@ -968,7 +968,7 @@ size_t dense_bwd_workspace_bytes(const DenseArgs& a) {
 }
 
 cudaError_t launch_dense_bwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why) {
-    if (a.B * a.Hq == 0) return cudaSuccess;
+    if (a.B == 0 || a.Hq == 0) return cudaSuccess;
     dense_plan_carve(a, workspace, true);
     a.stats = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + dense_plan_bytes(a, true));
     a.part = a.stats + (size_t)a.B * a.Hq * dense_units(a.Sq) * kDenseStats;

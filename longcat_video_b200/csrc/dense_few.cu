@@ -546,7 +546,7 @@ size_t dense_fwd_workspace_bytes(const DenseArgs& a) {
 }
 
 cudaError_t launch_dense_fwd(DenseArgs a, void* workspace, cudaStream_t st, const char** why) {
-    if (a.B * a.Hq == 0 || a.Sq == 0) return cudaSuccess;
+    if (a.B == 0 || a.Hq == 0 || a.Sq == 0) return cudaSuccess;
     if (!few_queries(a) && a.impl == LCBSA_ATTN_TC && !dense_tc_supported(a)) {
         *why = "the tcgen05 kernel takes at least one query and one key, and tokens a stride apart";
         return cudaErrorInvalidValue;

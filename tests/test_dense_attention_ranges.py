@@ -1,4 +1,5 @@
 """The ends of what dense_attention takes: refusals and conversions on the host, before any launch."""
+import ctypes
 import math
 
 import pytest
@@ -59,3 +60,11 @@ def test_numbers_that_32_bits_do_not_hold():
     assert _shape(cu_q=same)[4] is same
     strided = torch.arange(6, dtype=torch.int32)[::3]
     assert _shape(cu_q=strided)[4].tolist() == [0, 3] and _shape(cu_q=strided)[4].is_contiguous()
+
+
+def test_a_backward_of_many_rows_needs_its_lse():
+    """2^31 rows, a product that is not positive in 32 bits."""
+    q, k = _desc(32768, 1, 65536, 64), _desc(32768, 1, 1, 64)
+    ref = ctypes.byref
+    rc = L.lib().lcbsa_dense_attn_bwd(ref(q), ref(k), ref(k), ref(q), ref(q), ref(_scores()), None, None, ref(q), ref(k), ref(k), None, 0, None)
+    assert rc == -1 and "null lse" in L.lib().lcbsa_last_error().decode()
