@@ -9,6 +9,7 @@ import functools
 import importlib.util
 import os
 import struct
+import sysconfig
 from typing import Sequence
 
 import torch
@@ -133,17 +134,25 @@ def lib() -> ctypes.CDLL:
 _binding = None
 
 
+def binding_path() -> str:
+    """Where ``csrc/binding.cpp`` is built to.  The file is compiled against one torch's C++ classes and one Python's and says so in its name, so
+    that one of another torch is never loaded."""
+    built_for = f"torch{torch.__version__}-{sysconfig.get_config_var('SOABI')}-abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+    return os.path.join(_HERE, "csrc", f"_binding-{built_for}.so")
+
+
 def binding():
-    """The Python functions of ``csrc/binding.cpp``, over the liblcbsa.so next to them; raises if it has not been built."""
+    """The Python functions of ``csrc/binding.cpp``, over the liblcbsa.so next to them; raises if it has not been built for this torch and Python."""
     global _binding
     if _binding is None:
-        path = os.path.join(_HERE, "csrc", "_binding.so")
+        path = binding_path()
         if not os.path.exists(path):
             raise RuntimeError(f"{path} is missing: build it with `python -m longcat_video_b200.build`")
         lib()
         spec = importlib.util.spec_from_file_location("_binding", path)
-        _binding = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(_binding)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _binding = module
     return _binding
 
 

@@ -1,5 +1,5 @@
-"""Build ``liblcbsa.so`` (the CUDA kernels plus the C ABI of ``include/lcbsa.h``) in-tree with nvcc, and ``_binding.so``, the
-Python functions and autograd nodes of ``csrc/binding.cpp``, with g++ against this Python's torch.
+"""Build ``liblcbsa.so`` (the CUDA kernels plus the C ABI of ``include/lcbsa.h``) in-tree with nvcc, and ``_binding-<torch and Python>.so``,
+the Python functions and autograd nodes of ``csrc/binding.cpp``, with g++ against this Python's torch.
 
     python -m longcat_video_b200.build [--force]
 
@@ -16,7 +16,6 @@ import sys
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB = os.path.join(CSRC, "liblcbsa.so")
-BINDING = os.path.join(CSRC, "_binding.so")
 SOURCES = ["api.cu", "pool.cu", "select.cu", "select_gemm.cu", "select_cdf.cu", "attn_mma.cu", "attn_tc.cu", "attn_tc128.cu", "attn_bwd.cu", "attn_bwd_tc.cu", "noalloc.cu", "norm_rope.cu",
            "rotary.cu", "dense_plan.cu", "dense_few.cu", "dense_tc.cu", "dense_bwd_tc.cu"]
 HEADERS = ["common.cuh", "select_common.cuh", "tc_common.cuh", "mma_common.cuh", "dense_common.cuh", os.path.join("..", "..", "include", "lcbsa.h")]
@@ -45,17 +44,20 @@ def _stale() -> bool:
 
 def _build_binding(force: bool) -> None:
     src, header = os.path.join(CSRC, "binding.cpp"), os.path.join(CSRC, "..", "..", "include", "lcbsa.h")
-    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) > max(os.path.getmtime(p) for p in (src, header)):
-        return
     import sysconfig
 
     import torch
+
+    from ._lib import binding_path
+    binding = binding_path()  # another one for another torch or Python
+    if not force and os.path.exists(binding) and os.path.getmtime(binding) > max(os.path.getmtime(p) for p in (src, header)):
+        return
     root = os.path.dirname(torch.__file__)
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
                os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
     lib = os.path.join(root, "lib")
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-isystem{p}" for p in include), src, "-o", BINDING, f"-L{CSRC}", "-l:liblcbsa.so", "-Wl,-rpath,$ORIGIN", f"-L{lib}", "-ltorch",
+           *(f"-isystem{p}" for p in include), src, "-o", binding, f"-L{CSRC}", "-l:liblcbsa.so", "-Wl,-rpath,$ORIGIN", f"-L{lib}", "-ltorch",
            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
