@@ -78,7 +78,7 @@ __device__ __forceinline__ Seen dense_seen(const DenseMask& m, int b, int i, int
         if (d < 0 || d >= m.docs) return Seen{0, 0, 0};  // before the first document or behind the last
         k0 = min(max(__ldg(ck + d), 0), Sk);
         k1 = min(max(__ldg(ck + d + 1), k0), Sk);
-        q1 = __ldg(cq + d + 1);
+        q1 = min(__ldg(cq + d + 1), Sq);
     } else if (m.k_len != nullptr) {
         k1 = min(max(__ldg(m.k_len + b), 0), Sk);
     }

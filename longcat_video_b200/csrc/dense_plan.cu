@@ -58,7 +58,7 @@ __device__ __forceinline__ void plan_cta(const DenseArgs& a, int cta, int b, int
         k0 = min(max(__ldg(ck + d), 0), a.Sk);
         k1 = min(max(__ldg(ck + d + 1), k0), a.Sk);
         q0 = __ldg(cq + d);
-        q1 = __ldg(cq + d + 1);
+        q1 = min(max(__ldg(cq + d + 1), 0), a.Sq);
         q_end = __ldg(cq + d1 + 1);
     } else if (m.k_len != nullptr) {
         k1 = min(max(__ldg(m.k_len + b), 0), a.Sk);
@@ -67,7 +67,7 @@ __device__ __forceinline__ void plan_cta(const DenseArgs& a, int cta, int b, int
     if (m.causal) {
         const int pre = m.prefix != nullptr ? min(max(__ldg(m.prefix + b * m.prefix_stride + d), 0), a.Sk - k0) : 0;
         const int key = max(k_first, k0);
-        if (key >= k0 + pre) q0 = (int)max((long long)q0, (long long)q1 - (k1 - key));  // a bound far before the tensor stays before it
+        if (key >= k0 + pre) q0 = max(q0, q1 - (k1 - key));
     }
     q0 = min(max(q0, 0), a.Sq);
     a.hulls[(long long)b * n_k + u] = make_int2(q0, min(max(q_end, q0), a.Sq));

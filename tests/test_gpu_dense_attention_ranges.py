@@ -262,3 +262,20 @@ def test_a_document_far_before_the_queries():
         cu_q = torch.tensor([first, first, 600], dtype=torch.int32, device="cuda")
         return torch.autograd.grad(_dense()(*leaves, causal=True, cu_q=cu_q, cu_k=cu_k), leaves, dout)
     assert all(torch.equal(a, b) for a, b in zip(grads(-2 ** 31), grads(0)))
+
+
+@pytest.mark.parametrize("impl", [TC, MMA])
+def test_bounds_beyond_the_tensors_under_an_order(impl):
+    """Documents that reach beyond the tensors are cut at their ends before anything is counted from these: the last query there is stands at the last
+    key there is."""
+    q, k, v, dout = _inputs(2, 4, 2, 150, 230, 128, torch.bfloat16, seed=28)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def all_of(cu_q, cu_k, **kw):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = _dense()(*leaves, causal=True, cu_q=ints(*cu_q), cu_k=ints(*cu_k), impl=impl, **kw)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+    for kw in (dict(), dict(slopes=_slopes(4)), dict(prefix_lens=ints(30, 90), softcap=10.0)):
+        want = all_of((0, 60, 150), (0, 100, 230), **kw)
+        for cu_q, cu_k in (((0, 60, 178), (0, 100, 230)), ((-30, 60, 2 ** 31 - 1), (-5, 100, 231)), ((0, 60, 150), (-2 ** 31, 100, 2 ** 31 - 1))):
+            assert all(torch.equal(a, b) for a, b in zip(all_of(cu_q, cu_k, **kw), want))
