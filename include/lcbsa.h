@@ -320,12 +320,13 @@ int lcbsa_norm_rope_jobs(const LcbsaRowJob* jobs, int n_jobs, float eps, void* s
  * Keys and values that no query of a call sees, and those hidden from a query, may hold anything, infinities and NaN included.
  *
  * scale, cap: finite, up to 2^126 in size, cap 0 or within a factor of 2^20 of the size of scale (scale 0: any cap).
- * lse: fp32 dense [B, Hq, Sq], natural log, nullable in the forward.  A row with a NaN or +inf score is NaN, its lse too.
+ * lse: fp32 dense [B, Hq, Sq], natural log, nullable in the forward.  A row with a NaN or +inf score is NaN, its lse too; scores of
+ * -inf weigh nothing, and a row that sees no others comes out as one that sees nothing (its gradients are NaN).
  * rest: nullable, dense [B, Hq, Sq, D] in the type of q: what rounding out to its type left.  A backward that is given it takes
  * rowsum(dout * out) from both, which halves what that sum adds to the error of dq and dk.
  * The workspace (lcbsa_dense_attn_workspace_bytes, 256-byte aligned) belongs to one call until its kernels have run.
  * The backward takes the forward's out and lse and writes every row of dq, dk and dv; no atomics, so two calls give the same
- * bits; the slopes are constants.
+ * bits; the slopes are constants, of any sign.
  */
 typedef struct LcbsaScores {
     float scale, cap;
@@ -347,7 +348,8 @@ int lcbsa_dense_attn_bwd(const LcbsaTensor* q, const LcbsaTensor* k, const Lcbsa
  * Rotary positions along one axis (the 3-D form over a latent grid is lcbsa_norm_rope) for one or two tensors [B, H_i, S, D] that share
  * dtype, batch, S and D: q and k of a layer.  The first 2 * pairs dimensions turn, the others are copied; pairs are (2p, 2p + 1) with
  * interleaved, else (p, p + pairs).  Pair p turns by position * turns[p] / 2^64 turns and is multiplied by factor; inverse turns the other way
- * (the gradient).  positions: int32 or int64 (pos_bits) with the given strides, or null: offset + index of the token; any value.
+ * (the gradient).  positions: int32 or int64 (pos_bits) with the given strides, or null: offset + index of the token; of any
+ * sign, up to 2^40 in size without a loss (beyond, an angle is off by |position| * 2^-65 turns).
  * bf16 or fp16, head_dim a multiple of 8, pairs a multiple of 8 up to 128.  Outputs overlap neither the inputs nor each other.
  */
 int lcbsa_rotary(const LcbsaTensor* x, const LcbsaTensor* out, int n, const uint64_t* turns, int pairs, int interleaved, int inverse,

@@ -449,7 +449,10 @@ __global__ void __launch_bounds__(128) dense_combine_kernel(const __grid_constan
     write_row<T, kPer>(a, bh / a.Hk, bh % a.Hk, (int)(gr % P.rows), lane * kPer, acc, l, m, D, lane == 0);
 }
 
-// How the keys are shared out.
+// How the keys are shared out.  A cluster of CTAs for each 16 or 32 rows, as large as it takes for one CTA an SM, if there are keys for all of them; and
+// larger where a CTA still has 64 rounds or more (GPU alone, without / with that second step: 32 caches of 32768 keys, 8 heads of 128, 652 / 614
+// us, their lengths between a quarter and the whole 473 / 383; 24 ragged ones 404 / 305; 40 ragged ones of 20000 keys, 4 heads, 225 / 170; 16 heads of 64, 32 of
+// 16384 keys, 322 / 326, ragged 227 / 211; 100 of 8192 keys, 8 heads, 481 / 487, ragged 338 / 326).
 void few_plan(const DenseArgs& a, FewParams& P) {
     const int kStep = few_step(a.D);
     P.rows = a.group * a.Sq;

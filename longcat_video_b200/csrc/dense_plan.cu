@@ -3,8 +3,8 @@
 // What every query sees, in the order of the queries; per unit of 64 queries the union of the runs of its rows (min lo, max hi) and the
 // run that all see (max lo, min hi); per unit of 64 keys the first and the last query that can see one of them, from the
 // documents at its two ends.  A warp takes a query unit, a thread of the CTAs behind them a key unit.  The backward's row sums need none of it
-// and ride in the same launch.  Bound by HBM where the row sums are many: 37 heads of 2048 rows 14 us, half of the DRAM rate (three streams of 16 bytes
-// a thread, one row per eight or sixteen lanes).
+// and ride in the same launch.  Bound by issue slots where the row sums are many: 37 heads of 2048 rows 15.6 us, 74 % of them busy, DRAM 46 % (three streams
+// of 16 bytes a thread, one row per eight or sixteen lanes).
 #include "dense_common.cuh"
 
 namespace lcbsa {

@@ -15,9 +15,10 @@
 // mixed, and only mixed units are masked element by element; heads share keys; scores are capped and biased on the arithmetic pipes
 // (five operations per pair of scores for a cap, one for a bias: see ScoreShape and BiasLine).
 //
-// Bound by the softmax warps: 8192 exponentials of a unit take 512 of the 1024 cycles that its two products take, and the
-// warps that compute them wait for each other's S and PV.  37 heads of 4096 tokens, head_dim 128: 540 ns a unit (1.1 PFLOP/s), 690 with a cap, 630
-// with a bias, 760 with both; at 37 x 2048 under the profiler the tensor pipe is 47 % busy, 35 % with a cap, issue slots 43 and 45 %.  Every eighth
+// Bound by the latency of a unit's chain S -> registers -> exponentials -> P -> PV with two softmax warps on a scheduler, not by a pipe: the two
+// products of a unit take 512 cycles of the tensor pipe and its 8192 exponentials 512 of the special functions', and a unit takes 1120 (37 heads of
+// 2048 tokens, 128 units an SM: 144 000 cycles).  37 heads of 4096 tokens, head_dim 128: 540 ns a unit (1.1 PFLOP/s), 690 with a cap, 630
+// with a bias, 760 with both; at 37 x 2048 under the profiler the tensor pipe is 46 % busy, 35 % with a cap, issue slots 43 and 45 %.  Every eighth
 // pair of exponentials on the arithmetic pipes instead (a polynomial of degree 4): 455 us in the place of 447 at head_dim 128, 412 of 434 at 64;
 // every fourth 471 and 413: not worth a second kind.
 //

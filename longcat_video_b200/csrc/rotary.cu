@@ -6,8 +6,9 @@
 // element once and writes it once: bound by HBM (2 bytes in, 2 bytes out per element).
 //
 // The angle is kept as a fraction of a turn in 64-bit fixed point: frequency = F / 2^64 turns per position, and position * F modulo 2^64
-// is the fraction, exact for every position there is, where position * frequency in fp32 is off by 0.03 radians at position 10^6.
-// Its upper 32 bits, rounded to 24, go to sincospif: off by 2^-24 of half a turn at most.  No table: the frequencies are an argument
+// is the fraction, with no rounding but F's own, where position * frequency in fp32 is off by 0.03 radians at position 10^6.
+// Its upper 32 bits, rounded to 24, go to sincospif: off by 2^-24 of half a turn at most.  F is off by up to 2^-65 turns, which makes 2^-25 of a turn,
+// as much as that, at position 2^40 and doubles with every power of two beyond.  No table: the frequencies are an argument
 // of the launch, so a call reads nothing but its rows and its positions.
 //
 // A thread owns one 16-byte vector of a token (half layout: the two vectors that its eight pairs lie in) and walks over a group

@@ -2,7 +2,7 @@
 
 What stands beside the block-sparse attention of the DiT: its cross-attention from the video tokens to packed prompts
 (``MultiHeadCrossAttention`` with ``kv_seqlen``, longcat_video/modules/attention.py:184-260, a document mask), its
-self-attention with block sparsity off (attention.py:67-104), a text encoder whose scores are biased by distance, an
+self-attention with block sparsity off (attention.py:67-104), a text encoder whose scores fall off in a line with the distance, an
 autoregressive model that shares the GPU.  Forward, backward, and a form for a few tokens of every sequence behind a long cache.
 All arithmetic is in liblcbsa.so (``lcbsa_dense_attn_fwd`` / ``_bwd``), which ``csrc/binding.cpp`` calls; there is no CPU path.
 """
@@ -86,16 +86,20 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
     ``q [B, Hq, Sq, D]``, ``k``, ``v`` ``[B, Hk, Sk, D]``, bf16 or fp16, D 64 or 128, Hq a multiple of Hk (query head h reads key head
     ``h // (Hq // Hk)``), any strides with D contiguous.  ``scale`` defaults to ``D ** -0.5``; ``softcap`` 0 caps nothing,
     others lie within a factor of 2^20 of ``scale``, both up to 2^126;
-    ``slopes [Hq]`` (constants) weigh the distance between the query's place among the keys and the key.
+    ``slopes [Hq]`` (constants, of any sign) weigh the distance between the query's place among the keys and the key: a line in the distance, no
+    table over it.
 
     Which keys a query sees: all of its batch entry's; with ``k_lens [B]`` the first that many (a padded cache); with ``cu_q``
     (``[docs + 1]`` for all entries or ``[B, docs + 1]``, the first token of every document and the end of the last) and ``cu_k`` (default
     ``cu_q``) those of its own document, none if it belongs to none.  The last query of a document (of an entry) stands at its last key;
     ``causal`` hides the keys behind a query's place, except the first ``prefix_lens`` (``[docs]`` or ``[B, docs]``, docs 1 without
     ``cu_q``) of the document.  These numbers stay on the GPU: nothing is read back, and a captured call replays with what they then
-    hold.  A query that sees nothing gets 0 (``lse`` -inf).  What is hidden may hold anything, infinities and NaN included.
+    hold.  A query that sees nothing gets 0 (``lse`` -inf).  What is hidden may hold anything, infinities and NaN included.  Bounds in 64 bits are
+    cut to 32.
 
     ``impl`` names the forward kernel (``ATTN_TC``: tcgen05, ``ATTN_MMA``: the one for few queries) where the choice by size is not wanted.
+
+    A call that is recorded for a backward keeps its operands, ``out``, ``lse`` and one more tensor of the size of ``out``: what rounding left of it.
 
     Returns ``out [B, Hq, Sq, D]``, with ``return_lse`` also the fp32 ``lse [B, Hq, Sq]`` (no gradient runs through it)."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda):

@@ -1,8 +1,8 @@
 """Rotary positions along one axis: interleaved and half layouts, part of the head, frequencies scaled for long contexts.
 
 The 1-D counterpart of the rotary embedding over a latent grid (``rope_3d.py``, longcat_video/modules/rope_3d.py:60-120), for q
-and k of a text model in front of ``dense_attention``.  The angles are exact for every position (64-bit fixed-point turns
-inside the kernel, see ``csrc/rotary.cu``).  All arithmetic on q and k is in liblcbsa.so (``lcbsa_rotary``); there is no CPU path.
+and k of a text model in front of ``dense_attention``.  The angles are right to 2^-24 of half a turn up to positions of 2^40 (64-bit
+fixed-point turns inside the kernel, see ``csrc/rotary.cu``).  All arithmetic on q and k is in liblcbsa.so (``lcbsa_rotary``); there is no CPU path.
 """
 from __future__ import annotations
 
@@ -124,7 +124,8 @@ def embed_rotary(x: torch.Tensor, freqs: RotaryFrequencies, positions: Optional[
                  interleaved: bool = False) -> torch.Tensor:
     """The rows of ``x [B, H, S, D]`` (bf16 or fp16, any strides with D contiguous, D a multiple of 8) with the first ``2 * freqs.pairs``
     dimensions turned by their positions: pairs ``(2p, 2p + 1)`` if ``interleaved``, else ``(p, p + pairs)``; the rest of the head is
-    copied.  ``positions``: int32 or int64 ``[S]`` or ``[B, S]`` on the GPU, any values; without them token s stands at ``offset + s``."""
+    copied.  ``positions``: int32 or int64 ``[S]`` or ``[B, S]`` on the GPU, of any sign, the angles of those beyond 2^40 in size off by
+    ``|position| * 2^-65`` turns; without them token s stands at ``offset + s``."""
     return _embed((x,), freqs, positions, offset, interleaved)[0]
 
 
